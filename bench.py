@@ -245,9 +245,9 @@ def make_host_table(V, Fdim, rank, local_rank, world, dev, tag):
         path = None
     registered = False
     try:
-        rc = torch.cuda.cudart().cudaHostRegister(tab.data_ptr(), tab.numel() * 4, 0)
-        registered = int(rc) == 0
-        log(f"[bench] rank {rank}: hipHostRegister rc={rc}")
+        from pagraph_amd import _lib as L
+        registered = L.host_register(tab.data_ptr(), tab.numel() * 4)
+        log(f"[bench] rank {rank}: host table {'registered' if registered else 'not registered (refused)'}")
     except Exception as e:  # staged mode works from unpinned memory too
         log(f"[bench] rank {rank}: host register unavailable ({e})")
     return tab, registered

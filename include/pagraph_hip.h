@@ -71,6 +71,9 @@ typedef struct pg_tape pg_tape_t;
 int pg_tape_from_graph(void* hip_graph, pg_tape_t** out, int32_t* n_kernels, int32_t* n_other);
 int pg_tape_launch(const pg_tape_t* tape, pg_stream_t stream);
 int pg_tape_destroy(pg_tape_t* tape);
+/* Page-locks `bytes` bytes of existing host memory so that the device may address it (hipHostRegister). A machine that does not
+ * allow it answers PG_ERR_HIP; no HIP error is left behind for the next call to report.                                       */
+int pg_host_register(void* host, int64_t bytes);
 /* number of CUs of the current device, or <0 when no HIP device is visible */
 int pg_device_cu_count(void);
 

@@ -148,6 +148,7 @@ _SIGS = {
     "pg_bounds_enabled": (ctypes.c_int, []),
     "pg_bounds_region": (ctypes.c_int, [vp, c_i64]),
     "pg_bounds_report": (ctypes.c_int, [ctypes.POINTER(c_u64), ctypes.c_char_p, c_i32, c_i32]),
+    "pg_host_register": (ctypes.c_int, [vp, c_i64]),
     "pg_device_cu_count": (ctypes.c_int, []),
     "pg_batch_prepare": (ctypes.c_int, [ctypes.POINTER(PgBatchPlan), c_u64]),
     "pg_tape_from_graph": (ctypes.c_int, [vp, ctypes.POINTER(vp), ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]),
@@ -260,6 +261,11 @@ def load():
 _K_NAMES = ("?", "k_spmm_fwd_rows(_w)", "k_compose_edge_slots", "k_sx (sample)", "k_sx (relabel)", "k_bm_rank", "k_t_keys",
             "k_t_block", "k_split / k_slots_full", "k_gather", "k_gather_labels", "k_linear_fwd<ROWS>", "k_linear_bwd_w<ROWS>",
             "k_gcn_head", "k_spmm_bwd_gather", "k_spmm_fwd(_drop)", "k_spmm_bwd", "k_scatter")
+
+
+def host_register(ptr, nbytes):
+    """page-lock existing host memory for the device; False where the machine refuses (no HIP error stays behind)"""
+    return load().pg_host_register(ctypes.c_void_p(ptr), int(nbytes)) == 0
 
 
 def note(t):

@@ -173,6 +173,14 @@ int pg_bounds_report(uint64_t* rec, char* unit, int32_t unit_len, int32_t reset)
 #endif
 }
 
+int pg_host_register(void* host, int64_t bytes) {
+  if (!host || bytes <= 0) return PG_ERR_INVALID;
+  const hipError_t e = hipHostRegister(host, (size_t)bytes, hipHostRegisterDefault);
+  if (e == hipSuccess) return PG_OK;
+  (void)hipGetLastError();      // the runtime keeps the refusal as its last error: the next launch's check would report it
+  return pg::hip_fail(e);
+}
+
 int pg_device_cu_count(void) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return -1;

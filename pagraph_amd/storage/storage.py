@@ -60,7 +60,7 @@ def huge_page_tensor(shape, dtype=torch.float32, register=True):
     if register and torch.cuda.is_available() and n:
         try:
             ptr = t.data_ptr()
-            ok = int(torch.cuda.cudart().cudaHostRegister(ptr, n * itemsize, 0)) == 0
+            ok = L.host_register(ptr, n * itemsize)
             if ok:
                 weakref.finalize(arr, _unregister, ptr)          # before the mapping goes
         except Exception:
@@ -182,7 +182,7 @@ class HostFeatureStore:
                 ok = False
                 if register and torch.cuda.is_available():
                     try:
-                        ok = int(torch.cuda.cudart().cudaHostRegister(t.data_ptr(), t.numel() * 4, 0)) == 0
+                        ok = L.host_register(t.data_ptr(), t.numel() * 4)
                     except Exception:
                         ok = False
                 seen[t.data_ptr()] = ok
