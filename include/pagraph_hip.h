@@ -579,6 +579,87 @@ int pg_xent_fwd(const float* logits, int32_t stride, const int64_t* labels, int6
 int pg_xent_bwd(const float* dlogits, int32_t d_stride, int64_t n, int32_t C, const float* meta,
                 const float* grad_out, float* gx, int32_t gx_stride, pg_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of a model's dense tail. Rows are fp32, bf16 or fp16 with fp32 arithmetic and one rounding per stored element; row
+ * strides are in elements (an input's may be 0: one row for all), the columns of a row are contiguous, any alignment of whole
+ * elements. n == 0 is allowed.                                                                     */
+#define PG_DTYPE_F32 0
+#define PG_DTYPE_BF16 1
+#define PG_DTYPE_F16 2
+/* y = dropout(x) with pg_dropout_t's mask (row r of x draws what pg_spmm_fwd_drop draws for source row r), which is not stored:
+ * the gradient is the same call on gy. y may be x. n < 2^32, d < 2^31; drop->threshold in [1, 65535].
+ * step_used (device, may be NULL) receives the step the mask was drawn with: hand it to the gradient's call as drop->step, so that
+ * a counter the caller has advanced in between does not change the mask.                                                      */
+int pg_dropout_apply(const void* x, int64_t x_stride, void* y, int64_t y_stride, int64_t n, int64_t d, int32_t dtype,
+                     const pg_dropout_t* drop, uint64_t* step_used, pg_stream_t stream);
+/* Layer norm over the columns: y = (s - mean) * rstd * weight + bias, rstd = 1 / sqrt(biased variance + eps).
+ * forward:  s = x, or with `residual`: s = round(dropout(x) + residual), written to `sum`. has_drop needs a residual (use
+ *           pg_dropout_apply otherwise). mean / rstd [n] fp32: both or neither (no gradient wanted). step_used: as above.
+ * backward: `sum` = the rows that were normalised (x without a residual), gy and optionally gsum (gradient of the handed-on sum):
+ *           ds = rstd (gh - mean(gh) - xh mean(gh xh)) + gsum with gh = gy weight; dres = ds, dx = dropout's gradient of ds; dw, db
+ *           summed over the rows in a fixed order through partials (pg_layer_norm_scratch(n, d) floats). Each of dx, dres, dw, db
+ *           may be NULL. n == 0 writes zeros to dw, db.
+ * weight / bias (either may be NULL: 1 / 0) and dw / db are of param_dtype: dtype's or PG_DTYPE_F32. d <= PG_NORM_MAX_COLUMNS
+ * (a row lives in one workgroup's registers; wider: PG_ERR_UNSUPPORTED).                                                      */
+#define PG_NORM_MAX_COLUMNS 32768
+typedef struct pg_norm_desc {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  const void* bias;
+  void* sum;
+  void* y;
+  float* mean;
+  float* rstd;
+  const void* gy;
+  const void* gsum;
+  void* dx;
+  void* dres;
+  void* dw;
+  void* db;
+  float* partials;
+  uint64_t* step_used;
+  int64_t n, d, x_stride, residual_stride, sum_stride, y_stride, gy_stride, gsum_stride, dx_stride, dres_stride;
+  int32_t dtype, param_dtype;
+  float eps;
+  int32_t has_drop;
+  pg_dropout_t drop;
+} pg_norm_desc_t;
+int pg_layer_norm_fwd(const pg_norm_desc_t* desc, pg_stream_t stream);
+int64_t pg_layer_norm_scratch(int64_t n, int64_t d);
+int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
+/* CrossEntropyLoss(h W^T + bias, labels) for any number of classes without the logits [n, C] in memory (a wide head's counterpart
+ * of pg_head + pg_xent_*): h [n, K], W [C, K], bias [C] or NULL, all of `dtype`. Rows whose label is ignore_index or outside
+ * [0, C) are not counted, have loss 0 and gradient 0, and do not enter dW / db whatever h holds there.
+ * forward:  lse [n], flag [n] (1: counted), row_loss [n], meta[4] = {mean loss (nan when no row counts), 1 / #counted rows (0),
+ *           sum, unused}.
+ * backward: given the forward's lse, flag, meta and grad = d objective / d loss (device fp32: one value for PG_XENT_MEAN / _SUM,
+ *           [n] with grad_stride for PG_XENT_NONE): dh [n, K], dW [C, K], db [C], dense, each may be NULL. n >= 1.
+ * scratch: pg_linear_xent_scratch(n, K, C, dtype, backward) bytes (negative: the sizes are refused). Deterministic.           */
+#define PG_XENT_MEAN 0
+#define PG_XENT_SUM 1
+#define PG_XENT_NONE 2
+typedef struct pg_linear_xent_desc {
+  const void* h;
+  const void* W;
+  const void* bias;
+  const int64_t* labels;
+  float* lse;
+  float* flag;
+  float* row_loss;
+  float* meta;
+  const float* grad;
+  void* dh;
+  void* dW;
+  void* db;
+  void* scratch;
+  int64_t n, K, C, h_stride, w_stride, grad_stride, ignore_index;
+  int32_t dtype, reduction;
+} pg_linear_xent_desc_t;
+int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, int32_t backward);
+int pg_linear_xent_fwd(const pg_linear_xent_desc_t* desc, pg_stream_t stream);
+int pg_linear_xent_bwd(const pg_linear_xent_desc_t* desc, pg_stream_t stream);
+
 /* Output head of the sampled GCN in one pass (pg_head.hip): the last block's aggregation with the model's
  * dropout (gcn_nssc.py:66-74), the output NodeUpdate z = W agg + b (gcn_nssc.py:18,58: no activation), the
  * CrossEntropyLoss of pa_gcn.py:80,101-104 and their gradients. h [n_src, K] (K <= 64), W [C, K] (C <= 64).

@@ -27,6 +27,9 @@ PG_ADAM_FULL, PG_ADAM_REDUCE_ONLY = 0, 1
 PG_REDUCE_MEAN = 0
 PG_REDUCE_SUM = 1
 PG_REDUCE_MAX = 2
+PG_DTYPE_F32, PG_DTYPE_BF16, PG_DTYPE_F16 = 0, 1, 2
+PG_XENT_MEAN, PG_XENT_SUM, PG_XENT_NONE = 0, 1, 2
+PG_NORM_MAX_COLUMNS = 32768
 PG_PROF_END0, PG_PROF_SHARDS, PG_PROF_SHARD_STRIDE = 16, 16, 16      # pg_spmm_fwd_rows' self-timing ring (include/pagraph_hip.h)
 PG_PROF_WORDS = PG_PROF_END0 + PG_PROF_SHARDS * PG_PROF_SHARD_STRIDE
 
@@ -104,6 +107,20 @@ class PgHeadDesc(ctypes.Structure):
                 ("reduce", c_i32), ("flags", c_i32), ("has_drop", c_i32), ("drop", PgDropout), ("logits", vp), ("dagg", vp),
                 ("partials", vp), ("dW", vp), ("db_loss", vp), ("h_self", vp), ("W_self", vp), ("bias_self", vp), ("dself", vp),
                 ("hs_stride", c_i32), ("Ks", c_i32)]
+
+
+class PgNormDesc(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("x", "residual", "weight", "bias", "sum", "y", "mean", "rstd", "gy", "gsum", "dx", "dres", "dw", "db",
+                                  "partials", "step_used")] + \
+               [(n, c_i64) for n in ("n", "d", "x_stride", "residual_stride", "sum_stride", "y_stride", "gy_stride", "gsum_stride",
+                                     "dx_stride", "dres_stride")] + \
+               [("dtype", c_i32), ("param_dtype", c_i32), ("eps", ctypes.c_float), ("has_drop", c_i32), ("drop", PgDropout)]
+
+
+class PgLinearXentDesc(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("h", "W", "bias", "labels", "lse", "flag", "row_loss", "meta", "grad", "dh", "dW", "db", "scratch")] + \
+               [(n, c_i64) for n in ("n", "K", "C", "h_stride", "w_stride", "grad_stride", "ignore_index")] + \
+               [("dtype", c_i32), ("reduction", c_i32)]
 
 
 class PgBatchEarly(ctypes.Structure):
@@ -211,6 +228,13 @@ _SIGS = {
     "pg_linear_bwd_w": (ctypes.c_int, [ctypes.POINTER(PgLinearBwdDesc), vp]),
     "pg_xent_fwd": (ctypes.c_int, [vp, c_i32, vp, c_i64, c_i32, c_i64, vp, c_i32, vp, vp, vp]),
     "pg_xent_bwd": (ctypes.c_int, [vp, c_i32, c_i64, c_i32, vp, vp, vp, c_i32, vp]),
+    "pg_dropout_apply": (ctypes.c_int, [vp, c_i64, vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(PgDropout), vp, vp]),
+    "pg_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(PgNormDesc), vp]),
+    "pg_layer_norm_scratch": (c_i64, [c_i64, c_i64]),
+    "pg_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(PgNormDesc), vp]),
+    "pg_linear_xent_scratch": (c_i64, [c_i64, c_i64, c_i64, c_i32, c_i32]),
+    "pg_linear_xent_fwd": (ctypes.c_int, [ctypes.POINTER(PgLinearXentDesc), vp]),
+    "pg_linear_xent_bwd": (ctypes.c_int, [ctypes.POINTER(PgLinearXentDesc), vp]),
     "pg_gcn_head_scratch": (c_i64, [c_i64, c_i32, c_i32]),
     "pg_gcn_head_row_len": (c_i32, [c_i32, c_i32]),
     "pg_head": (ctypes.c_int, [ctypes.POINTER(PgHeadDesc), vp]),
