@@ -856,11 +856,33 @@ def gcn_head(indptr, src, h, linear, labels, n_valid, grad_seed=None, ignore_ind
 
 
 # ---- the dense tail of a model: dropout, layer norm with its residual, the loss of a wide class head -------------------------
+# A call costs the host more than most of these kernels cost the card, and a backward pass runs on autograd's own thread: what
+# stands between the arguments and the launch is kept short (descriptors filled positionally, no device switch where none is due:
+# 149 -> 85 us for a forward and backward pass of ops.dropout on small rows, 31 us of them autograd's own).
 _DTYPES = {torch.float32: L.PG_DTYPE_F32, torch.bfloat16: L.PG_DTYPE_BF16, torch.float16: L.PG_DTYPE_F16}
+
+
+def _enqueue(name, device, *args):
+    """one library call on `device`'s current stream, which becomes its last argument"""
+    fn = getattr(L.load(), name)
+    at = device.index
+    if torch._C._cuda_getDevice() == at:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(at))
+    if rc:
+        L.check(rc, name)
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _rows_of(x):
     """x [..., d] as [n, d] with contiguous columns and a row stride the kernels take (0: one row for all, or >= d)"""
+    if x.dim() == 2 and x.is_contiguous():
+        return x
     x = x.reshape(-1, x.size(-1))
     if (x.stride(1) != 1 and x.size(1) > 1) or (x.size(0) > 1 and x.stride(0) != 0 and x.stride(0) < x.size(1)):
         x = x.contiguous()
@@ -871,27 +893,37 @@ def _row_stride(x):
     return x.stride(0) if x.size(0) > 1 else x.size(1)
 
 
+def _like(rows, shape):
+    return rows if rows.shape == shape else rows.view(shape)
+
+
 def _need_rows(name, x):
     if not x.is_cuda or x.dtype not in _DTYPES or x.dim() < 1 or x.size(-1) == 0:
         raise L.PgError(f"{name} needs fp32, bf16 or fp16 CUDA rows [..., d] with d >= 1 (no CPU fallback)")
 
 
-def _need_same_device(name, x, **others):
-    for what, t in others.items():
-        if t is not None and t.device != x.device:
-            raise L.PgError(f"{name}: {what} is on {t.device}, the rows on {x.device}")
+def _need_device(name, x, what, t):
+    if t is not None and t.device != x.device:
+        raise L.PgError(f"{name}: {what} is on {t.device}, the rows on {x.device}")
 
 
 def _need_spec(name, x, spec):
     if spec.step is not None:
-        _need_same_device(name, x, **{"the dropout's step": spec.step})
+        _need_device(name, x, "the dropout's step", spec.step)
         if spec.step.dtype != torch.int64 or spec.step.numel() != 1:
             raise L.PgError(f"{name}: the dropout's step must be an int64 device tensor of one element")
 
 
-def _drop_again(spec, step_used):
-    """the forward's mask for its gradient: the step is the one the forward's launch noted, not what the counter holds by now"""
-    return L.PgDropout(spec.threshold, spec.tag, spec.seed, L.ptr(step_used), spec.step_value)
+def _once(name):
+    """their backward passes are kernels: a graph of a gradient (create_graph=True) would silently lack them"""
+    if torch.is_grad_enabled():
+        raise L.PgError(f"{name}: a gradient's own graph (create_graph=True) is not supported")
+
+
+def _drop_struct(spec, step_used=None):
+    """the mask's parameters; for a gradient the step is the one the forward's launch noted, not what the counter holds by now"""
+    step = spec.step.data_ptr() if step_used is None and spec.step is not None else step_used
+    return L.PgDropout(spec.threshold, spec.tag, spec.seed, step, spec.step_value)
 
 
 class _Dropout(torch.autograd.Function):
@@ -900,23 +932,19 @@ class _Dropout(torch.autograd.Function):
         rows = _rows_of(x)
         y = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
         used = torch.empty(1, dtype=torch.int64, device=x.device) if spec.step is not None and ctx.needs_input_grad[0] else None
-        _Dropout.launch(rows, y, spec.struct(), used)
+        _enqueue("pg_dropout_apply", x.device, rows.data_ptr(), _row_stride(rows), y.data_ptr(), rows.size(1), rows.size(0), rows.size(1),
+                 _DTYPES[x.dtype], _drop_struct(spec), _addr(used))
         ctx.spec, ctx.used = spec, used
-        return y.view(x.shape)
+        return _like(y, x.shape)
 
     @staticmethod
-    def launch(x, y, struct, used=None):
-        with torch.cuda.device(x.device):
-            L.check(L.load().pg_dropout_apply(L.ptr(x), _row_stride(x), L.ptr(y), _row_stride(y), x.size(0), x.size(1), _DTYPES[x.dtype],
-                                              ctypes.byref(struct), L.ptr(used), L.stream_ptr()), "pg_dropout_apply")
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _once("dropout")
         rows = _rows_of(gy)
         gx = torch.empty(rows.shape, dtype=gy.dtype, device=gy.device)
-        _Dropout.launch(rows, gx, _drop_again(ctx.spec, ctx.used))
-        return gx.view(gy.shape), None
+        _enqueue("pg_dropout_apply", gy.device, rows.data_ptr(), _row_stride(rows), gx.data_ptr(), rows.size(1), rows.size(0), rows.size(1),
+                 _DTYPES[gy.dtype], _drop_struct(ctx.spec, _addr(ctx.used)), None)
+        return _like(gx, gy.shape), None
 
 
 def dropout(x, spec):
@@ -934,88 +962,67 @@ def dropout(x, spec):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps, spec):
-        lib = L.load()
         rows = _rows_of(x)
         n, d = rows.shape
         res = _rows_of(residual) if residual is not None else None
-        y = torch.empty((n, d), dtype=x.dtype, device=x.device)
-        total = torch.empty((n, d), dtype=x.dtype, device=x.device) if res is not None else None
+        dev, t = x.device, x.dtype
+        y = torch.empty((n, d), dtype=t, device=dev)
+        total = torch.empty((n, d), dtype=t, device=dev) if res is not None else None
         # mean | rstd | the step the mask was drawn with
-        stats = torch.empty(2 * n + 2, dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad[:4]) else None
-        a = _LayerNorm.desc(rows, weight, bias, eps)
-        a.x, a.x_stride = L.ptr(rows).value, _row_stride(rows)
-        a.y, a.y_stride = L.ptr(y).value, d
-        if res is not None:
-            a.residual, a.residual_stride = L.ptr(res).value, _row_stride(res)
-            a.sum, a.sum_stride = L.ptr(total).value, d
-        if spec is not None:
-            a.has_drop, a.drop = 1, spec.struct()
-        if stats is not None:
-            a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n
-            a.step_used = stats.data_ptr() + 8 * n
-        with torch.cuda.device(x.device):
-            L.check(lib.pg_layer_norm_fwd(ctypes.byref(a), L.stream_ptr()), "pg_layer_norm_fwd")
+        grad = ctx.needs_input_grad
+        stats = torch.empty(2 * n + 2, dtype=torch.float32, device=dev) if grad[0] or grad[1] or grad[2] or grad[3] else None
+        at = _addr(stats)
+        param = weight if weight is not None else bias
+        _enqueue("pg_layer_norm_fwd", dev, L.PgNormDesc(
+            rows.data_ptr(), _addr(res), _addr(weight), _addr(bias), _addr(total), y.data_ptr(), at, at + 4 * n if at is not None else None,
+            None, None, None, None, None, None, None, at + 8 * n if at is not None else None,
+            n, d, _row_stride(rows), _row_stride(res) if res is not None else 0, d, d, 0, 0, 0, 0,
+            _DTYPES[t], _DTYPES[param.dtype] if param is not None else _DTYPES[t], eps, 1 if spec is not None else 0,
+            _drop_struct(spec) if spec is not None else L.PgDropout()))
         ctx.eps, ctx.spec = eps, spec
         ctx.set_materialize_grads(False)
-        y = y.view(x.shape)
+        y = _like(y, x.shape)
         if res is None:
             ctx.save_for_backward(x, weight, bias, stats)
             return y
-        total = total.view(x.shape)
+        total = _like(total, x.shape)
         ctx.save_for_backward(total, weight, bias, stats)
         return y, total
 
     @staticmethod
-    def desc(rows, weight, bias, eps):
-        a = L.PgNormDesc()
-        param = weight if weight is not None else bias
-        a.n, a.d, a.dtype, a.eps = rows.size(0), rows.size(1), _DTYPES[rows.dtype], eps
-        a.param_dtype = _DTYPES[param.dtype] if param is not None else a.dtype
-        a.weight, a.bias = L.ptr(weight).value, L.ptr(bias).value
-        return a
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gsum=None):
+        _once("layer_norm")
         s, weight, bias, stats = ctx.saved_tensors
         need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
-        lib = L.load()
+        spec = ctx.spec
         if gy is None:
             if gsum is None:
                 return (None,) * 6
             gy = torch.zeros((), dtype=s.dtype, device=s.device).expand(s.shape)      # only the sum was used
         rows, g = _rows_of(s), _rows_of(gy)
+        gs = _rows_of(gsum) if gsum is not None else None
         n, d = rows.shape
+        dev, t = s.device, s.dtype
         need_w, need_b = need_w and weight is not None, need_b and bias is not None
-        a = _LayerNorm.desc(rows, weight, bias, ctx.eps)
-        a.sum, a.sum_stride, a.gy, a.gy_stride = L.ptr(rows).value, _row_stride(rows), L.ptr(g).value, _row_stride(g)
-        if gsum is not None:
-            gs = _rows_of(gsum)
-            a.gsum, a.gsum_stride = L.ptr(gs).value, _row_stride(gs)
-        a.mean, a.rstd = stats.data_ptr(), stats.data_ptr() + 4 * n
-        dx = dres = dw = db = None
-        if ctx.spec is not None:
-            a.has_drop, a.drop = 1, _drop_again(ctx.spec, stats[2 * n:] if ctx.spec.step is not None else None)
-        if need_x or (need_res and ctx.spec is None):
-            dx = torch.empty((n, d), dtype=s.dtype, device=s.device)
-            a.dx, a.dx_stride = L.ptr(dx).value, d
-        if need_res:
-            if ctx.spec is None:
-                dres = dx                          # one gradient for both summands, as of a sum
-            else:
-                dres = torch.empty((n, d), dtype=s.dtype, device=s.device)
-                a.dres, a.dres_stride = L.ptr(dres).value, d
-        if need_w:
-            dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
-        if need_b:
-            db = torch.empty_like(bias, memory_format=torch.contiguous_format)
+        dx = torch.empty((n, d), dtype=t, device=dev) if need_x or (need_res and spec is None) else None
+        # one gradient for both summands, as of a sum, unless a mask stands before one of them
+        dres = torch.empty((n, d), dtype=t, device=dev) if need_res and spec is not None else None
+        param = weight if weight is not None else bias
+        dw = torch.empty(d, dtype=weight.dtype, device=dev) if need_w else None
+        db = torch.empty(d, dtype=bias.dtype, device=dev) if need_b else None
         part = None
         if need_w or need_b:
-            part = torch.empty(lib.pg_layer_norm_scratch(n, d), dtype=torch.float32, device=s.device)
-            a.dw, a.db, a.partials = L.ptr(dw).value, L.ptr(db).value, L.ptr(part).value
-        with torch.cuda.device(s.device):
-            L.check(lib.pg_layer_norm_bwd(ctypes.byref(a), L.stream_ptr()), "pg_layer_norm_bwd")
-        return (dx.view(s.shape) if need_x else None, dw, db, dres.view(s.shape) if need_res else None, None, None)
+            part = torch.empty(L.load().pg_layer_norm_scratch(n, d), dtype=torch.float32, device=dev)
+        at = stats.data_ptr()
+        _enqueue("pg_layer_norm_bwd", dev, L.PgNormDesc(
+            None, None, _addr(weight), _addr(bias), rows.data_ptr(), None, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
+            _addr(dw), _addr(db), _addr(part), None,
+            n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
+            _DTYPES[t], _DTYPES[param.dtype] if param is not None else _DTYPES[t], ctx.eps, 1 if spec is not None else 0,
+            _drop_struct(spec, at + 8 * n if spec.step is not None else None) if spec is not None else L.PgDropout()))
+        if need_res:
+            dres = _like(dx if spec is None else dres, s.shape)
+        return (_like(dx, s.shape) if need_x else None, dw, db, dres, None, None)
 
 
 def layer_norm(x, module, residual=None, dropout=None):
@@ -1032,7 +1039,7 @@ def layer_norm(x, module, residual=None, dropout=None):
     for p in (w, b):
         if p is not None and (p.dtype not in (x.dtype, torch.float32) or not p.is_contiguous() or (w is not None and p.dtype != w.dtype)):
             raise L.PgError("layer_norm: weight and bias must be contiguous and share one type, the rows' or fp32")
-    _need_same_device("layer_norm", x, weight=w, bias=b, residual=residual)
+        _need_device("layer_norm", x, "weight or bias", p)
     if dropout is not None and dropout.threshold == 0:
         dropout = None
     if residual is None:
@@ -1040,6 +1047,8 @@ def layer_norm(x, module, residual=None, dropout=None):
             raise L.PgError("layer_norm: dropout comes with a residual; use ops.dropout in front of the norm otherwise")
     elif residual.shape != x.shape or residual.dtype != x.dtype:
         raise L.PgError("layer_norm: the residual must have the rows' shape and type")
+    else:
+        _need_device("layer_norm", x, "the residual", residual)
     if dropout is not None:
         _need_spec("layer_norm", x, dropout)
     return _LayerNorm.apply(x, w, b, residual, float(module.eps), dropout)
@@ -1051,60 +1060,50 @@ _REDUCTIONS = {"mean": L.PG_XENT_MEAN, "sum": L.PG_XENT_SUM, "none": L.PG_XENT_N
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, bias, labels, ignore_index, reduction):
-        lib = L.load()
         rows = _rows_of(h)
-        if weight.stride(1) != 1 or weight.stride(0) < weight.size(1):
-            weight = weight.contiguous()
-        labels = labels.reshape(-1).contiguous()
-        n = rows.size(0)
-        stats = torch.empty(3 * n + 4, dtype=torch.float32, device=h.device)      # lse | counted? | row losses | meta
-        a = _LinearCrossEntropy.desc(rows, weight, bias, labels, stats, ignore_index, reduction)
-        size = lib.pg_linear_xent_scratch(n, rows.size(1), weight.size(0), a.dtype, 0)
+        weight, labels = _table(weight), labels.reshape(-1).contiguous()
+        n, K, C = rows.size(0), rows.size(1), weight.size(0)
+        dev, t = h.device, _DTYPES[h.dtype]
+        stats = torch.empty(3 * n + 4, dtype=torch.float32, device=dev)           # lse | counted? | row losses | meta
+        size = L.load().pg_linear_xent_scratch(n, K, C, t, 0)
         if size < 0:
-            raise L.PgError(f"linear_cross_entropy: {n} rows x {weight.size(0)} classes x {rows.size(1)} columns are not supported")
-        scratch = torch.empty(size, dtype=torch.uint8, device=h.device)
-        a.scratch = L.ptr(scratch).value
-        with torch.cuda.device(h.device):
-            L.check(lib.pg_linear_xent_fwd(ctypes.byref(a), L.stream_ptr()), "pg_linear_xent_fwd")
+            raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        at = stats.data_ptr()
+        _enqueue("pg_linear_xent_fwd", dev, L.PgLinearXentDesc(
+            rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
+            None, None, None, None, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
         ctx.save_for_backward(h, weight, bias, labels, stats)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        if reduction == "none":
-            return stats[2 * n:3 * n].view(h.shape[:-1])
-        return stats[3 * n + (0 if reduction == "mean" else 2)]
+        if reduction == L.PG_XENT_NONE:
+            return _like(stats[2 * n:3 * n], h.shape[:-1])
+        return stats[3 * n + (0 if reduction == L.PG_XENT_MEAN else 2)]
 
     @staticmethod
-    def desc(rows, weight, bias, labels, stats, ignore_index, reduction):
-        a = L.PgLinearXentDesc()
-        n = rows.size(0)
-        a.h, a.W, a.bias, a.labels = L.ptr(rows).value, L.ptr(weight).value, L.ptr(bias).value, L.ptr(labels).value
-        a.lse = L.ptr(stats).value
-        a.flag, a.row_loss, a.meta = a.lse + 4 * n, a.lse + 8 * n, a.lse + 12 * n
-        a.n, a.K, a.C, a.h_stride, a.w_stride = n, rows.size(1), weight.size(0), _row_stride(rows), _row_stride(weight)
-        a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[rows.dtype], _REDUCTIONS[reduction]
-        return a
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        _once("linear_cross_entropy")
         h, weight, bias, labels, stats = ctx.saved_tensors
         need_h, need_w, need_b = ctx.needs_input_grad[:3]
-        need_b = need_b and bias is not None
-        lib = L.load()
         rows = _rows_of(h)
-        n, K = rows.shape
+        n, K, C = rows.size(0), rows.size(1), weight.size(0)
+        dev, t = h.device, _DTYPES[h.dtype]
         new = torch.zeros if n == 0 else torch.empty
-        dh = new((n, K), dtype=h.dtype, device=h.device) if need_h else None
-        dw = new(weight.shape, dtype=weight.dtype, device=h.device) if need_w else None
-        db = new(bias.shape, dtype=bias.dtype, device=h.device) if need_b else None
+        dh = new((n, K), dtype=h.dtype, device=dev) if need_h else None
+        dw = new((C, K), dtype=h.dtype, device=dev) if need_w else None
+        db = new((C,), dtype=h.dtype, device=dev) if need_b and bias is not None else None
         if n > 0:
             g = g.reshape(-1)                        # fp32, as the loss is
-            a = _LinearCrossEntropy.desc(rows, weight, bias, labels, stats, ctx.ignore_index, ctx.reduction)
-            scratch = torch.empty(lib.pg_linear_xent_scratch(n, K, weight.size(0), a.dtype, 1), dtype=torch.uint8, device=h.device)
-            a.scratch, a.grad, a.grad_stride = L.ptr(scratch).value, L.ptr(g).value, g.stride(0)
-            a.dh, a.dW, a.db = L.ptr(dh).value, L.ptr(dw).value, L.ptr(db).value
-            with torch.cuda.device(h.device):
-                L.check(lib.pg_linear_xent_bwd(ctypes.byref(a), L.stream_ptr()), "pg_linear_xent_bwd")
-        return dh.view(h.shape) if need_h else None, dw, db, None, None, None
+            scratch = torch.empty(L.load().pg_linear_xent_scratch(n, K, C, t, 1), dtype=torch.uint8, device=dev)
+            at = stats.data_ptr()
+            _enqueue("pg_linear_xent_bwd", dev, L.PgLinearXentDesc(
+                rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
+                g.data_ptr(), _addr(dh), _addr(dw), _addr(db), scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight),
+                g.stride(0), ctx.ignore_index, t, ctx.reduction))
+        return _like(dh, h.shape) if need_h else None, dw, db, None, None, None
+
+
+def _table(weight):
+    return weight if weight.stride(1) == 1 and weight.stride(0) >= weight.size(1) else weight.contiguous()
 
 
 def linear_cross_entropy(h, module, labels, ignore_index=-100, reduction="mean"):
@@ -1123,5 +1122,6 @@ def linear_cross_entropy(h, module, labels, ignore_index=-100, reduction="mean")
         raise L.PgError("linear_cross_entropy: labels must be int64, one for every row of h")
     if reduction not in _REDUCTIONS:
         raise L.PgError(f"linear_cross_entropy: reduction {reduction!r}: mean, sum or none")
-    _need_same_device("linear_cross_entropy", h, weight=w, bias=b, labels=labels)
-    return _LinearCrossEntropy.apply(h, w, b, labels, int(ignore_index), reduction)
+    for what, p in (("the weight", w), ("the bias", b), ("labels", labels)):
+        _need_device("linear_cross_entropy", h, what, p)
+    return _LinearCrossEntropy.apply(h, w, b, labels, int(ignore_index), _REDUCTIONS[reduction])
