@@ -3,293 +3,240 @@
 //   G = (exp(z - lse) - onehot(label)) * (row factor),  dh = G W,  dW = G^T h,  db = sum_r G.
 // The logits [n, C] exist only as tiles in registers. Forward: every workgroup leaves (maximum, sum of exponentials) of its tile's
 // rows, a second launch joins them. Backward: the logits are computed again in pieces of the vocabulary; a piece's G leaves in
-// the operands' 16 bits (fp32 for fp32 operands) and feeds the two gradient products before the next piece overwrites it.
-// 8 n K C operations instead of the 6 n K C with kept logits, against 8 bytes of fp32 logit traffic per element of [n, C].
+// 16-bit parts and feeds the two gradient products before the next piece overwrites it. 8 n K C operations instead of the 6 n K C
+// with kept logits, against 8 bytes of fp32 logit traffic per element of [n, C].
 //
-// Products run on the matrix cores with fp32 accumulation. fp32 operands: each value is split into three bf16 parts
-// (x = x0 + x1 + x2 to 24 bits) and six of the nine partial products are summed, what is left out is below 2^-24 of the product —
-// 2.5 PF / 6 where the fp32 matrix instructions reach 0.157 PF.
-// G in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-9, fp16 2^-12 relative), independently per element, as
-// are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability of 2^-28 is still a normal number.
-#include "pg_elem.h"
+// All three products run on one tile engine (pg_mm.h) with fp32 accumulation. Its operands are 16-bit parts in rows padded to
+// whole tiles: 16-bit rows that are so already are used in place, others are packed first (k_lx_pack). fp32 values are split
+// into three bf16 parts (x = x0 + x1 + x2 to 24 bits) and six of the nine partial products are summed; what is left out is below
+// 2^-24 of the product — 2.5 PF / 6 where the fp32 matrix instructions reach 0.157 PF.
+// G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-9, fp16 2^-12 relative),
+// independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
+// of 2^-28 is still a normal number.
+#include "pg_mm.h"
 
 namespace pg {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
-typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// how an operand type is multiplied: parts per value, the parts' type, depth of a tile
+// how an operand type is multiplied: the parts' type and number, G's scale
 template <typename T> struct Mul;
-template <> struct Mul<float>  { typedef bf16_t E; typedef bf16x8 V; static constexpr int NP = 3, BK = 32, MB = 2; };
-template <> struct Mul<bf16_t> { typedef bf16_t E; typedef bf16x8 V; static constexpr int NP = 1, BK = 64, MB = 4; };
-template <> struct Mul<f16_t>  { typedef f16_t E;  typedef f16x8 V;  static constexpr int NP = 1, BK = 64, MB = 4; };
-
-__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
-// LDS tile [rows][BK] of one part: 16-byte chunks, chunk index XORed with bits of the row so that the 8 lanes of a read phase
-// (consecutive rows) and of a transposing write (rows 4 resp. 2 apart) meet different banks
-template <int BK>
-__device__ __forceinline__ int lds_at(int row, int chunk) {
-  return BK == 64 ? row * 64 + ((chunk ^ ((row ^ (row >> 2)) & 7)) << 3) : row * 32 + ((chunk ^ ((row >> 1) & 3)) << 3);
-}
-
-template <typename T>
-__device__ __forceinline__ void split_write(typename Mul<T>::E* tile, int part_stride, int at, const T (&v)[8]) {
-  typename Mul<T>::V o;
-  if constexpr (Mul<T>::NP == 1) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = v[i];
-    *reinterpret_cast<typename Mul<T>::V*>(tile + at) = o;
-  } else {
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = v[i];
-#pragma unroll
-    for (int p = 0; p < 3; ++p) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        o[i] = (bf16_t)x[i];
-        x[i] -= (float)o[i];                       // exact
-      }
-      *reinterpret_cast<bf16x8*>(tile + p * part_stride + at) = o;
-    }
-  }
-}
-
-// Operand whose reduction index is contiguous: p[row * ld + k]. Rows >= nrows and k >= K read as 0.
-template <typename T, int ROWS>
-struct LoadK {
-  static constexpr int BK = Mul<T>::BK, CH = BK / 8, U = ROWS * CH / 256;
-  const T* p;
-  int64_t ld, row0, nrows, K;
-  T v[U][8];
-  __device__ __forceinline__ void load(int64_t k0, int tid) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int id = tid + u * 256, row = id / CH, ch = id % CH;
-      const int64_t k = k0 + ch * 8, r = row0 + row;
-      const T* s = p + r * ld + k;
-      if (r < nrows && k + 8 <= K) {
-        __builtin_memcpy(v[u], s, sizeof(v[u]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[u][i] = r < nrows && k + i < K ? s[i] : (T)0.f;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(typename Mul<T>::E* tile, int tid) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int id = tid + u * 256;
-      split_write<T>(tile, ROWS * BK, lds_at<BK>(id / CH, id % CH), v[u]);
-    }
-  }
-};
-
-// Operand whose row index is contiguous: p[k * ld + row], transposed on its way into LDS: a thread holds MB rows x 8 k.
-// flag (may be NULL): k with flag[k] == 0 read as 0 without being read (ignored rows may hold anything)
-template <typename T, int ROWS>
-struct LoadM {
-  static constexpr int BK = Mul<T>::BK, MB = Mul<T>::MB, UR = ROWS / MB, UNITS = UR * (BK / 8);
-  const T* p;
-  int64_t ld, row0, nrows, K;
-  const float* flag;
-  T v[8][MB];
-  __device__ __forceinline__ void load(int64_t k0, int tid) {
-    if (UNITS < 256 && tid >= UNITS) return;
-    const int64_t r = row0 + (tid % UR) * MB;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t k = k0 + (tid / UR) * 8 + j;
-      const bool ok = k < K && (!flag || flag[k] != 0.f);
-      const T* s = p + k * ld + r;
-      if (ok && r + MB <= nrows) {
-        __builtin_memcpy(v[j], s, sizeof(v[j]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < MB; ++i) v[j][i] = ok && r + i < nrows ? s[i] : (T)0.f;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(typename Mul<T>::E* tile, int tid) {
-    if (UNITS < 256 && tid >= UNITS) return;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      T c[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = v[j][i];
-      split_write<T>(tile, ROWS * BK, lds_at<BK>((tid % UR) * MB + i, tid / UR), c);
-    }
-  }
-};
-
-struct NoSide { __device__ __forceinline__ void operator()() const {} };
-
-// acc[i][j] += A(64-row slab wm of BM) x B(slab wn of BN): 4 waves, 2 x 2; reduction over [k_lo, k_hi). One register-staged tile
-// ahead, two LDS buffers, one barrier per step. side() runs once per loaded A tile (its values are in la.v).
-template <typename T, int BM, int BN, typename LA, typename LB, typename Side>
-__device__ __forceinline__ void product(LA& la, LB& lb, int64_t k_lo, int64_t k_hi, typename Mul<T>::E* lds,
-                                        f32x16 (&acc)[BM / 64][BN / 64], Side side) {
-  typedef typename Mul<T>::E E;
-  typedef typename Mul<T>::V V;
-  constexpr int BK = Mul<T>::BK, NP = Mul<T>::NP, STAGE = NP * (BM + BN) * BK;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  int buf = 0;
-  la.load(k_lo, tid);
-  lb.load(k_lo, tid);
-  for (int64_t k0 = k_lo; k0 < k_hi; k0 += BK) {
-    E* ta = lds + buf * STAGE;
-    E* tb = ta + NP * BM * BK;
-    side();
-    la.store(ta, tid);
-    lb.store(tb, tid);
-    if (k0 + BK < k_hi) {
-      la.load(k0 + BK, tid);
-      lb.load(k0 + BK, tid);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      const int chunk = kk * 2 + (lane >> 5);
-      V a[NP][BM / 64], b[NP][BN / 64];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-#pragma unroll
-        for (int i = 0; i < BM / 64; ++i)
-          a[p][i] = *reinterpret_cast<const V*>(ta + p * BM * BK + lds_at<BK>(wm * (BM / 2) + i * 32 + (lane & 31), chunk));
-#pragma unroll
-        for (int j = 0; j < BN / 64; ++j)
-          b[p][j] = *reinterpret_cast<const V*>(tb + p * BN * BK + lds_at<BK>(wn * (BN / 2) + j * 32 + (lane & 31), chunk));
-      }
-#pragma unroll
-      for (int i = 0; i < BM / 64; ++i)
-#pragma unroll
-        for (int j = 0; j < BN / 64; ++j) {
-          if constexpr (NP == 3) {                 // smallest first
-            acc[i][j] = mma(a[2][i], b[0][j], acc[i][j]);
-            acc[i][j] = mma(a[1][i], b[1][j], acc[i][j]);
-            acc[i][j] = mma(a[0][i], b[2][j], acc[i][j]);
-            acc[i][j] = mma(a[1][i], b[0][j], acc[i][j]);
-            acc[i][j] = mma(a[0][i], b[1][j], acc[i][j]);
-          }
-          acc[i][j] = mma(a[0][i], b[0][j], acc[i][j]);
-        }
-    }
-    buf ^= 1;                                      // the other buffer's readers have passed the barrier above
-  }
-}
+template <> struct Mul<float>  { typedef bf16_t E; static constexpr int NP = 3; static constexpr float G = 1.f; };
+template <> struct Mul<bf16_t> { typedef bf16_t E; static constexpr int NP = 1; static constexpr float G = 1.f; };
+template <> struct Mul<f16_t>  { typedef f16_t E;  static constexpr int NP = 1; static constexpr float G = 16384.f; };
 
 struct LxArgs {
-  const void *h, *w, *bias;
+  const void *h, *w, *bias;                // operands in parts: h [parts][h_rows][h_ld], w [parts][w_rows][w_ld]
+  int64_t h_ld, h_part, h_rows, w_ld, w_part;
   const int64_t* labels;
-  int64_t n, K, C, hs, ws, ignore;
-  float2* part;            // [n][tiles] maximum, sum of exponentials
+  int64_t n, K, Kp, C, ignore;             // Kp: K padded to whole tiles
+  float2* part;                            // [n][tiles] maximum, sum of exponentials
   float *zlab, *lse, *row_loss, *flag, *meta;
   int64_t tiles;
   // backward
-  const float *rowf;       // row factors: flag, or the normalised incoming gradients
-  const float *f1, *f2;    // the outputs' factor = *f1 * *f2 (NULL = 1)
-  void* g;                 // a piece of G: [n][ldg]
-  int64_t ldg, c_lo, c_hi; // the piece's classes
-  float* acc;              // fp32 partial products [split][rows][K]
-  float* accb;
+  const float* rowf;                       // row factors: flag, or the normalised incoming gradients
+  const float *f1, *f2;                    // the outputs' factor = *f1 * *f2 (NULL = 1)
+  void* g;                                 // a piece of G: [parts][g_rows][ldg], zeros beyond n and beyond c_hi
+  int64_t ldg, g_rows, c_lo, c_hi;         // the piece's classes
+  float* acc;                              // fp32 partial products [split][rows][K]
+  float* dbp;                              // [row tiles][C] partial sums of G
   void *dh, *dw, *db;
-  int64_t k_split;         // reduction range of one split
-  int32_t splits, first;
+  int64_t range;                           // reduction range of one split
+  int32_t splits, first, direct;           // direct: one split and one piece, the product itself is the output
 };
 
-template <typename T> struct GScale { static constexpr float v = 1.f; };
-template <> struct GScale<f16_t> { static constexpr float v = 16384.f; };
-
 __device__ __forceinline__ bool label_ok(int64_t lab, const LxArgs& a) { return lab != a.ignore && lab >= 0 && lab < a.C; }
+// a label's place in the tile of classes [c0, c0 + width), far below 0 elsewhere
+__device__ __forceinline__ int label_in(int64_t lab, int64_t c0, int width) {
+  return lab >= c0 && lab < c0 + width ? (int)(lab - c0) : -(1 << 30);
+}
 __device__ __forceinline__ float out_factor(const LxArgs& a) { return (a.f1 ? *a.f1 : 1.f) * (a.f2 ? *a.f2 : 1.f); }
 
-// Workgroups go round the 8 XCDs in turn: give each XCD a contiguous run of tiles, so that its own L2 sees a tile's neighbours
-__device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total) {
-  const int64_t per = total / 8, rest = total % 8, x = b % 8, i = b / 8;
-  return x * per + (x < rest ? x : rest) + i;
+// rows of T as padded rows of parts: dst [NP][rows_p][ldp]; columns beyond K, rows beyond `rows` and (labels != NULL) rows that do
+// not count are zeros, whatever the source holds there
+struct PackArgs {
+  const void* src;
+  void* dst;
+  int64_t rows, rows_p, K, ld, ldp;
+  const int64_t* labels;
+  int64_t ignore, C;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1) {
+  typedef typename Mul<T>::E E;
+  const PackArgs& a = blockIdx.y ? a1 : a0;
+  if (!a.dst) return;
+  const int64_t ch = a.ldp / 8, total = a.rows_p * ch;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / ch, c = (t - r * ch) * 8;
+    bool ok = r < a.rows;
+    if (ok && a.labels) {
+      const int64_t lab = a.labels[r];
+      ok = lab != a.ignore && lab >= 0 && lab < a.C;
+    }
+    const T* s = (const T*)a.src + r * a.ld + c;
+    T v[8];
+    if (ok && c + 8 <= a.K) {
+      __builtin_memcpy(v, s, sizeof(v));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = ok && c + i < a.K ? s[i] : (T)0.f;
+    }
+    E o[8];
+    E* d = (E*)a.dst + r * a.ldp + c;
+    if constexpr (Mul<T>::NP == 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = (E)v[i];
+      __builtin_memcpy(d, o, sizeof(o));
+    } else {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = v[i];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          o[i] = (E)x[i];
+          x[i] -= (float)o[i];                       // exact
+        }
+        __builtin_memcpy(d + p * a.rows_p * a.ldp, o, sizeof(o));
+      }
+    }
+  }
 }
 
-// One 128-class x BN-row tile of logits; a lane holds one row's classes in registers: row = wn * BN/2 + 32 j + lane % 32,
-// class = wm * 64 + 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4. PIECE: writes G, else the tile's row statistics.
-template <typename T, int BN, bool PIECE>
-__global__ __launch_bounds__(256) void k_lx_logits(LxArgs a) {
-  typedef typename Mul<T>::E E;
-  constexpr int BM = 128, BK = Mul<T>::BK, NP = Mul<T>::NP;
-  __shared__ __align__(16) E lds[2 * NP * (BM + BN) * BK];
-  __shared__ float2 red[2][BN];
+// One BM-class x BN-row tile of logits; a lane holds one row's classes in registers: row = 32 j + lane % 32 of its wave's rows,
+// class = 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4 of its wave's classes, so a row's maximum and sum are taken in registers.
+// PIECE: writes G (through LDS: whole 16-byte pieces of rows) and the column sums of the tile, else the tile's row statistics.
+template <typename T, typename S, bool PIECE>
+__global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
+  typedef typename S::E E;
+  constexpr int BM = S::BM, BN = S::BN, WM = BM / S::WR, WN = BN / S::WC;
+  __shared__ __align__(16) short buf[2 * S::TILE];
+  __shared__ float2 red[PIECE ? 1 : S::WR][PIECE ? 1 : BN];
+  __shared__ __align__(16) float bias[BM];                   // -inf beyond the last class: its exponentials are 0
   const int64_t row_tiles = ceil_div<int64_t>(a.n, BN), c_tiles = ceil_div<int64_t>(a.c_hi - a.c_lo, BM);
-  const int64_t t = xcd_run(blockIdx.x, row_tiles * c_tiles);
-  const int64_t ct = t / row_tiles, r0 = t % row_tiles * BN, c0 = a.c_lo + ct * BM;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  f32x16 acc[2][BN / 64] = {};
-  LoadK<T, BM> la{(const T*)a.w, a.ws, c0, a.c_hi, a.K};
-  LoadK<T, BN> lb{(const T*)a.h, a.hs, r0, a.n, a.K};
-  product<T, BM, BN>(la, lb, 0, a.K, lds, acc, NoSide{});
+  // an XCD's 32 CUs work on 8 row tiles x 4 class tiles at a time
+  const int64_t t = xcd_run(blockIdx.x, row_tiles * c_tiles), group = t / (8 * c_tiles);
+  const int64_t in_group = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8, u = t - group * 8 * c_tiles;
+  const int64_t ct = u / in_group, rt = group * 8 + u % in_group, r0 = rt * BN, c0 = a.c_lo + ct * BM;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
+  for (int c = tid; c < BM; c += S::THREADS)
+    bias[c] = c0 + c >= a.c_hi ? -INFINITY : a.bias ? (float)((const T*)a.bias)[c0 + c] : 0.f;
+  f32x16 acc[S::FI][S::FJ] = {};
+  mm_product<S, ROWS, ROWS>(Operand{a.w, a.w_ld, a.w_part, c0, a.C, 0}, Operand{a.h, a.h_ld, a.h_part, r0, a.h_rows, 0}, 0, a.Kp, buf, buf + S::TILE, acc);
+  const int cw = wm * WM + 4 * (lane >> 5);                  // the lane's first class within the tile
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t c = c0 + wm * 64 + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-      float b = c < a.c_hi ? 0.f : -INFINITY;
-      if (a.bias && c < a.c_hi) b = (float)((const T*)a.bias)[c];
+    for (int q = 0; q < 4; ++q) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + cw + i * 32 + 8 * q);
 #pragma unroll
-      for (int j = 0; j < BN / 64; ++j) acc[i][j][e] += b;
+      for (int j = 0; j < S::FJ; ++j) {
+        acc[i][j][4 * q] += b.x;
+        acc[i][j][4 * q + 1] += b.y;
+        acc[i][j][4 * q + 2] += b.z;
+        acc[i][j][4 * q + 3] += b.w;
+      }
     }
+  if constexpr (!PIECE) {
 #pragma unroll
-  for (int j = 0; j < BN / 64; ++j) {
-    const int rl = wn * (BN / 2) + j * 32 + (lane & 31);
-    const int64_t r = r0 + rl;
-    const int64_t lab = r < a.n ? a.labels[r] : -1;
-    if constexpr (!PIECE) {
+    for (int j = 0; j < S::FJ; ++j) {
+      const int rl = wn * WN + j * 32 + (lane & 31);
+      const int64_t r = r0 + rl;
+      const int at = r < a.n ? label_in(a.labels[r], c0, BM) - cw : -1;
       float m = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::FI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           m = fmaxf(m, acc[i][j][e]);
-          const int64_t c = c0 + wm * 64 + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-          if (c == lab && r < a.n) a.zlab[r] = acc[i][j][e];
+          if (at == i * 32 + 8 * (e / 4) + e % 4) a.zlab[r] = acc[i][j][e];
         }
       m = fmaxf(m, __shfl_xor(m, 32, kWave));
       const float base = m == -INFINITY ? 0.f : m;         // nothing but -inf so far: every exponential is 0
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::FI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - base) * kLog2e);
       s += __shfl_xor(s, 32, kWave);
       if (lane < 32) red[wm][rl] = make_float2(m, s);
-    } else if (r < a.n) {
-      const float lse = a.lse[r], f = a.rowf[r] * GScale<T>::v;
-      T* g = (T*)a.g + r * a.ldg + (c0 - a.c_lo) + wm * 64 + 4 * (lane >> 5);
+    }
+    __syncthreads();
+    for (int rl = tid; rl < BN; rl += S::THREADS)
+      if (r0 + rl < a.n) {
+        float m = red[0][rl].x, s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 1; i < S::WR; ++i) m = fmaxf(m, red[i][rl].x);
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float o[4];
+        for (int i = 0; i < S::WR; ++i) s += red[i][rl].y * __builtin_amdgcn_exp2f((red[i][rl].x - base) * kLog2e);
+        a.part[(r0 + rl) * a.tiles + ct] = make_float2(m, s);
+      }
+  } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int64_t c = c0 + wm * 64 + i * 32 + 8 * q + 4 * (lane >> 5) + e;
-            const float pr = __builtin_amdgcn_exp2f((acc[i][j][q * 4 + e] - lse) * kLog2e) - (c == lab ? 1.f : 0.f);
-            o[e] = f == 0.f || c >= a.c_hi ? 0.f : pr * f;
-          }
-          store4(g + i * 32 + 8 * q, o);
+    for (int j = 0; j < S::FJ; ++j) {
+      const int64_t r = r0 + wn * WN + j * 32 + (lane & 31);
+      const bool in = r < a.n;
+      const int at = in ? label_in(a.labels[r], c0, BM) - cw : -1;
+      const float f = in ? a.rowf[r] * Mul<T>::G : 0.f, lse = in ? a.lse[r] : 0.f;
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * kLog2e) - (at == i * 32 + 8 * (e / 4) + e % 4 ? 1.f : 0.f);
+          acc[i][j][e] = f == 0.f ? 0.f : p * f;
         }
     }
-  }
-  if constexpr (!PIECE) {
+    // [BN rows][BM classes] of one part in the tile buffers, 16-byte chunks swizzled by the row
+    constexpr int CH = BM / 8, RP = S::THREADS / CH;
+    static_assert(BM * BN <= S::TILE * 2, "a part of G fits the tile buffers");
+    static_assert(RP * BM * 4 <= 4 * S::TILE, "and so do its column sums");
+    short* stage = buf;
+    float sum[8] = {};
+#pragma unroll 1
+    for (int part = 0; part < S::NP; ++part) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < S::FJ; ++j) {
+        const int rl = wn * WN + j * 32 + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            E o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              o[e] = (E)acc[i][j][q * 4 + e];
+              acc[i][j][q * 4 + e] -= (float)o[e];
+            }
+            const int chunk = (wm * WM + i * 32 + 8 * q) / 8;
+            __builtin_memcpy(stage + rl * BM + ((chunk ^ (rl & (CH - 1))) << 3) + 4 * (lane >> 5), o, 8);
+          }
+      }
+      __syncthreads();
+      const int ch = tid % CH;
+      E* g = (E*)a.g + part * a.g_rows * a.ldg + r0 * a.ldg + (c0 - a.c_lo) + ch * 8;
+      for (int rl = tid / CH; rl < BN; rl += RP) {
+        E o[8];
+        __builtin_memcpy(o, stage + rl * BM + ((ch ^ (rl & (CH - 1))) << 3), 16);
+        __builtin_memcpy(g + rl * a.ldg, o, 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += (float)o[e];
+      }
+    }
     __syncthreads();
-    for (int rl = tid; rl < BN; rl += 256)
-      if (r0 + rl < a.n) {
-        const float2 x = red[0][rl], y = red[1][rl];
-        const float m = fmaxf(x.x, y.x), base = m == -INFINITY ? 0.f : m;
-        a.part[(r0 + rl) * a.tiles + ct] =
-            make_float2(m, x.y * __builtin_amdgcn_exp2f((x.x - base) * kLog2e) + y.y * __builtin_amdgcn_exp2f((y.x - base) * kLog2e));
+    float* cs = (float*)stage;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[(tid / CH) * BM + tid % CH * 8 + e] = sum[e];
+    __syncthreads();
+    for (int c = tid; c < BM; c += S::THREADS)
+      if (c0 + c < a.c_hi) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < RP; ++i) s += cs[i * BM + c];
+        a.dbp[rt * a.C + c0 + c] = s;
       }
   }
 }
@@ -369,245 +316,285 @@ __global__ __launch_bounds__(1024) void k_lx_row_factors(const float* __restrict
   if (threadIdx.x == 0) *top = m;
 }
 
-// dh partials: acc[split][r][k] (+)= sum over the split's classes of G[r][c] W[c][k]
-template <typename T, int BN>
-__global__ __launch_bounds__(256) void k_lx_dh(LxArgs a) {
-  typedef typename Mul<T>::E E;
-  constexpr int BM = 128, BK = Mul<T>::BK, NP = Mul<T>::NP;
-  __shared__ __align__(16) E lds[2 * NP * (BM + BN) * BK];
-  const int64_t row_tiles = ceil_div<int64_t>(a.n, BM), k_tiles = ceil_div<int64_t>(a.K, BN);
-  const int64_t t = xcd_run(blockIdx.x, row_tiles * k_tiles * a.splits);
-  const int64_t kt = t % k_tiles, rt = t / k_tiles % row_tiles, sp = t / k_tiles / row_tiles;
-  const int64_t r0 = rt * BM, n0 = kt * BN, len = a.c_hi - a.c_lo;
-  const int64_t lo = sp * a.k_split, hi = lo + a.k_split < len ? lo + a.k_split : len;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  f32x16 acc[2][BN / 64] = {};
-  if (lo < hi) {
-    LoadK<T, BM> la{(const T*)a.g, a.ldg, r0, a.n, hi};
-    LoadM<T, BN> lb{(const T*)a.w + a.c_lo * a.ws, a.ws, n0, a.K, hi, nullptr};
-    product<T, BM, BN>(la, lb, lo, hi, lds, acc, NoSide{});
-  }
-  float* out = a.acc + sp * a.n * a.K;
+// f(row, column, value) for the values a lane holds that lie inside rows x cols of the tile
+template <typename S, typename F>
+__device__ __forceinline__ void each_output(const f32x16 (&acc)[S::FI][S::FJ], int row, int col, int rows, int cols, F f) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < S::FJ; ++j)
+    if (col + 32 * j < cols) {
 #pragma unroll
-    for (int j = 0; j < BN / 64; ++j) {
-      const int64_t k = n0 + wn * (BN / 2) + j * 32 + (lane & 31);
+      for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t r = r0 + wm * 64 + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        if (r < a.n && k < a.K) {
-          float* p = out + r * a.K + k;
-          *p = (a.first ? 0.f : *p) + acc[i][j][e];
+        for (int e = 0; e < 16; ++e) {
+          const int r = row + i * 32 + 8 * (e / 4) + e % 4;
+          if (r < rows) f(r, col + 32 * j, acc[i][j][e]);
         }
-      }
     }
 }
 
+// dh: acc[split][r][k] (+)= sum over the split's classes of G[r][c] W[c][k]
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
+  constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
+  __shared__ __align__(16) short buf[2 * S::TILE];
+  const int64_t row_tiles = ceil_div<int64_t>(a.n, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
+  const int64_t t = xcd_run(blockIdx.x, row_tiles * k_tiles * a.splits);
+  const int64_t kt = t % k_tiles, rt = t / k_tiles % row_tiles, sp = t / k_tiles / row_tiles;
+  const int64_t r0 = rt * S::BM, n0 = kt * S::BN, len = (a.c_hi - a.c_lo + kDepth - 1) / kDepth * kDepth;
+  const int64_t lo = sp * a.range, hi = lo + a.range < len ? lo + a.range : len;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
+  f32x16 acc[S::FI][S::FJ] = {};
+  mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
+                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, buf + S::TILE, acc);
+  const int rl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);       // the lane's first row, first column of the tile
+  const int rows = (int)(a.n - r0 < S::BM ? a.n - r0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
+  if (a.direct) {
+    const float f = out_factor(a) / Mul<T>::G;
+    T* out = (T*)a.dh + r0 * a.K + n0;
+    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
+  } else {
+    float* out = a.acc + sp * a.n * a.K + r0 * a.K + n0;
+    if (a.first)
+      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = v; });
+    else
+      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] += v; });
+  }
+}
+
+// the splits of dh added in order; blockIdx.y == 1: the row tiles' partial sums of db likewise
 template <typename T>
-__global__ __launch_bounds__(256) void k_lx_dh_out(LxArgs a) {
-  const float f = out_factor(a) / GScale<T>::v;
-  const int64_t total = a.n * a.K;
+__global__ __launch_bounds__(256) void k_lx_sums(LxArgs a, int64_t row_tiles) {
+  const float f = out_factor(a) / Mul<T>::G;
+  if (blockIdx.y == 0) {
+    if (!a.dh || a.direct) return;
+    const int64_t total = a.n * a.K;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+      float s = 0.f;
+      for (int i = 0; i < a.splits; ++i) s += a.acc[i * total + t];
+      ((T*)a.dh)[t] = a.rowf[t / a.K] == 0.f ? (T)0.f : (T)(s * f);
+    }
+  } else {
+    if (!a.db) return;
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < a.C; c += (int64_t)gridDim.x * 256) {
+      float s = 0.f;
+      for (int64_t i = 0; i < row_tiles; ++i) s += a.dbp[i * a.C + c];
+      ((T*)a.db)[c] = (T)(s * f);
+    }
+  }
+}
+
+// dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]
+template <typename T, typename S>
+__global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
+  constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
+  __shared__ __align__(16) short buf[2 * S::TILE];
+  const int64_t len = a.c_hi - a.c_lo, c_tiles = ceil_div<int64_t>(len, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
+  const int64_t t = xcd_run(blockIdx.x, c_tiles * k_tiles * a.splits);
+  const int64_t kt = t % k_tiles, ct = t / k_tiles % c_tiles, sp = t / k_tiles / c_tiles;
+  const int64_t c0 = ct * S::BM, n0 = kt * S::BN, rows = (a.n + kDepth - 1) / kDepth * kDepth;
+  const int64_t lo = sp * a.range, hi = lo + a.range < rows ? lo + a.range : rows;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
+  f32x16 acc[S::FI][S::FJ] = {};
+  mm_product<S, COLS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, c0, a.g_rows, a.ldg},
+                            Operand{a.h, a.h_ld, a.h_part, n0, a.h_rows, a.Kp}, lo, hi, buf, buf + S::TILE, acc);
+  const int cl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);
+  const int cs = (int)(len - c0 < S::BM ? len - c0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
+  if (a.splits > 1) {
+    float* out = a.acc + (sp * len + c0) * a.K + n0;
+    each_output<S>(acc, cl, kl, cs, cols, [&](int c, int k, float v) { out[c * a.K + k] = v; });
+  } else {
+    const float f = out_factor(a) / Mul<T>::G;
+    T* out = (T*)a.dw + (a.c_lo + c0) * a.K + n0;
+    each_output<S>(acc, cl, kl, cs, cols, [&](int c, int k, float v) { out[c * a.K + k] = (T)(v * f); });
+  }
+}
+
+// the splits of one piece's dW added in order
+template <typename T>
+__global__ __launch_bounds__(256) void k_lx_dw_out(LxArgs a) {
+  const float f = out_factor(a) / Mul<T>::G;
+  const int64_t total = (a.c_hi - a.c_lo) * a.K;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
     float s = 0.f;
     for (int i = 0; i < a.splits; ++i) s += a.acc[i * total + t];
-    ((T*)a.dh)[t] = a.rowf[t / a.K] == 0.f ? (T)0.f : (T)(s * f);
-  }
-}
-
-// dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]; db rides along in the workgroups of the first column tile
-template <typename T, int BN>
-__global__ __launch_bounds__(256) void k_lx_dw(LxArgs a) {
-  typedef typename Mul<T>::E E;
-  constexpr int BM = 128, BK = Mul<T>::BK, NP = Mul<T>::NP, MB = Mul<T>::MB;
-  __shared__ __align__(16) E lds[2 * NP * (BM + BN) * BK];
-  __shared__ float sdb[BK / 8][BM];
-  const int64_t len = a.c_hi - a.c_lo, c_tiles = ceil_div<int64_t>(len, BM), k_tiles = ceil_div<int64_t>(a.K, BN);
-  const int64_t t = xcd_run(blockIdx.x, c_tiles * k_tiles * a.splits);
-  const int64_t kt = t % k_tiles, ct = t / k_tiles % c_tiles, sp = t / k_tiles / c_tiles;
-  const int64_t c0 = ct * BM, n0 = kt * BN;
-  const int64_t lo = sp * a.k_split, hi = lo + a.k_split < a.n ? lo + a.k_split : a.n;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
-  f32x16 acc[2][BN / 64] = {};
-  float bsum[MB] = {};
-  LoadM<T, BM> la{(const T*)a.g, a.ldg, c0, a.ldg, hi, nullptr};
-  LoadM<T, BN> lb{(const T*)a.h, a.hs, n0, a.K, hi, a.rowf};
-  if (lo < hi)
-    product<T, BM, BN>(la, lb, lo, hi, lds, acc, [&] {
-      if (kt == 0) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int i = 0; i < MB; ++i) bsum[i] += (float)la.v[j][i];
-      }
-    });
-  const float f = out_factor(a) / GScale<T>::v;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < BN / 64; ++j) {
-      const int64_t k = n0 + wn * (BN / 2) + j * 32 + (lane & 31);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t c = c0 + wm * 64 + i * 32 + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        if (c < len && k < a.K) {
-          if (a.splits > 1)
-            a.acc[(sp * len + c) * a.K + k] = acc[i][j][e];
-          else if (a.dw)
-            ((T*)a.dw)[(a.c_lo + c) * a.K + k] = (T)(acc[i][j][e] * f);
-        }
-      }
-    }
-  if (kt == 0 && (a.db || a.accb)) {
-    constexpr int UR = BM / MB;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) sdb[tid / UR][tid % UR * MB + i] = bsum[i];
-    __syncthreads();
-    if (tid < BM && c0 + tid < len) {
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < BK / 8; ++i) s += sdb[i][tid];
-      if (a.splits == 1)
-        ((T*)a.db)[a.c_lo + c0 + tid] = (T)(s * f);
-      else
-        a.accb[sp * len + c0 + tid] = s;
-    }
-  }
-}
-
-// the splits of one piece's dW (rows x K) and db added in order
-template <typename T>
-__global__ __launch_bounds__(256) void k_lx_dw_out(LxArgs a) {
-  const float f = out_factor(a) / GScale<T>::v;
-  const int64_t len = a.c_hi - a.c_lo, total = len * a.K;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total + len; t += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    if (t < total) {
-      if (!a.dw) continue;
-      for (int i = 0; i < a.splits; ++i) s += a.acc[i * total + t];
-      ((T*)a.dw)[a.c_lo * a.K + t] = (T)(s * f);
-    } else if (a.db) {
-      for (int i = 0; i < a.splits; ++i) s += a.accb[i * len + t - total];
-      ((T*)a.db)[a.c_lo + t - total] = (T)(s * f);
-    }
+    ((T*)a.dw)[a.c_lo * a.K + t] = (T)(s * f);
   }
 }
 
 inline int64_t up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
 
-// sizes of one call: everything follows from (n, K, C, type) alone, so that the scratch the caller allocates fits the launches
+// sizes of one call: everything follows from the shapes, types and alignments of the operands, so that the scratch the caller
+// allocates (for packed operands always) fits the launches
 struct LxPlan {
-  int64_t tiles, piece, ldg, part_bytes, g_bytes, acc_bytes;
-  int32_t dh_splits, dw_splits;
+  int64_t Kp, h_rows, tiles, row_tiles, piece, ldg, g_rows;
+  int64_t h_bytes, w_bytes, part_bytes, g_bytes, acc_dh, acc_dw, dbp_bytes;
+  int32_t dh_splits, dw_splits, pieces;
   int64_t dh_range, dw_range;
-  int bn_rows, bn_cols;
+  int big, cols;                            // tile shapes: 256 x 256 logits; columns of a gradient tile
 };
 
 inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   LxPlan p{};
-  const int64_t e = dtype == PG_DTYPE_F32 ? 4 : 2, bk = dtype == PG_DTYPE_F32 ? 32 : 64;
-  p.tiles = ceil_div<int64_t>(C, 128);
-  p.bn_rows = n <= 64 ? 64 : 128;
-  p.bn_cols = K <= 64 ? 64 : 128;
-  p.part_bytes = n * p.tiles * 8;
-  // a piece of G within 128 MB: the 256 MB memory-side cache then holds it between the three products
-  int64_t cols = (int64_t(128) << 20) / (e * (n > 0 ? n : 1)) / 128 * 128;
-  if (cols < 128) cols = 128;
-  const int64_t pieces = ceil_div<int64_t>(C, cols);
-  p.piece = up(ceil_div<int64_t>(C, pieces), 128);
+  const int64_t np = dtype == PG_DTYPE_F32 ? 3 : 1;
+  p.Kp = up(K, kDepth);
+  p.h_rows = up(n, 256);
+  p.h_bytes = up(np * p.h_rows * p.Kp * 2, 256);
+  p.w_bytes = up(np * C * p.Kp * 2, 256);
+  p.big = n > 128 && C > 128 && p.Kp * np >= 256;
+  const int64_t bm = p.big ? 256 : 128;
+  p.tiles = ceil_div<int64_t>(C, bm);
+  p.row_tiles = ceil_div<int64_t>(n, bm);
+  p.part_bytes = up(n * p.tiles * 8, 256);
+  p.cols = p.Kp >= 256 ? 256 : p.Kp > 64 ? 128 : 64;
+  // a piece of G
+  p.g_rows = up(n, 256);
+  int64_t cols = (int64_t(256) << 20) / (np * 2 * p.g_rows) / 256 * 256;
+  if (cols < 256) cols = 256;
+  if (cols > (1 << 18)) cols = 1 << 18;
+  p.pieces = (int32_t)ceil_div<int64_t>(C, cols);
+  p.piece = up(ceil_div<int64_t>(C, p.pieces), 256);
+  p.pieces = (int32_t)ceil_div<int64_t>(C, p.piece);
   p.ldg = p.piece;
-  p.g_bytes = n * p.ldg * e;
-  // splits of the reductions: at least two workgroups per CU, ranges of at least eight tile depths
+  p.g_bytes = up(np * p.g_rows * p.ldg * 2, 256);
+  // splits of the reductions: enough workgroups for the 256 CUs, ranges of at least eight tiles
+  const int64_t gm = p.cols == 256 ? 256 : 128;
   auto split = [&](int64_t tiles, int64_t len, int32_t* s, int64_t* range) {
-    int64_t want = ceil_div<int64_t>(512, tiles), most = len / (8 * bk);
+    int64_t want = ceil_div<int64_t>(gm == 256 ? 256 : 512, tiles), most = len / (8 * kDepth);
     if (want > most) want = most;
     if (want < 1) want = 1;
-    *range = up(ceil_div<int64_t>(len, want), bk);
+    *range = up(ceil_div<int64_t>(len, want), kDepth);
     *s = (int32_t)ceil_div<int64_t>(len, *range);
   };
-  split(ceil_div<int64_t>(n, 128) * ceil_div<int64_t>(K, p.bn_cols), p.piece, &p.dh_splits, &p.dh_range);
-  split(p.piece / 128 * ceil_div<int64_t>(K, p.bn_cols), n > 0 ? n : 1, &p.dw_splits, &p.dw_range);
-  const int64_t a = (int64_t)p.dh_splits * n * K * 4, b = p.dw_splits > 1 ? (int64_t)p.dw_splits * p.piece * (K + 1) * 4 : 0;
-  p.acc_bytes = up(a, 256) + up(b, 256);
+  split(ceil_div<int64_t>(n, gm) * ceil_div<int64_t>(K, p.cols), p.piece, &p.dh_splits, &p.dh_range);
+  split(ceil_div<int64_t>(p.piece, gm) * ceil_div<int64_t>(K, p.cols), up(n, kDepth), &p.dw_splits, &p.dw_range);
+  p.acc_dh = p.dh_splits > 1 || p.pieces > 1 ? up((int64_t)p.dh_splits * n * K * 4, 256) : 0;
+  p.acc_dw = p.dw_splits > 1 ? up((int64_t)p.dw_splits * p.piece * K * 4, 256) : 0;
+  p.dbp_bytes = up(p.row_tiles * C * 4, 256);
   return p;
 }
 
+template <typename T> using BigTile = Shape<typename Mul<T>::E, Mul<T>::NP, 256, 256, 2, 4>;
+template <typename T> using MidTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128, 128, 2, 2>;
+template <typename T> using SlimTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128, 64, 2, 2>;
+
+// operands in parts: in place where they are padded 16-bit rows already, else packed into h_dst / w_dst by one launch
 template <typename T>
-int lx_forward(LxArgs& a, const LxPlan& p, hipStream_t st) {
+int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* h_dst, char* w_dst, bool mask, hipStream_t st) {
+  constexpr int NP = Mul<T>::NP;
+  auto fits = [&](const void* q, int64_t ld) { return NP == 1 && d->K == p.Kp && ld % 8 == 0 && ld < (1 << 21) && (uintptr_t)q % 16 == 0; };
+  PackArgs h{}, w{};
+  if (!mask && fits(d->h, d->h_stride)) {
+    a.h = d->h; a.h_ld = d->h_stride; a.h_rows = d->n;
+  } else {
+    h = PackArgs{d->h, h_dst, d->n, p.h_rows, d->K, d->h_stride, p.Kp, d->labels, d->ignore_index, d->C};
+    a.h = h_dst; a.h_ld = p.Kp; a.h_rows = p.h_rows; a.h_part = p.h_rows * p.Kp;
+  }
+  if (fits(d->W, d->w_stride)) {
+    a.w = d->W; a.w_ld = d->w_stride;
+  } else {
+    w = PackArgs{d->W, w_dst, d->C, d->C, d->K, d->w_stride, p.Kp, nullptr, 0, 0};
+    a.w = w_dst; a.w_ld = p.Kp; a.w_part = d->C * p.Kp;
+  }
+  if (!h.dst && !w.dst) return PG_OK;
+  const int64_t most = (w.dst && (!h.dst || d->C > p.h_rows) ? d->C : p.h_rows) * (p.Kp / 8);
+  const int64_t blocks = ceil_div<int64_t>(most, 256);
+  if (!h.dst) { h = w; w = PackArgs{}; }
+  hipLaunchKernelGGL(k_lx_pack<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), w.dst ? 2 : 1), dim3(256), 0, st, h, w);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+
+template <typename T>
+int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  a.part = (float2*)s;
+  a.zlab = (float*)(s + p.part_bytes);
+  char* h = s + p.part_bytes + up(4 * a.n, 256);
+  const int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, st);
+  if (rc != PG_OK) return rc;
+  a.tiles = p.tiles;
   a.c_lo = 0;
   a.c_hi = a.C;
-  const dim3 grid((unsigned)(p.tiles * ceil_div<int64_t>(a.n, p.bn_rows)));
-  if (p.bn_rows == 64)
-    hipLaunchKernelGGL((k_lx_logits<T, 64, false>), grid, dim3(256), 0, st, a);
+  const dim3 grid((unsigned)(p.tiles * p.row_tiles));
+  if (p.big)
+    hipLaunchKernelGGL((k_lx_logits<T, BigTile<T>, false>), grid, dim3(BigTile<T>::THREADS), 0, st, a);
   else
-    hipLaunchKernelGGL((k_lx_logits<T, 128, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, false>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
   PG_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
 
-template <typename T>
-int lx_backward(LxArgs& a, const LxPlan& p, char* scratch, hipStream_t st) {
-  a.g = scratch;
-  float* acc_dh = (float*)(scratch + up(p.g_bytes, 256));
-  float* acc_dw = (float*)((char*)acc_dh + up((int64_t)p.dh_splits * a.n * a.K * 4, 256));
-  a.ldg = p.ldg;
-  const int64_t row_tiles = ceil_div<int64_t>(a.n, 128), k_tiles = ceil_div<int64_t>(a.K, p.bn_cols);
-  for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
-    a.c_hi = a.c_lo + p.piece < a.C ? a.c_lo + p.piece : a.C;
-    const int64_t len = a.c_hi - a.c_lo, c_tiles = ceil_div<int64_t>(len, 128);
-    const dim3 g1((unsigned)(c_tiles * ceil_div<int64_t>(a.n, p.bn_rows)));
-    if (p.bn_rows == 64)
-      hipLaunchKernelGGL((k_lx_logits<T, 64, true>), g1, dim3(256), 0, st, a);
-    else
-      hipLaunchKernelGGL((k_lx_logits<T, 128, true>), g1, dim3(256), 0, st, a);
-    PG_LAUNCH_CHECK();
-    if (a.dh) {
-      a.acc = acc_dh;
-      a.splits = p.dh_splits;
-      a.k_split = p.dh_range;
-      a.first = a.c_lo == 0;
-      const dim3 g2((unsigned)(row_tiles * k_tiles * a.splits));
-      if (p.bn_cols == 64)
-        hipLaunchKernelGGL((k_lx_dh<T, 64>), g2, dim3(256), 0, st, a);
-      else
-        hipLaunchKernelGGL((k_lx_dh<T, 128>), g2, dim3(256), 0, st, a);
-      PG_LAUNCH_CHECK();
-    }
-    if (a.dw || a.db) {
-      a.acc = acc_dw;
-      a.accb = p.dw_splits > 1 ? acc_dw + (int64_t)p.dw_splits * len * a.K : nullptr;
-      a.splits = p.dw_splits;
-      a.k_split = p.dw_range;
-      const dim3 g3((unsigned)(c_tiles * k_tiles * a.splits));
-      if (p.bn_cols == 64)
-        hipLaunchKernelGGL((k_lx_dw<T, 64>), g3, dim3(256), 0, st, a);
-      else
-        hipLaunchKernelGGL((k_lx_dw<T, 128>), g3, dim3(256), 0, st, a);
-      PG_LAUNCH_CHECK();
-      if (a.splits > 1) {
-        const int64_t b = ceil_div<int64_t>(len * (a.K + 1), 256);
-        hipLaunchKernelGGL(k_lx_dw_out<T>, dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(256), 0, st, a);
-        PG_LAUNCH_CHECK();
-      }
-    }
-  }
+template <typename T, typename S>
+int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipStream_t st) {
+  const int64_t k_tiles = ceil_div<int64_t>(a.K, S::BN), len = a.c_hi - a.c_lo;
   if (a.dh) {
     a.acc = acc_dh;
     a.splits = p.dh_splits;
-    const int64_t b = ceil_div<int64_t>(a.n * a.K, 256);
-    hipLaunchKernelGGL(k_lx_dh_out<T>, dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(256), 0, st, a);
+    a.range = p.dh_range;
+    a.first = a.c_lo == 0;
+    a.direct = p.dh_splits == 1 && p.pieces == 1;
+    hipLaunchKernelGGL((k_lx_dh<T, S>), dim3((unsigned)(ceil_div<int64_t>(a.n, S::BM) * k_tiles * a.splits)), dim3(S::THREADS), 0, st, a);
+    PG_LAUNCH_CHECK();
+  }
+  if (a.dw) {
+    a.acc = acc_dw;
+    a.splits = p.dw_splits;
+    a.range = p.dw_range;
+    hipLaunchKernelGGL((k_lx_dw<T, S>), dim3((unsigned)(ceil_div<int64_t>(len, S::BM) * k_tiles * a.splits)), dim3(S::THREADS), 0, st, a);
+    PG_LAUNCH_CHECK();
+    if (a.splits > 1) {
+      const int64_t b = ceil_div<int64_t>(len * a.K, 256);
+      hipLaunchKernelGGL(k_lx_dw_out<T>, dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(256), 0, st, a);
+      PG_LAUNCH_CHECK();
+    }
+  }
+  return PG_OK;
+}
+
+template <typename T>
+int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  a.g = s;
+  s += p.g_bytes;
+  float* acc_dh = (float*)s;
+  s += p.acc_dh;
+  float* acc_dw = (float*)s;
+  s += p.acc_dw;
+  a.dbp = (float*)s;
+  s += p.dbp_bytes;
+  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, st);
+  if (rc != PG_OK) return rc;
+  a.ldg = p.ldg;
+  a.g_rows = p.g_rows;
+  for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
+    a.c_hi = a.c_lo + p.piece < a.C ? a.c_lo + p.piece : a.C;
+    const dim3 grid((unsigned)(ceil_div<int64_t>(a.c_hi - a.c_lo, p.big ? 256 : 128) * p.row_tiles));
+    if (p.big)
+      hipLaunchKernelGGL((k_lx_logits<T, BigTile<T>, true>), grid, dim3(BigTile<T>::THREADS), 0, st, a);
+    else
+      hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, true>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
+    PG_LAUNCH_CHECK();
+    rc = p.cols == 256 ? lx_gradients<T, BigTile<T>>(a, p, acc_dh, acc_dw, st)
+       : p.cols == 128 ? lx_gradients<T, MidTile<T>>(a, p, acc_dh, acc_dw, st)
+                       : lx_gradients<T, SlimTile<T>>(a, p, acc_dh, acc_dw, st);
+    if (rc != PG_OK) return rc;
+  }
+  a.direct = p.dh_splits == 1 && p.pieces == 1;
+  if ((a.dh && !a.direct) || a.db) {
+    a.acc = acc_dh;
+    a.splits = p.dh_splits;
+    const int64_t b = ceil_div<int64_t>(a.dh && !a.direct ? (a.n * a.K > a.C ? a.n * a.K : a.C) : a.C, 256);
+    hipLaunchKernelGGL(k_lx_sums<T>, dim3((unsigned)(b > 4096 ? 4096 : b), 2), dim3(256), 0, st, a, p.row_tiles);
     PG_LAUNCH_CHECK();
   }
   return PG_OK;
 }
 
-// the grids are one-dimensional: every product's tile count has to fit
+// the grids are one-dimensional, and a tile's offsets have 32 bits
 inline int lx_check(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   if (n < 0 || K <= 0 || C <= 0 || dtype < PG_DTYPE_F32 || dtype > PG_DTYPE_F16) return PG_ERR_INVALID;
-  if (n > (int64_t(1) << 31) || K > (int64_t(1) << 24) || C > (int64_t(1) << 31)) return PG_ERR_UNSUPPORTED;
-  if (ceil_div<int64_t>(n, 64) * ceil_div<int64_t>(C, 128) > 0x7fffffffll / 2) return PG_ERR_UNSUPPORTED;
+  if (n > (int64_t(1) << 31) || K > (int64_t(1) << 20) || C > (int64_t(1) << 31)) return PG_ERR_UNSUPPORTED;
+  if (ceil_div<int64_t>(n, 128) * ceil_div<int64_t>(C, 128) > 0x7fffffffll / 2) return PG_ERR_UNSUPPORTED;
   return PG_OK;
 }
 
@@ -615,11 +602,11 @@ int lx_args(const pg_linear_xent_desc_t* d, LxArgs* a) {
   if (!d) return PG_ERR_INVALID;
   const int rc = lx_check(d->n, d->K, d->C, d->dtype);
   if (rc != PG_OK) return rc;
-  if (d->h_stride < d->K || d->w_stride < d->K) return PG_ERR_INVALID;
-  if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->lse || !d->flag))) return PG_ERR_INVALID;
+  if ((d->h_stride < d->K && d->h_stride != 0) || d->w_stride < d->K) return PG_ERR_INVALID;
+  if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->lse || !d->flag || !d->scratch))) return PG_ERR_INVALID;
   *a = LxArgs{};
-  a->h = d->h; a->w = d->W; a->bias = d->bias; a->labels = d->labels;
-  a->n = d->n; a->K = d->K; a->C = d->C; a->hs = d->h_stride; a->ws = d->w_stride; a->ignore = d->ignore_index;
+  a->bias = d->bias; a->labels = d->labels;
+  a->n = d->n; a->K = d->K; a->Kp = up(d->K, kDepth); a->C = d->C; a->ignore = d->ignore_index;
   a->lse = d->lse; a->flag = d->flag; a->row_loss = d->row_loss; a->meta = d->meta;
   return PG_OK;
 }
@@ -634,7 +621,8 @@ int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, i
   if (lx_check(n, K, C, dtype) != PG_OK) return -1;
   if (n == 0) return 0;
   const LxPlan p = lx_plan(n, K, C, dtype);
-  return backward ? up(p.g_bytes, 256) + p.acc_bytes + up(4 * n, 256) + 256 : up(p.part_bytes, 256) + up(4 * n, 256);
+  const int64_t ops = p.h_bytes + p.w_bytes;
+  return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + up(4 * n, 256) + ops;
 }
 
 int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
@@ -643,12 +631,11 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   if (rc != PG_OK) return rc;
   hipStream_t st = as_stream(stream);
   if (a.n > 0) {
-    if (!d->row_loss || !d->scratch) return PG_ERR_INVALID;
+    if (!d->row_loss) return PG_ERR_INVALID;
     const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype);
-    a.part = (float2*)d->scratch;
-    a.zlab = (float*)((char*)d->scratch + up(p.part_bytes, 256));
-    a.tiles = p.tiles;
-    rc = d->dtype == PG_DTYPE_F32 ? lx_forward<float>(a, p, st) : d->dtype == PG_DTYPE_BF16 ? lx_forward<bf16_t>(a, p, st) : lx_forward<f16_t>(a, p, st);
+    char* s = (char*)d->scratch;
+    rc = d->dtype == PG_DTYPE_F32 ? lx_forward<float>(a, d, p, s, st) : d->dtype == PG_DTYPE_BF16 ? lx_forward<bf16_t>(a, d, p, s, st)
+                                                                                                  : lx_forward<f16_t>(a, d, p, s, st);
     if (rc != PG_OK) return rc;
   }
   hipLaunchKernelGGL(k_lx_mean, dim3(1), dim3(1024), 0, st, a.row_loss, a.flag, a.n, a.meta);
@@ -658,18 +645,17 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
 
 int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   LxArgs a;
-  int rc = lx_args(d, &a);
+  const int rc = lx_args(d, &a);
   if (rc != PG_OK) return rc;
   if (!d->grad || d->reduction < PG_XENT_MEAN || d->reduction > PG_XENT_NONE) return PG_ERR_INVALID;
   if (a.n == 0) return PG_ERR_INVALID;            // no row, no gradient to compute: the caller's zeros
-  if (!d->scratch) return PG_ERR_INVALID;
   hipStream_t st = as_stream(stream);
   const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype);
   char* s = (char*)d->scratch;
   a.dh = d->dh; a.dw = d->dW; a.db = d->db;
   if (d->reduction == PG_XENT_NONE) {
-    float* rowf = (float*)(s + up(p.g_bytes, 256) + p.acc_bytes);
-    float* top = (float*)((char*)rowf + up(4 * a.n, 256));
+    float* rowf = (float*)s;
+    float* top = (float*)(s + up(4 * a.n, 256));
     hipLaunchKernelGGL(k_lx_row_factors, dim3(1), dim3(1024), 0, st, d->grad, d->grad_stride, a.flag, a.n, rowf, top);
     PG_LAUNCH_CHECK();
     a.rowf = rowf;
@@ -679,7 +665,9 @@ int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
     a.f1 = d->grad;
     a.f2 = d->reduction == PG_XENT_MEAN ? a.meta + 1 : nullptr;
   }
-  return d->dtype == PG_DTYPE_F32 ? lx_backward<float>(a, p, s, st) : d->dtype == PG_DTYPE_BF16 ? lx_backward<bf16_t>(a, p, s, st) : lx_backward<f16_t>(a, p, s, st);
+  s += up(4 * a.n, 256) + 256;
+  return d->dtype == PG_DTYPE_F32 ? lx_backward<float>(a, d, p, s, st) : d->dtype == PG_DTYPE_BF16 ? lx_backward<bf16_t>(a, d, p, s, st)
+                                                                                                   : lx_backward<f16_t>(a, d, p, s, st);
 }
 
 }  // extern "C"
