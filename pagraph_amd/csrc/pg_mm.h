@@ -59,7 +59,7 @@ struct TileLoad {
     for (int t = 0; t < T; ++t) {
       const int piece = wave * T + t;
       if constexpr (KIND == ROWS) {
-        const int r = piece * 8 + lane / 8, chunk = (lane & 7) ^ (r & 7);
+        const int r = piece * 8 + lane / 8, chunk = (lane & 7) ^ ((r >> 1) & 7);
         const int64_t last = o.rows - 1 - o.r0;
         row[t] = (uint32_t)(r < last ? r : last) * ld2 + chunk * 16;
       } else {
@@ -94,7 +94,7 @@ template <int KIND, int R>
 __device__ __forceinline__ s16x8 fragment(const short* lds, int rb, int kk, int lane) {
   if constexpr (KIND == ROWS) {
     const int r = rb + (lane & 31), chunk = kk * 2 + (lane >> 5);
-    return *reinterpret_cast<const s16x8*>(lds + r * kDepth + ((chunk ^ (r & 7)) << 3));
+    return *reinterpret_cast<const s16x8*>(lds + r * kDepth + ((chunk ^ ((r >> 1) & 7)) << 3));
   } else {
     const int i = lane & 15, g = lane >> 4;
     const int k = kk * 16 + (g >> 1) * 8 + (i >> 2), chunk = (rb >> 3) + (g & 1) * 2 + ((i & 3) >> 1);

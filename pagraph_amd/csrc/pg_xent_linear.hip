@@ -13,7 +13,7 @@
 // G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-9, fp16 2^-12 relative),
 // independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
 // of 2^-28 is still a normal number.
-#include "pg_mm.h"
+#include "pg_xent_narrow.h"
 
 namespace pg {
 
@@ -61,9 +61,50 @@ struct PackArgs {
   const int64_t* labels;
   int64_t ignore, C;
 };
+// what the narrow form reads beside the operands, padded past the last class / row (see NxArgs): base-2 biases, labels as int32,
+// and for the gradients the rows' lse (less the exponent of G's scale) and factors
+struct SideArgs {
+  const void* bias;
+  float *bias2, *lse2, *rowf2;             // bias2 == NULL: nothing to do; lse2 == NULL: no gradients
+  int32_t* lab;
+  const float *lse, *rowf;
+  const int64_t* labels;
+  int64_t n, rows_p, C, classes_p, ignore;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1) {
+__device__ __forceinline__ void lx_side(const SideArgs& a) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.classes_p || i < a.rows_p; i += (int64_t)gridDim.x * 256) {
+    if (i < a.classes_p) {
+      float b = i < a.C ? 0.f : -INFINITY;
+      if (i < a.C && a.bias) {
+        b = (float)((const T*)a.bias)[i];
+        // (a finite lowest value stays finite: a row of nothing else is uniform, not empty)
+        b = b == -INFINITY ? b : b * kLog2e < -3.402823466e38f ? -3.402823466e38f : b * kLog2e;
+      }
+      a.bias2[i] = b;
+    }
+    if (i < a.rows_p) {
+      const int64_t lab = i < a.n ? a.labels[i] : -1;
+      const bool ok = i < a.n && lab != a.ignore && lab >= 0 && lab < a.C;
+      if (a.lse2) {
+        const float f = ok ? a.rowf[i] : 0.f;
+        a.lse2[i] = f != 0.f ? a.lse[i] - __builtin_log2f(Mul<T>::G) : INFINITY;       // rows without a gradient: exponentials of 0
+        a.rowf2[i] = f;
+        a.lab[i] = f != 0.f ? (int32_t)lab : -1;
+      } else {
+        a.lab[i] = ok ? (int32_t)lab : -1;
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1, SideArgs side) {
   typedef typename Mul<T>::E E;
+  if (blockIdx.y == 2) {
+    if (side.bias2) lx_side<T>(side);
+    return;
+  }
   const PackArgs& a = blockIdx.y ? a1 : a0;
   if (!a.dst) return;
   const int64_t ch = a.ldp / 8, total = a.rows_p * ch;
@@ -241,8 +282,9 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   }
 }
 
-// a wave per row: joins the tiles' statistics
-__global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
+// a wave per row: joins the tiles' (narrow form: the splits') statistics. unit: log2(e), or 1 where they are in base 2 already;
+// the lse is kept in the same unit
+__global__ __launch_bounds__(256) void k_lx_rows(LxArgs a, float unit) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (r >= a.n) return;
@@ -250,22 +292,22 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
   for (int64_t t = lane; t < a.tiles; t += 64) {
     const float2 x = a.part[r * a.tiles + t];
     const float mm = fmaxf(m, x.x), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f((m - base) * kLog2e) + x.y * __builtin_amdgcn_exp2f((x.x - base) * kLog2e);
+    s = s * __builtin_amdgcn_exp2f((m - base) * unit) + x.y * __builtin_amdgcn_exp2f((x.x - base) * unit);
     m = mm;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float om = __shfl_xor(m, o, kWave), os = __shfl_xor(s, o, kWave);
     const float mm = fmaxf(m, om), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f((m - base) * kLog2e) + os * __builtin_amdgcn_exp2f((om - base) * kLog2e);
+    s = s * __builtin_amdgcn_exp2f((m - base) * unit) + os * __builtin_amdgcn_exp2f((om - base) * unit);
     m = mm;
   }
   if (lane == 0) {
-    const float lse = m + logf(s);
+    const float lse = m + (unit == 1.f ? log2f(s) : logf(s));
     const bool ok = label_ok(a.labels[r], a);
     a.lse[r] = lse;
     a.flag[r] = ok ? 1.f : 0.f;
-    a.row_loss[r] = ok ? lse - a.zlab[r] : 0.f;
+    a.row_loss[r] = ok ? (lse - a.zlab[r]) * (unit == 1.f ? 0.693147180559945309417f : 1.f) : 0.f;
   }
 }
 
@@ -354,33 +396,48 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
     each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
   } else {
     float* out = a.acc + sp * a.n * a.K + r0 * a.K + n0;
+    // (rows that do not count leave as zeros, whatever W holds)
     if (a.first)
-      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = v; });
+      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? 0.f : v; });
     else
-      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] += v; });
+      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] += a.rowf[r0 + r] == 0.f ? 0.f : v; });
   }
 }
 
-// the splits of dh added in order; blockIdx.y == 1: the row tiles' partial sums of db likewise
+// partial sums added in order: out[i] = (sum over splits of acc[split][i]) * factor. Up to three such sums a launch
+struct SumArgs {
+  const float* acc;
+  void* out;
+  int64_t total, splits;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_lx_sums(LxArgs a, int64_t row_tiles) {
-  const float f = out_factor(a) / Mul<T>::G;
-  if (blockIdx.y == 0) {
-    if (!a.dh || a.direct) return;
-    const int64_t total = a.n * a.K;
-    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-      float s = 0.f;
-      for (int i = 0; i < a.splits; ++i) s += a.acc[i * total + t];
-      ((T*)a.dh)[t] = a.rowf[t / a.K] == 0.f ? (T)0.f : (T)(s * f);
+__global__ __launch_bounds__(256) void k_lx_sums(SumArgs a0, SumArgs a1, SumArgs a2, const float* f1, const float* f2) {
+  const SumArgs& a = blockIdx.y == 0 ? a0 : blockIdx.y == 1 ? a1 : a2;
+  if (!a.out) return;
+  const float f = (f1 ? *f1 : 1.f) * (f2 ? *f2 : 1.f) / Mul<T>::G;
+  for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; t < a.total; t += (int64_t)gridDim.x * 1024) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
+#pragma unroll 4
+    for (int64_t i = 0; i < a.splits; ++i) {
+      load4_tail(a.acc + i * a.total + t, a.total - t, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v[e];
     }
-  } else {
-    if (!a.db) return;
-    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < a.C; c += (int64_t)gridDim.x * 256) {
-      float s = 0.f;
-      for (int64_t i = 0; i < row_tiles; ++i) s += a.dbp[i * a.C + c];
-      ((T*)a.db)[c] = (T)(s * f);
-    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] *= f;
+    store4_tail((T*)a.out + t, a.total - t, s);
   }
+}
+template <typename T>
+int lx_sums(const SumArgs& a, const SumArgs& b, const SumArgs& c, const LxArgs& x, hipStream_t st) {
+  int64_t most = a.out ? a.total : 0;
+  if (b.out && b.total > most) most = b.total;
+  if (c.out && c.total > most) most = c.total;
+  if (most == 0) return PG_OK;
+  const int64_t blocks = ceil_div<int64_t>(most, 1024);
+  hipLaunchKernelGGL(k_lx_sums<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), c.out ? 3 : b.out ? 2 : 1), dim3(256), 0, st, a, b, c, x.f1, x.f2);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
 }
 
 // dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]
@@ -409,18 +466,6 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
   }
 }
 
-// the splits of one piece's dW added in order
-template <typename T>
-__global__ __launch_bounds__(256) void k_lx_dw_out(LxArgs a) {
-  const float f = out_factor(a) / Mul<T>::G;
-  const int64_t total = (a.c_hi - a.c_lo) * a.K;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (int i = 0; i < a.splits; ++i) s += a.acc[i * total + t];
-    ((T*)a.dw)[a.c_lo * a.K + t] = (T)(s * f);
-  }
-}
-
 inline int64_t up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
 
 // sizes of one call: everything follows from the shapes, types and alignments of the operands, so that the scratch the caller
@@ -431,7 +476,26 @@ struct LxPlan {
   int32_t dh_splits, dw_splits, pieces;
   int64_t dh_range, dw_range;
   int big, cols;                            // tile shapes: 256 x 256 logits; columns of a gradient tile
+  // narrow form
+  int narrow, xt_stats, xt_grad, yt;
+  int32_t nx_stats, nx_dh, nx_dw;           // splits
+  int64_t rs_stats, rs_dh, rs_dw;           // their ranges
+  int64_t classes_p, rows_p, side_bytes;
 };
+
+// splits of the narrow form's y for t tiles of x: every CU gets the same number of workgroups, or nearly, and at least two of them
+// where there is that much work; a split adds a partial result to write and to sum
+inline void narrow_split(int64_t t, int64_t y_tiles, int32_t* splits, int64_t* range, int64_t yt) {
+  int64_t best = 1;
+  double cost = 1e30;
+  for (int64_t s = 1; s <= 512 && s * 4 <= y_tiles + 3; ++s) {
+    const double c = (double)ceil_div<int64_t>(t * s, 256) / (double)s + (t * s < 512 ? 0.25 * (double)t / 256. : 0.) + 0.002 * (double)(t * s) / 256.;
+    if (c < cost) { cost = c; best = s; }
+  }
+  const int64_t r = ceil_div<int64_t>(y_tiles, best);
+  *range = r * yt;
+  *splits = (int32_t)ceil_div<int64_t>(y_tiles, r);
+}
 
 inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   LxPlan p{};
@@ -440,6 +504,23 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   p.h_rows = up(n, 256);
   p.h_bytes = up(np * p.h_rows * p.Kp * 2, 256);
   p.w_bytes = up(np * C * p.Kp * 2, 256);
+  p.narrow = p.Kp <= (np == 3 ? 128 : 256);
+  if (p.narrow) {
+    p.xt_stats = 128 * narrow_xb((int)np, (int)p.Kp, NX_STATS);
+    p.xt_grad = 128 * narrow_xb((int)np, (int)p.Kp, NX_DH);
+    p.yt = np * p.Kp <= 256 ? 64 : 32;
+    const int64_t classes = ceil_div<int64_t>(C, p.yt);
+    narrow_split(ceil_div<int64_t>(n, p.xt_stats), classes, &p.nx_stats, &p.rs_stats, p.yt);
+    narrow_split(ceil_div<int64_t>(n, p.xt_grad), classes, &p.nx_dh, &p.rs_dh, p.yt);
+    narrow_split(ceil_div<int64_t>(C, p.xt_grad), ceil_div<int64_t>(n, p.yt), &p.nx_dw, &p.rs_dw, p.yt);
+    p.part_bytes = up(n * p.nx_stats * 8, 256);
+    p.acc_dh = p.nx_dh > 1 ? up((int64_t)p.nx_dh * n * K * 4, 256) : 0;
+    p.acc_dw = p.nx_dw > 1 ? up((int64_t)p.nx_dw * C * (K + 1) * 4, 256) : 0;
+    p.classes_p = up(C, 256) + 64;
+    p.rows_p = p.h_rows + 64;
+    p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
+    return p;
+  }
   p.big = n > 128 && C > 128 && p.Kp * np >= 256;
   const int64_t bm = p.big ? 256 : 128;
   p.tiles = ceil_div<int64_t>(C, bm);
@@ -479,7 +560,7 @@ template <typename T> using SlimTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128
 
 // operands in parts: in place where they are padded 16-bit rows already, else packed into h_dst / w_dst by one launch
 template <typename T>
-int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* h_dst, char* w_dst, bool mask, hipStream_t st) {
+int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* h_dst, char* w_dst, bool mask, const SideArgs& side, hipStream_t st) {
   constexpr int NP = Mul<T>::NP;
   auto fits = [&](const void* q, int64_t ld) { return NP == 1 && d->K == p.Kp && ld % 8 == 0 && ld < (1 << 21) && (uintptr_t)q % 16 == 0; };
   PackArgs h{}, w{};
@@ -495,21 +576,120 @@ int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
     w = PackArgs{d->W, w_dst, d->C, d->C, d->K, d->w_stride, p.Kp, nullptr, 0, 0};
     a.w = w_dst; a.w_ld = p.Kp; a.w_part = d->C * p.Kp;
   }
-  if (!h.dst && !w.dst) return PG_OK;
-  const int64_t most = (w.dst && (!h.dst || d->C > p.h_rows) ? d->C : p.h_rows) * (p.Kp / 8);
+  if (!h.dst && !w.dst && !side.bias2) return PG_OK;
+  const int64_t most = (w.dst && (!h.dst || d->C > p.h_rows) ? d->C : h.dst ? p.h_rows : 32) * (p.Kp / 8);
   const int64_t blocks = ceil_div<int64_t>(most, 256);
   if (!h.dst) { h = w; w = PackArgs{}; }
-  hipLaunchKernelGGL(k_lx_pack<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), w.dst ? 2 : 1), dim3(256), 0, st, h, w);
+  hipLaunchKernelGGL(k_lx_pack<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), side.bias2 ? 3 : w.dst ? 2 : 1), dim3(256), 0, st, h, w, side);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+
+template <typename T, int KP, int MODE>
+int launch_narrow_kp(const NxArgs& n, hipStream_t st) {
+  constexpr int XB = narrow_xb(Mul<T>::NP, KP, MODE);
+  hipLaunchKernelGGL((k_lx_narrow<T, KP, XB, MODE>), dim3((unsigned)(ceil_div<int64_t>(n.nx, 128 * XB) * n.splits)), dim3(256), 0, st, n);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+template <typename T, int MODE>
+int launch_narrow(const NxArgs& n, const LxPlan& p, hipStream_t st) {
+  if (p.Kp == 64) return launch_narrow_kp<T, 64, MODE>(n, st);
+  if constexpr (Mul<T>::NP == 1) {
+    if (p.Kp == 192) return launch_narrow_kp<T, 192, MODE>(n, st);
+    if (p.Kp == 256) return launch_narrow_kp<T, 256, MODE>(n, st);
+  }
+  return launch_narrow_kp<T, 128, MODE>(n, st);
+}
+
+// the side arrays at s, in the order bias2 | labels | lse | row factors
+inline SideArgs narrow_side(const LxArgs& a, const LxPlan& p, char* s, bool grads) {
+  SideArgs side{};
+  const int64_t rows = up(p.rows_p * 4, 256);
+  side.bias = a.bias; side.labels = a.labels; side.ignore = a.ignore;
+  side.n = a.n; side.rows_p = p.rows_p; side.C = a.C; side.classes_p = p.classes_p;
+  side.bias2 = (float*)s;
+  side.lab = (int32_t*)(s + up(p.classes_p * 4, 256));
+  if (grads) {
+    side.lse2 = (float*)((char*)side.lab + rows);
+    side.rowf2 = (float*)((char*)side.lab + 2 * rows);
+    side.lse = a.lse; side.rowf = a.rowf;
+  }
+  return side;
+}
+
+inline NxArgs narrow_args(const LxArgs& a, bool classes_are_x) {
+  NxArgs n{};
+  if (classes_are_x) {
+    n.x = a.w; n.x_ld = a.w_ld; n.x_part = a.w_part; n.x_rows = a.C; n.nx = a.C;
+    n.y = a.h; n.y_ld = a.h_ld; n.y_part = a.h_part; n.y_rows = a.h_rows; n.ny = a.n;
+  } else {
+    n.x = a.h; n.x_ld = a.h_ld; n.x_part = a.h_part; n.x_rows = a.h_rows; n.nx = a.n;
+    n.y = a.w; n.y_ld = a.w_ld; n.y_part = a.w_part; n.y_rows = a.C; n.ny = a.C;
+  }
+  n.K = a.K; n.f1 = a.f1; n.f2 = a.f2;
+  return n;
+}
+
+template <typename T>
+int narrow_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  a.part = (float2*)s;
+  a.zlab = (float*)(s + p.part_bytes);
+  char* h = s + p.part_bytes + up(4 * a.n, 256);
+  const SideArgs side = narrow_side(a, p, h + p.h_bytes + p.w_bytes, false);
+  int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, side, st);
+  if (rc != PG_OK) return rc;
+  NxArgs n = narrow_args(a, false);
+  n.side0 = side.bias2; n.xlab = side.lab; n.part = a.part; n.zlab = a.zlab;
+  n.splits = p.nx_stats; n.range = p.rs_stats;
+  rc = launch_narrow<T, NX_STATS>(n, p, st);
+  if (rc != PG_OK) return rc;
+  a.tiles = p.nx_stats;
+  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a, 1.f);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
 
 template <typename T>
+int narrow_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  float* acc_dh = (float*)s;
+  s += p.acc_dh;
+  float* acc_dw = (float*)s;
+  s += p.acc_dw;
+  const SideArgs side = narrow_side(a, p, s + p.h_bytes + p.w_bytes, true);
+  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, side, st);
+  if (rc != PG_OK) return rc;
+  SumArgs dh{}, dw{}, db{};
+  if (a.dh) {
+    NxArgs n = narrow_args(a, false);
+    n.side0 = side.bias2; n.xa = side.lse2; n.xb = side.rowf2; n.xlab = side.lab;
+    n.splits = p.nx_dh; n.range = p.rs_dh; n.acc = acc_dh; n.out = a.dh;
+    rc = launch_narrow<T, NX_DH>(n, p, st);
+    if (rc != PG_OK) return rc;
+    if (n.splits > 1) dh = SumArgs{acc_dh, a.dh, a.n * a.K, n.splits};
+  }
+  if (a.dw || a.db) {
+    NxArgs n = narrow_args(a, true);
+    n.side0 = side.lse2; n.side1 = (const float*)side.lab; n.side2 = side.rowf2; n.xa = side.bias2;
+    n.scaled = a.rowf != a.flag;
+    n.splits = p.nx_dw; n.range = p.rs_dw; n.acc = acc_dw; n.accb = acc_dw + (int64_t)p.nx_dw * a.C * a.K; n.out = a.dw; n.outb = a.db;
+    rc = launch_narrow<T, NX_DW>(n, p, st);
+    if (rc != PG_OK) return rc;
+    if (n.splits > 1) {
+      if (a.dw) dw = SumArgs{acc_dw, a.dw, a.C * a.K, n.splits};
+      if (a.db) db = SumArgs{n.accb, a.db, a.C, n.splits};
+    }
+  }
+  return lx_sums<T>(dh, dw, db, a, st);
+}
+
+template <typename T>
 int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  if (p.narrow) return narrow_forward<T>(a, d, p, s, st);
   a.part = (float2*)s;
   a.zlab = (float*)(s + p.part_bytes);
   char* h = s + p.part_bytes + up(4 * a.n, 256);
-  const int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, st);
+  const int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, SideArgs{}, st);
   if (rc != PG_OK) return rc;
   a.tiles = p.tiles;
   a.c_lo = 0;
@@ -520,7 +700,7 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   else
     hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, false>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
   PG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a, kLog2e);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
@@ -543,17 +723,14 @@ int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipSt
     a.range = p.dw_range;
     hipLaunchKernelGGL((k_lx_dw<T, S>), dim3((unsigned)(ceil_div<int64_t>(len, S::BM) * k_tiles * a.splits)), dim3(S::THREADS), 0, st, a);
     PG_LAUNCH_CHECK();
-    if (a.splits > 1) {
-      const int64_t b = ceil_div<int64_t>(len * a.K, 256);
-      hipLaunchKernelGGL(k_lx_dw_out<T>, dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(256), 0, st, a);
-      PG_LAUNCH_CHECK();
-    }
+    if (a.splits > 1) return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, len * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
   }
   return PG_OK;
 }
 
 template <typename T>
 int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
+  if (p.narrow) return narrow_backward<T>(a, d, p, s, st);
   a.g = s;
   s += p.g_bytes;
   float* acc_dh = (float*)s;
@@ -562,7 +739,7 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   s += p.acc_dw;
   a.dbp = (float*)s;
   s += p.dbp_bytes;
-  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, st);
+  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, SideArgs{}, st);
   if (rc != PG_OK) return rc;
   a.ldg = p.ldg;
   a.g_rows = p.g_rows;
@@ -579,15 +756,8 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
                        : lx_gradients<T, SlimTile<T>>(a, p, acc_dh, acc_dw, st);
     if (rc != PG_OK) return rc;
   }
-  a.direct = p.dh_splits == 1 && p.pieces == 1;
-  if ((a.dh && !a.direct) || a.db) {
-    a.acc = acc_dh;
-    a.splits = p.dh_splits;
-    const int64_t b = ceil_div<int64_t>(a.dh && !a.direct ? (a.n * a.K > a.C ? a.n * a.K : a.C) : a.C, 256);
-    hipLaunchKernelGGL(k_lx_sums<T>, dim3((unsigned)(b > 4096 ? 4096 : b), 2), dim3(256), 0, st, a, p.row_tiles);
-    PG_LAUNCH_CHECK();
-  }
-  return PG_OK;
+  const bool direct = p.dh_splits == 1 && p.pieces == 1;
+  return lx_sums<T>(SumArgs{acc_dh, direct ? nullptr : a.dh, a.n * a.K, p.dh_splits}, SumArgs{a.dbp, a.db, a.C, p.row_tiles}, SumArgs{}, a, st);
 }
 
 // the grids are one-dimensional, and a tile's offsets have 32 bits
@@ -621,7 +791,7 @@ int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, i
   if (lx_check(n, K, C, dtype) != PG_OK) return -1;
   if (n == 0) return 0;
   const LxPlan p = lx_plan(n, K, C, dtype);
-  const int64_t ops = p.h_bytes + p.w_bytes;
+  const int64_t ops = p.h_bytes + p.w_bytes + p.side_bytes;
   return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + up(4 * n, 256) + ops;
 }
 
