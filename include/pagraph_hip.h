@@ -597,7 +597,7 @@ int pg_dropout_apply(const void* x, int64_t x_stride, void* y, int64_t y_stride,
  *           pg_dropout_apply otherwise). mean / rstd [n] fp32: both or neither (no gradient wanted). step_used: as above.
  * backward: `sum` = the rows that were normalised (x without a residual), gy and optionally gsum (gradient of the handed-on sum):
  *           ds = rstd (gh - mean(gh) - xh mean(gh xh)) + gsum with gh = gy weight; dres = ds, dx = dropout's gradient of ds; dw, db
- *           summed over the rows in a fixed order through partials (pg_layer_norm_scratch(n, d) floats). Each of dx, dres, dw, db
+ *           summed over the rows in a fixed order through partials (pg_layer_norm_scratch(n, d, dtype) floats). Each of dx, dres, dw, db
  *           may be NULL. n == 0 writes zeros to dw, db.
  * weight / bias (either may be NULL: 1 / 0) and dw / db are of param_dtype: dtype's or PG_DTYPE_F32. d <= PG_NORM_MAX_COLUMNS
  * (a row lives in one workgroup's registers; wider: PG_ERR_UNSUPPORTED).                                                      */
@@ -626,7 +626,7 @@ typedef struct pg_norm_desc {
   pg_dropout_t drop;
 } pg_norm_desc_t;
 int pg_layer_norm_fwd(const pg_norm_desc_t* desc, pg_stream_t stream);
-int64_t pg_layer_norm_scratch(int64_t n, int64_t d);
+int64_t pg_layer_norm_scratch(int64_t n, int64_t d, int32_t dtype);
 int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
 /* CrossEntropyLoss(h W^T + bias, labels) for any number of classes without the logits [n, C] in memory (a wide head's counterpart
  * of pg_head + pg_xent_*): h [n, K], W [C, K], bias [C] or NULL, all of `dtype`. Rows whose label is ignore_index or outside

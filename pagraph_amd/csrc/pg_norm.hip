@@ -17,43 +17,89 @@
 namespace pg {
 
 // pairs of pieces of a row of d columns (the counter's second word runs over [0, pairs))
-__host__ __device__ inline int64_t row_pairs(int64_t d) {
+__host__ __device__ inline int row_pairs(int64_t d) {
   const int64_t rem = d % 512, last = (rem + 3) / 4;
-  return d / 512 * 64 + (last > 64 ? 64 : last);
-}
-__device__ __forceinline__ int64_t pair_col(int64_t q) { return (q >> 6) * 512 + (q & 63) * 4; }
-
-__device__ __forceinline__ void drop4(float (&v)[4], uint32_t w0, uint32_t w1, uint32_t thr, float scale) {
-  v[0] = (w0 & 0xffffu) >= thr ? v[0] * scale : 0.f;
-  v[1] = (w0 >> 16) >= thr ? v[1] * scale : 0.f;
-  v[2] = (w1 & 0xffffu) >= thr ? v[2] * scale : 0.f;
-  v[3] = (w1 >> 16) >= thr ? v[3] * scale : 0.f;
+  return (int)(d / 512 * 64 + (last > 64 ? 64 : last));
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_t xs, T* __restrict__ y, int64_t ys, int64_t n,
-                                                 int64_t d, int64_t nq, int32_t rows_per_block, float inv_nq, DropArgs dr,
-                                                 uint64_t* step_used) {
+// A unit of work is V neighbouring pairs: 4 V columns from unit_col on and 4 V columns 256 further. V = 2 for 16-bit rows of whole
+// 16-byte pieces (d % 8 == 0), else 1. RAGGED: d is no multiple of 4 V, a row's last piece is moved element by element.
+template <int V>
+__device__ __forceinline__ int unit_col(int u) {
+  const int q = u * V;
+  return (q >> 6) * 512 + (q & 63) * 4;
+}
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void load_piece(const T* __restrict__ row, int c, int d, float (&v)[4 * V]) {
+  if (c + 4 * V <= d) {
+    T t[4 * V];
+    __builtin_memcpy(t, row + c, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) v[i] = RAGGED && c + i < d ? (float)row[c + i] : 0.f;
+  }
+}
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void store_piece(T* __restrict__ row, int c, int d, const float (&v)[4 * V]) {
+  if (c + 4 * V <= d) {
+    T t[4 * V];
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) t[i] = (T)v[i];
+    __builtin_memcpy(row + c, t, sizeof(t));
+  } else if (RAGGED) {
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i)
+      if (c + i < d) row[c + i] = (T)v[i];
+  }
+}
+
+struct UnitMask {
+  uint32_t w[4];
+};
+template <int V>
+__device__ __forceinline__ void draw_unit(const DropArgs& dr, uint32_t step, uint32_t r, int u, UnitMask (&m)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) Philox::gen(r, (uint32_t)(u * V + k), dr.tag, step, dr.k0, dr.k1, m[k].w);
+}
+// half 0: the unit's first 4 V columns, half 1: those 256 further
+template <int V>
+__device__ __forceinline__ void drop_piece(float (&v)[4 * V], const UnitMask (&m)[V], int half, uint32_t thr, float scale) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const uint32_t w0 = m[k].w[2 * half], w1 = m[k].w[2 * half + 1];
+    v[4 * k] = (w0 & 0xffffu) >= thr ? v[4 * k] * scale : 0.f;
+    v[4 * k + 1] = (w0 >> 16) >= thr ? v[4 * k + 1] * scale : 0.f;
+    v[4 * k + 2] = (w1 & 0xffffu) >= thr ? v[4 * k + 2] * scale : 0.f;
+    v[4 * k + 3] = (w1 >> 16) >= thr ? v[4 * k + 3] * scale : 0.f;
+  }
+}
+
+template <typename T, int V, bool RAGGED>
+__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_t xs, T* __restrict__ y, int64_t ys, int64_t n, int d,
+                                                 int units, int rows_per_block, float inv_units, DropArgs dr, uint64_t* step_used) {
   const uint32_t step = drop_step_of(dr);
   if (step_used && blockIdx.x == 0 && threadIdx.x == 0) *step_used = step;
   for (int64_t r0 = (int64_t)blockIdx.x * rows_per_block; r0 < n; r0 += (int64_t)gridDim.x * rows_per_block) {
-    const int64_t rows = n - r0 < rows_per_block ? n - r0 : rows_per_block;
-    const int64_t total = rows * nq;
-    for (int64_t i = threadIdx.x; i < total; i += 256) {
-      // (several rows per block only while rows * nq <= 2048: the quotient in floating point is then exact)
-      const int64_t lr = rows_per_block > 1 ? (int64_t)(((float)(int32_t)i + 0.5f) * inv_nq) : 0;
-      const int64_t q = i - lr * nq, r = r0 + lr, c0 = pair_col(q), c1 = c0 + 256;
-      float a[4], b[4];
-      load4_tail(x + r * xs + c0, d - c0, a);
-      if (c1 < d) load4_tail(x + r * xs + c1, d - c1, b);
-      uint32_t o[4];
-      Philox::gen((uint32_t)r, (uint32_t)q, dr.tag, step, dr.k0, dr.k1, o);
-      drop4(a, o[0], o[1], dr.thr, dr.scale);
-      store4_tail(y + r * ys + c0, d - c0, a);
-      if (c1 < d) {
-        drop4(b, o[2], o[3], dr.thr, dr.scale);
-        store4_tail(y + r * ys + c1, d - c1, b);
-      }
+    const int rows = n - r0 < rows_per_block ? (int)(n - r0) : rows_per_block;
+    const int total = rows * units;
+    for (int i = threadIdx.x; i < total; i += 256) {
+      // (several rows per block only while rows * units <= 1024: the quotient in floating point is then exact)
+      const int lr = rows_per_block > 1 ? (int)(((float)i + 0.5f) * inv_units) : 0;
+      const int u = i - lr * units, c0 = unit_col<V>(u), c1 = c0 + 256;
+      const int64_t r = r0 + lr;
+      const T* src = x + r * xs;
+      T* dst = y + r * ys;
+      float a[4 * V], b[4 * V];
+      load_piece<T, V, RAGGED>(src, c0, d, a);
+      load_piece<T, V, RAGGED>(src, c1, d, b);
+      UnitMask m[V];
+      draw_unit<V>(dr, step, (uint32_t)r, u, m);
+      drop_piece<V>(a, m, 0, dr.thr, dr.scale);
+      drop_piece<V>(b, m, 1, dr.thr, dr.scale);
+      store_piece<T, V, RAGGED>(dst, c0, d, a);
+      store_piece<T, V, RAGGED>(dst, c1, d, b);
     }
   }
 }
@@ -63,299 +109,347 @@ struct NormArgs {
   void *sum, *y, *dx, *dres;
   float *mean, *rstd, *part;
   uint64_t* step_used;
-  int64_t n, d, xs, rs, ss, ys, gys, gss, dxs, drs;
+  int64_t n, xs, rs, ss, ys, gys, gss, dxs, drs;
+  int d;
   float eps;
   int32_t w_f32, drop;
   DropArgs dr;
 };
 
-// sum over the G lanes of a row's group; above one wave through LDS (two slots in turn: a call may start while slow waves
-// still read the previous one's)
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* lds, int& turn) {
+// sums over the G lanes of a row's group, K at a time; above one wave through LDS (two slots in turn: a call may start while slow
+// waves still read the previous one's). Every lane of the workgroup calls it.
+template <int G, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& turn) {
 #pragma unroll
-  for (int o = (G < kWave ? G : kWave) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  for (int o = (G < kWave ? G : kWave) / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, kWave);
   if constexpr (G > kWave) {
-    constexpr int W = G / kWave;
-    float* s = lds + turn * W;
+    constexpr int W = G / kWave, ALL = (G > 256 ? G : 256) / kWave;
+    float* s = lds + turn * 2 * ALL;
     turn ^= 1;
-    if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x / kWave] = v;
-    __syncthreads();
-    v = 0.f;
+    const int wave = threadIdx.x / kWave;
+    if ((threadIdx.x & (kWave - 1)) == 0)
 #pragma unroll
-    for (int i = 0; i < W; ++i) v += s[i];
+      for (int k = 0; k < K; ++k) s[k * ALL + wave] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[k] += s[k * ALL + wave / W * W + i];
+    }
   }
-  return v;
 }
 
-template <typename T>
-__device__ __forceinline__ void load_param(const void* p, int f32, int64_t c, int64_t d, float fill, float (&v)[4]) {
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void load_param(const void* p, int f32, int c, int d, float fill, float (&v)[4 * V]) {
   if (p == nullptr) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fill;
+    for (int i = 0; i < 4 * V; ++i) v[i] = fill;
   } else if (f32) {
-    load4_tail((const float*)p + c, d - c, v);
+    load_piece<float, V, RAGGED>((const float*)p, c, d, v);
   } else {
-    load4_tail((const T*)p + c, d - c, v);
+    load_piece<T, V, RAGGED>((const T*)p, c, d, v);
   }
 }
 
-// G lanes per row, S pairs of pieces per lane: rows of up to 8 * G * S columns (4 * G * S below 256 columns)
-template <typename T, int G, int S>
+// G lanes per row, S units per lane: rows of up to 8 V G S columns (half of it below 256 columns)
+template <typename T, int V, bool RAGGED, int G, int S>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_fwd(NormArgs a) {
-  constexpr int B = G > 256 ? G : 256, RPB = B / G;
-  __shared__ float lds[G > kWave ? 2 * (G / kWave) : 1];
+  constexpr int B = G > 256 ? G : 256, RPB = B / G, P = 4 * V;
+  __shared__ float lds[G > kWave ? 4 * (B / kWave) : 1];
   int turn = 0;
-  const int lane = threadIdx.x % G;
-  const float cols = (float)a.d;
+  const int lane = threadIdx.x % G, d = a.d;
+  const float cols = (float)d;
   const uint32_t step = a.drop ? drop_step_of(a.dr) : 0u;
   if (a.drop && a.step_used && blockIdx.x == 0 && threadIdx.x == 0) *a.step_used = step;
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / G; r < a.n; r += (int64_t)gridDim.x * RPB) {
+  for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.n; rb += (int64_t)gridDim.x * RPB) {
+    const bool on = rb + threadIdx.x / G < a.n;
+    const int64_t r = on ? rb + threadIdx.x / G : a.n - 1;
     const T* x = (const T*)a.x + r * a.xs;
-    float v[2 * S][4];
-    float sum = 0.f;
+    float v[2 * S][P];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      const int64_t q = lane + (int64_t)s * G, c0 = pair_col(q);
+    for (int s = 0; s < S; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t c = c0 + 256 * h;
-        load4_tail(x + c, a.d - c, v[2 * s + h]);
-      }
-      if (a.drop && c0 < a.d) {
-        uint32_t o[4];
-        Philox::gen((uint32_t)r, (uint32_t)q, a.dr.tag, step, a.dr.k0, a.dr.k1, o);
-        drop4(v[2 * s], o[0], o[1], a.dr.thr, a.dr.scale);
-        drop4(v[2 * s + 1], o[2], o[3], a.dr.thr, a.dr.scale);
-      }
-      if (a.res) {
+      for (int h = 0; h < 2; ++h) load_piece<T, V, RAGGED>(x, unit_col<V>(lane + s * G) + 256 * h, d, v[2 * s + h]);
+    if (a.res) {
+      const T* res = (const T*)a.res + r * a.rs;
+      float t[2 * S][P];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int64_t c = c0 + 256 * h;
-          float t[4];
-          load4_tail((const T*)a.res + r * a.rs + c, a.d - c, t);
-          // the sum is handed on in T: what is normalised is that rounded row, which the backward pass reads back
+      for (int s = 0; s < S; ++s)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[2 * s + h][i] = (float)(T)(v[2 * s + h][i] + t[i]);
-          if (c < a.d) store4_tail((T*)a.sum + r * a.ss + c, a.d - c, v[2 * s + h]);
+        for (int h = 0; h < 2; ++h) load_piece<T, V, RAGGED>(res, unit_col<V>(lane + s * G) + 256 * h, d, t[2 * s + h]);
+      if (a.drop) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          UnitMask m[V];
+          draw_unit<V>(a.dr, step, (uint32_t)r, lane + s * G, m);
+          drop_piece<V>(v[2 * s], m, 0, a.dr.thr, a.dr.scale);
+          drop_piece<V>(v[2 * s + 1], m, 1, a.dr.thr, a.dr.scale);
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int k = 0; k < 2 * S; ++k) {
+        // the sum is handed on in T: what is normalised is that rounded row, which the backward pass reads back
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += v[2 * s + h][i];
+        for (int i = 0; i < P; ++i) v[k][i] = (float)(T)(v[k][i] + t[k][i]);
+        if (on) store_piece<T, V, RAGGED>((T*)a.sum + r * a.ss, unit_col<V>(lane + k / 2 * G) + 256 * (k & 1), d, v[k]);
+      }
     }
-    const float mean = group_sum<G>(sum, lds, turn) / cols;
-    float var = 0.f;
+    float mean[1] = {0.f}, var[1] = {0.f};
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int k = 0; k < 2 * S; ++k)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t c = pair_col(lane + (int64_t)s * G) + 256 * h;
+      for (int i = 0; i < P; ++i) mean[0] += v[k][i];
+    group_sum<G, 1>(mean, lds, turn);
+    mean[0] /= cols;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float t = v[2 * s + h][i] - mean;
-          var += c + i < a.d ? t * t : 0.f;
-        }
+    for (int k = 0; k < 2 * S; ++k) {
+      const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        v[k][i] -= mean[0];
+        if (RAGGED ? c + i < d : c < d) var[0] += v[k][i] * v[k][i];
       }
-    var = group_sum<G>(var, lds, turn) / cols;
-    const float rstd = 1.f / sqrtf(var + a.eps);
+    }
+    group_sum<G, 1>(var, lds, turn);
+    const float rstd = 1.f / sqrtf(var[0] / cols + a.eps);
+    if (!on) continue;
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int k = 0; k < 2 * S; ++k) {
+      const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
+      if (c >= d) continue;
+      float w[P], b[P];
+      load_param<T, V, RAGGED>(a.w, a.w_f32, c, d, 1.f, w);
+      load_param<T, V, RAGGED>(a.b, a.w_f32, c, d, 0.f, b);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t c = pair_col(lane + (int64_t)s * G) + 256 * h;
-        if (c < a.d) {
-          float w[4], b[4], y[4];
-          load_param<T>(a.w, a.w_f32, c, a.d, 1.f, w);
-          load_param<T>(a.b, a.w_f32, c, a.d, 0.f, b);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = (v[2 * s + h][i] - mean) * rstd * w[i] + b[i];
-          store4_tail((T*)a.y + r * a.ys + c, a.d - c, y);
-        }
-      }
+      for (int i = 0; i < P; ++i) v[k][i] = v[k][i] * rstd * w[i] + b[i];
+      store_piece<T, V, RAGGED>((T*)a.y + r * a.ys, c, d, v[k]);
+    }
     if (a.mean && lane == 0) {
-      a.mean[r] = mean;
+      a.mean[r] = mean[0];
       a.rstd[r] = rstd;
     }
   }
 }
 
-template <typename T, int G, int S>
+template <typename T, int V, bool RAGGED, int G, int S>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_bwd(NormArgs a) {
-  constexpr int B = G > 256 ? G : 256, RPB = B / G;
-  constexpr int COLS = G <= kWave ? 8 * G * S : 1;               // the workgroup's sum of dw, db (one row group per wave or less)
-  __shared__ float lds[G > kWave ? 2 * (G / kWave) : 1];
+  constexpr int B = G > 256 ? G : 256, RPB = B / G, P = 4 * V;
+  constexpr int COLS = RPB > 1 ? 2 * P * G * S : 1;             // the workgroup's sums of dw, db over its row groups
+  __shared__ float lds[G > kWave ? 4 * (B / kWave) : 1];
   __shared__ float acc_lds[2 * COLS];
   int turn = 0;
-  const int lane = threadIdx.x % G;
-  const float cols = (float)a.d;
+  const int lane = threadIdx.x % G, d = a.d;
+  const float cols = (float)d;
   const uint32_t step = a.drop ? drop_step_of(a.dr) : 0u;
-  float aw[2 * S][4] = {}, ab[2 * S][4] = {};
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / G; r < a.n; r += (int64_t)gridDim.x * RPB) {
+  float aw[2 * S][P] = {}, ab[2 * S][P] = {};
+  for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.n; rb += (int64_t)gridDim.x * RPB) {
+    const bool on = rb + threadIdx.x / G < a.n;
+    const int64_t r = on ? rb + threadIdx.x / G : a.n - 1;
     const float mean = a.mean[r], rstd = a.rstd[r];
-    float xh[2 * S][4], gh[2 * S][4];
-    float s1 = 0.f, s2 = 0.f;
+    float xh[2 * S][P], gh[2 * S][P], ds[2 * S][P], sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+    for (int k = 0; k < 2 * S; ++k) {
+      const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
+      load_piece<T, V, RAGGED>((const T*)a.x + r * a.xs, c, d, xh[k]);
+      load_piece<T, V, RAGGED>((const T*)a.gy + r * a.gys, c, d, gh[k]);
+      if (a.gs) load_piece<T, V, RAGGED>((const T*)a.gs + r * a.gss, c, d, ds[k]);
+    }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = 2 * s + h;
-        const int64_t c = pair_col(lane + (int64_t)s * G) + 256 * h;
-        load4_tail((const T*)a.x + r * a.xs + c, a.d - c, xh[k]);
-        load4_tail((const T*)a.gy + r * a.gys + c, a.d - c, gh[k]);
-      }
+    for (int k = 0; k < 2 * S; ++k) {
+      const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
+      float w[P];
+      load_param<T, V, RAGGED>(a.w, a.w_f32, c, d, 1.f, w);
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = 2 * s + h;
-        const int64_t c = pair_col(lane + (int64_t)s * G) + 256 * h;
-        float w[4];
-        load_param<T>(a.w, a.w_f32, c, a.d, 1.f, w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // (columns behind the row's end have gy = 0: they add nothing to any sum)
-          xh[k][i] = (xh[k][i] - mean) * rstd;
+      for (int i = 0; i < P; ++i) {
+        // columns behind the row's end have gy = 0 and must not meet an infinite xh there
+        xh[k][i] = (RAGGED ? c + i < d : c < d) ? (xh[k][i] - mean) * rstd : 0.f;
+        if (on) {
           ab[k][i] += gh[k][i];
-          aw[k][i] += c + i < a.d ? gh[k][i] * xh[k][i] : 0.f;
-          gh[k][i] *= w[i];
-          s1 += gh[k][i];
-          s2 += c + i < a.d ? gh[k][i] * xh[k][i] : 0.f;
+          aw[k][i] += gh[k][i] * xh[k][i];
         }
+        gh[k][i] *= w[i];
+        sum[0] += gh[k][i];
+        sum[1] += gh[k][i] * xh[k][i];
       }
-    s1 = group_sum<G>(s1, lds, turn) / cols;
-    s2 = group_sum<G>(s2, lds, turn) / cols;
+    }
+    group_sum<G, 2>(sum, lds, turn);
+    if (!on) continue;
+    const float s1 = sum[0] / cols, s2 = sum[1] / cols;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int64_t q = lane + (int64_t)s * G, c0 = pair_col(q);
-      uint32_t o[4];
-      if (a.drop && c0 < a.d) Philox::gen((uint32_t)r, (uint32_t)q, a.dr.tag, step, a.dr.k0, a.dr.k1, o);
+      UnitMask m[V];
+      if (a.drop) draw_unit<V>(a.dr, step, (uint32_t)r, lane + s * G, m);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = 2 * s + h;
-        const int64_t c = c0 + 256 * h;
-        if (c >= a.d) continue;
-        float ds[4];
-        if (a.gs)
-          load4_tail((const T*)a.gs + r * a.gss + c, a.d - c, ds);
-        else
-          ds[0] = ds[1] = ds[2] = ds[3] = 0.f;
+        const int k = 2 * s + h, c = unit_col<V>(lane + s * G) + 256 * h;
+        if (c >= d) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ds[i] += rstd * (gh[k][i] - s1 - xh[k][i] * s2);
-        if (a.dres) store4_tail((T*)a.dres + r * a.drs + c, a.d - c, ds);
+        for (int i = 0; i < P; ++i) ds[k][i] = rstd * (gh[k][i] - s1 - xh[k][i] * s2) + (a.gs ? ds[k][i] : 0.f);
+        if (a.dres) store_piece<T, V, RAGGED>((T*)a.dres + r * a.drs, c, d, ds[k]);
         if (a.dx) {
-          if (a.drop) drop4(ds, o[2 * h], o[2 * h + 1], a.dr.thr, a.dr.scale);
-          store4_tail((T*)a.dx + r * a.dxs + c, a.d - c, ds);
+          if (a.drop) drop_piece<V>(ds[k], m, h, a.dr.thr, a.dr.scale);
+          store_piece<T, V, RAGGED>((T*)a.dx + r * a.dxs, c, d, ds[k]);
         }
       }
     }
   }
   if (!a.part) return;
-  float* out = a.part + (int64_t)blockIdx.x * 2 * a.d;
-  if constexpr (G <= kWave) {
-    // the wave's groups first (lanes G apart hold the same columns), then the four waves one after the other
+  float* out = a.part + (int64_t)blockIdx.x * 2 * d;
+  if constexpr (RPB > 1) {
+    // lanes G apart in a wave hold the same columns: those first, then the waves (pairs of waves) one after the other
+    if constexpr (G < kWave) {
 #pragma unroll
-    for (int k = 0; k < 2 * S; ++k)
+      for (int k = 0; k < 2 * S; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int o = kWave / 2; o >= G; o >>= 1) {
-          aw[k][i] += __shfl_xor(aw[k][i], o, kWave);
-          ab[k][i] += __shfl_xor(ab[k][i], o, kWave);
-        }
-    for (int w = 0; w < B / kWave; ++w) {
-      if ((int)threadIdx.x / kWave == w && (threadIdx.x & (kWave - 1)) < G)
+          for (int o = kWave / 2; o >= G; o >>= 1) {
+            aw[k][i] += __shfl_xor(aw[k][i], o, kWave);
+            ab[k][i] += __shfl_xor(ab[k][i], o, kWave);
+          }
+    }
+    constexpr int L = G < kWave ? kWave : G;                    // lanes that hold one group of sums
+    for (int g = 0; g < B / L; ++g) {
+      if ((int)threadIdx.x / L == g && threadIdx.x % L < G)
 #pragma unroll
         for (int k = 0; k < 2 * S; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = (k * G + lane) * 4 + i;
-            acc_lds[at] = (w ? acc_lds[at] : 0.f) + aw[k][i];
-            acc_lds[COLS + at] = (w ? acc_lds[COLS + at] : 0.f) + ab[k][i];
+          for (int i = 0; i < P; ++i) {
+            const int at = (k * P + i) * G + lane;
+            acc_lds[at] = (g ? acc_lds[at] : 0.f) + aw[k][i];
+            acc_lds[COLS + at] = (g ? acc_lds[COLS + at] : 0.f) + ab[k][i];
           }
       __syncthreads();
     }
     for (int at = threadIdx.x; at < COLS; at += B) {
-      const int k = at / (4 * G), l = at / 4 % G;
-      const int64_t c = pair_col(l + (int64_t)(k / 2) * G) + 256 * (k & 1) + (at & 3);
-      if (c < a.d) {
+      const int k = at / G / P, i = at / G % P, l = at % G;
+      const int c = unit_col<V>(l + k / 2 * G) + 256 * (k & 1) + i;
+      if (c < d) {
         out[c] = acc_lds[at];
-        out[a.d + c] = acc_lds[COLS + at];
+        out[d + c] = acc_lds[COLS + at];
       }
     }
   } else {
 #pragma unroll
     for (int k = 0; k < 2 * S; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t c = pair_col(lane + (int64_t)(k / 2) * G) + 256 * (k & 1) + i;
-        if (c < a.d) {
+      for (int i = 0; i < P; ++i) {
+        const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1) + i;
+        if (c < d) {
           out[c] = aw[k][i];
-          out[a.d + c] = ab[k][i];
+          out[d + c] = ab[k][i];
         }
       }
   }
 }
 
-// dw, db = the workgroups' partial rows added up in a fixed order: 16 columns x 16 lanes over the rows per block
+// dw, db = the workgroups' partial rows added up in a fixed order: 16 columns per block, 64 lanes of four columns over the rows
 template <typename TW>
-__global__ __launch_bounds__(256) void k_norm_reduce(const float* __restrict__ part, int32_t rows, int64_t d, TW* __restrict__ dw,
+__global__ __launch_bounds__(256) void k_norm_reduce(const float* __restrict__ part, int32_t rows, int d, TW* __restrict__ dw,
                                                      TW* __restrict__ db) {
-  __shared__ float s[16][17];
-  const int64_t c = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-  const int l = threadIdx.x >> 4;
+  __shared__ float s[64][17];
   TW* out = blockIdx.y ? db : dw;
   if (!out) return;
+  const int c0 = blockIdx.x * 16, c = c0 + threadIdx.x % 4 * 4, l = threadIdx.x / 4;
   const float* p = part + (int64_t)blockIdx.y * d + c;
-  float acc = 0.f;
-  if (c < d) {
-#pragma unroll 8
-    for (int r = l; r < rows; r += 16) acc += p[(int64_t)r * 2 * d];
-  }
-  s[l][threadIdx.x & 15] = acc;
-  __syncthreads();
-  if (l == 0 && c < d) {
-    float t = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r = l; r < rows; r += 64) {
+    float v[4];
+    load4_tail(p + (int64_t)r * 2 * d, d - c, v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += s[i][threadIdx.x & 15];
-    out[c] = (TW)t;
+    for (int i = 0; i < 4; ++i) acc[i] += v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[l][threadIdx.x % 4 * 4 + i] = acc[i];
+  __syncthreads();
+  const int col = threadIdx.x % 16, g = threadIdx.x / 16;
+  float t = s[4 * g][col] + s[4 * g + 1][col] + s[4 * g + 2][col] + s[4 * g + 3][col];
+  __syncthreads();
+  s[g][col] = t;
+  __syncthreads();
+  if (g == 0 && c0 + col < d) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += s[i][col];
+    out[c0 + col] = (TW)t;
   }
 }
 
-// workgroups of the backward pass: enough to fill the card twice over; each leaves one partial row of 2 d floats
-inline int64_t norm_bwd_blocks(int64_t n, int64_t d) {
-  const int64_t nq = row_pairs(d);
-  const int64_t rpb = nq <= 16 ? 16 : nq <= 32 ? 8 : nq <= 256 ? 4 : 1;
-  const int64_t b = ceil_div<int64_t>(n, rpb);
-  return b < 1 ? 1 : b > 512 ? 512 : b;
+// 16-bit rows of whole 16-byte pieces move 16 bytes a lane
+inline int norm_v(int64_t d, int32_t dtype) { return dtype != PG_DTYPE_F32 && d % 8 == 0 ? 2 : 1; }
+
+// lanes per row: some 16 elements of a row per lane (more lanes idle on narrower rows, more registers on wider ones)
+inline int norm_lanes(int64_t d, int v) {
+  const int u = (row_pairs(d) + v - 1) / v;
+  if (u <= 64) return u <= 16 ? 16 : u <= 32 ? 32 : 64;
+  const int per = v == 2 ? 1 : 2;                                // units per lane above 64 units
+  const int g = (u + per - 1) / per;
+  return g <= 64 ? 64 : g <= 128 ? 128 : g <= 256 ? 256 : g <= 512 ? 512 : 1024;
 }
 
-template <typename T, int G, int S>
-int launch_norm(const NormArgs& a, bool bwd, hipStream_t st) {
+// workgroups of the backward pass: each leaves one partial row of 2 d floats, so each walks 8 rows at least, which keeps that
+// traffic to a tenth of the rows' own. At most the three a CU holds at once (registers): a second, partly filled round of them
+// took as long as the first (1024 workgroups 117 us, 768 89 us at 16384 x 2048 bf16 with dropout and residual)
+inline int64_t norm_bwd_blocks(int64_t n, int64_t d, int32_t dtype) {
+  const int g = norm_lanes(d, norm_v(d, dtype)), rpb = g >= 256 ? 1 : 256 / g;
+  const int64_t rows = rpb > 8 ? rpb : 8, b = ceil_div<int64_t>(n, rows);
+  return b < 1 ? 1 : b > 768 ? 768 : b;
+}
+
+template <typename T, int V, bool RAGGED, int G, int S>
+int launch_norm(const NormArgs& a, int64_t bwd_blocks, hipStream_t st) {
   constexpr int B = G > 256 ? G : 256;
-  if (bwd) {
-    hipLaunchKernelGGL((k_norm_bwd<T, G, S>), dim3((unsigned)norm_bwd_blocks(a.n, a.d)), dim3(B), 0, st, a);
+  if (bwd_blocks) {
+    hipLaunchKernelGGL((k_norm_bwd<T, V, RAGGED, G, S>), dim3((unsigned)bwd_blocks), dim3(B), 0, st, a);
   } else {
     const int64_t b = ceil_div<int64_t>(a.n, B / G);
-    hipLaunchKernelGGL((k_norm_fwd<T, G, S>), dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(B), 0, st, a);
+    hipLaunchKernelGGL((k_norm_fwd<T, V, RAGGED, G, S>), dim3((unsigned)(b > 8192 ? 8192 : b)), dim3(B), 0, st, a);
   }
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
 
-// lanes per row and pairs per lane by the row's width: a row stays in registers, with as few idle lanes as a power of two allows
+template <typename T, int V, bool RAGGED>
+int dispatch_norm_v(const NormArgs& a, int64_t bwd, hipStream_t st) {
+  const int u = (row_pairs(a.d) + V - 1) / V, g = norm_lanes(a.d, V);
+  constexpr int S = V == 2 ? 1 : 2;
+  if (g == 16) return launch_norm<T, V, RAGGED, 16, 1>(a, bwd, st);
+  if (g == 32) return launch_norm<T, V, RAGGED, 32, 1>(a, bwd, st);
+  if (u <= 64) return launch_norm<T, V, RAGGED, 64, 1>(a, bwd, st);
+  if (g == 64) return launch_norm<T, V, RAGGED, 64, S>(a, bwd, st);
+  if (g == 128) return launch_norm<T, V, RAGGED, 128, S>(a, bwd, st);
+  if (g == 256) return launch_norm<T, V, RAGGED, 256, S>(a, bwd, st);
+  if (g == 512) return launch_norm<T, V, RAGGED, 512, S>(a, bwd, st);
+  if (u <= 1024 * S) return launch_norm<T, V, RAGGED, 1024, S>(a, bwd, st);
+  return launch_norm<T, V, RAGGED, 1024, 2 * S>(a, bwd, st);
+}
+
 template <typename T>
-int dispatch_norm(const NormArgs& a, bool bwd, hipStream_t st) {
-  const int64_t nq = row_pairs(a.d);
-  if (nq <= 16) return launch_norm<T, 16, 1>(a, bwd, st);
-  if (nq <= 32) return launch_norm<T, 32, 1>(a, bwd, st);
-  if (nq <= 64) return launch_norm<T, 64, 1>(a, bwd, st);
-  if (nq <= 128) return launch_norm<T, 64, 2>(a, bwd, st);
-  if (nq <= 256) return launch_norm<T, 64, 4>(a, bwd, st);
-  if (nq <= 512) return launch_norm<T, 256, 2>(a, bwd, st);
-  if (nq <= 1024) return launch_norm<T, 256, 4>(a, bwd, st);
-  return launch_norm<T, 1024, 4>(a, bwd, st);
+int dispatch_norm(const NormArgs& a, int64_t bwd, hipStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.d % 8 == 0) return dispatch_norm_v<T, 2, false>(a, bwd, st);
+  } else {
+    if (a.d % 4 == 0) return dispatch_norm_v<T, 1, false>(a, bwd, st);
+  }
+  return dispatch_norm_v<T, 1, true>(a, bwd, st);
+}
+
+template <typename T>
+void launch_dropout(const void* x, int64_t xs, void* y, int64_t ys, int64_t n, int64_t d, const DropArgs& dr, uint64_t* used, hipStream_t st) {
+  const int v = sizeof(T) == 2 && d % 8 == 0 ? 2 : 1, units = (row_pairs(d) + v - 1) / v, rows = units >= 512 ? 1 : 1024 / units;
+  const int64_t blocks = ceil_div<int64_t>(n, rows);
+  const dim3 grid((unsigned)(blocks > 65536 ? 65536 : blocks));
+  const float inv = 1.f / (float)units;
+  if (v == 2)
+    hipLaunchKernelGGL((k_dropout<T, 2, false>), grid, dim3(256), 0, st, (const T*)x, xs, (T*)y, ys, n, (int)d, units, rows, inv, dr, used);
+  else if (d % 4 == 0)
+    hipLaunchKernelGGL((k_dropout<T, 1, false>), grid, dim3(256), 0, st, (const T*)x, xs, (T*)y, ys, n, (int)d, units, rows, inv, dr, used);
+  else
+    hipLaunchKernelGGL((k_dropout<T, 1, true>), grid, dim3(256), 0, st, (const T*)x, xs, (T*)y, ys, n, (int)d, units, rows, inv, dr, used);
 }
 
 int norm_args(const pg_norm_desc_t* p, NormArgs* a) {
@@ -365,7 +459,7 @@ int norm_args(const pg_norm_desc_t* p, NormArgs* a) {
   if (p->n > (int64_t)0xffffffffll) return PG_ERR_UNSUPPORTED;          // the mask's row counter has 32 bits
   *a = NormArgs{};
   a->n = p->n;
-  a->d = p->d;
+  a->d = (int)p->d;
   a->w = p->weight;
   a->b = p->bias;
   a->w_f32 = p->param_dtype == PG_DTYPE_F32;
@@ -387,22 +481,14 @@ extern "C" {
 int pg_dropout_apply(const void* x, int64_t x_stride, void* y, int64_t y_stride, int64_t n, int64_t d, int32_t dtype,
                      const pg_dropout_t* drop, uint64_t* step_used, pg_stream_t stream) {
   if (n < 0 || d <= 0 || dtype < PG_DTYPE_F32 || dtype > PG_DTYPE_F16 || y_stride < d || bad_stride(x, x_stride, d)) return PG_ERR_INVALID;
-  if (n > (int64_t)0xffffffffll || d > (int64_t)0x7fffffffll) return PG_ERR_UNSUPPORTED;      // the mask's counters have 32 bits
+  if (n > (int64_t)0xffffffffll || d > (int64_t)0x7ffffc00ll) return PG_ERR_UNSUPPORTED;      // the mask's counters have 32 bits
   DropArgs dr;
   if (!drop || !drop_args(drop, &dr)) return PG_ERR_INVALID;
   if (n == 0) return PG_OK;
   if (!x || !y) return PG_ERR_INVALID;
-  const int64_t nq = row_pairs(d);
-  const int32_t rows = nq >= 1024 ? 1 : (int32_t)(1024 / nq);
-  const int64_t blocks = ceil_div<int64_t>(n, rows);
-  const dim3 grid((unsigned)(blocks > 16384 ? 16384 : blocks));
-  const float inv = 1.f / (float)nq;
-  if (dtype == PG_DTYPE_F32)
-    hipLaunchKernelGGL(k_dropout<float>, grid, dim3(256), 0, as_stream(stream), (const float*)x, x_stride, (float*)y, y_stride, n, d, nq, rows, inv, dr, step_used);
-  else if (dtype == PG_DTYPE_BF16)
-    hipLaunchKernelGGL(k_dropout<bf16_t>, grid, dim3(256), 0, as_stream(stream), (const bf16_t*)x, x_stride, (bf16_t*)y, y_stride, n, d, nq, rows, inv, dr, step_used);
-  else
-    hipLaunchKernelGGL(k_dropout<f16_t>, grid, dim3(256), 0, as_stream(stream), (const f16_t*)x, x_stride, (f16_t*)y, y_stride, n, d, nq, rows, inv, dr, step_used);
+  if (dtype == PG_DTYPE_F32) launch_dropout<float>(x, x_stride, y, y_stride, n, d, dr, step_used, as_stream(stream));
+  else if (dtype == PG_DTYPE_BF16) launch_dropout<bf16_t>(x, x_stride, y, y_stride, n, d, dr, step_used, as_stream(stream));
+  else launch_dropout<f16_t>(x, x_stride, y, y_stride, n, d, dr, step_used, as_stream(stream));
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
@@ -422,14 +508,14 @@ int pg_layer_norm_fwd(const pg_norm_desc_t* p, pg_stream_t stream) {
   a.sum = p->sum; a.ss = p->sum_stride;
   a.y = p->y; a.ys = p->y_stride;
   a.step_used = p->step_used;
-  if (p->dtype == PG_DTYPE_F32) return dispatch_norm<float>(a, false, as_stream(stream));
-  if (p->dtype == PG_DTYPE_BF16) return dispatch_norm<bf16_t>(a, false, as_stream(stream));
-  return dispatch_norm<f16_t>(a, false, as_stream(stream));
+  if (p->dtype == PG_DTYPE_F32) return dispatch_norm<float>(a, 0, as_stream(stream));
+  if (p->dtype == PG_DTYPE_BF16) return dispatch_norm<bf16_t>(a, 0, as_stream(stream));
+  return dispatch_norm<f16_t>(a, 0, as_stream(stream));
 }
 
-int64_t pg_layer_norm_scratch(int64_t n, int64_t d) {
+int64_t pg_layer_norm_scratch(int64_t n, int64_t d, int32_t dtype) {
   if (n < 0 || d <= 0 || d > PG_NORM_MAX_COLUMNS) return 0;
-  return norm_bwd_blocks(n, d) * 2 * d;
+  return norm_bwd_blocks(n, d, dtype) * 2 * d;
 }
 
 int pg_layer_norm_bwd(const pg_norm_desc_t* p, pg_stream_t stream) {
@@ -448,20 +534,21 @@ int pg_layer_norm_bwd(const pg_norm_desc_t* p, pg_stream_t stream) {
   a.dres = p->dres; a.drs = p->dres_stride;
   a.part = params ? p->partials : nullptr;
   int r = PG_OK;
+  const int64_t blocks = norm_bwd_blocks(p->n, p->d, p->dtype);
   if (p->n > 0) {
-    if (p->dtype == PG_DTYPE_F32) r = dispatch_norm<float>(a, true, as_stream(stream));
-    else if (p->dtype == PG_DTYPE_BF16) r = dispatch_norm<bf16_t>(a, true, as_stream(stream));
-    else r = dispatch_norm<f16_t>(a, true, as_stream(stream));
+    if (p->dtype == PG_DTYPE_F32) r = dispatch_norm<float>(a, blocks, as_stream(stream));
+    else if (p->dtype == PG_DTYPE_BF16) r = dispatch_norm<bf16_t>(a, blocks, as_stream(stream));
+    else r = dispatch_norm<f16_t>(a, blocks, as_stream(stream));
   }
   if (r != PG_OK || !params) return r;
-  const int32_t rows = p->n > 0 ? (int32_t)norm_bwd_blocks(p->n, p->d) : 0;     // no rows: the sums are zeros
+  const int32_t rows = p->n > 0 ? (int32_t)blocks : 0;     // no rows: the sums are zeros
   const dim3 grid((unsigned)ceil_div<int64_t>(p->d, 16), 2);
   if (p->param_dtype == PG_DTYPE_F32)
-    hipLaunchKernelGGL(k_norm_reduce<float>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, p->d, (float*)p->dw, (float*)p->db);
+    hipLaunchKernelGGL(k_norm_reduce<float>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, (int)p->d, (float*)p->dw, (float*)p->db);
   else if (p->param_dtype == PG_DTYPE_BF16)
-    hipLaunchKernelGGL(k_norm_reduce<bf16_t>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, p->d, (bf16_t*)p->dw, (bf16_t*)p->db);
+    hipLaunchKernelGGL(k_norm_reduce<bf16_t>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, (int)p->d, (bf16_t*)p->dw, (bf16_t*)p->db);
   else
-    hipLaunchKernelGGL(k_norm_reduce<f16_t>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, p->d, (f16_t*)p->dw, (f16_t*)p->db);
+    hipLaunchKernelGGL(k_norm_reduce<f16_t>, grid, dim3(256), 0, as_stream(stream), p->partials, rows, (int)p->d, (f16_t*)p->dw, (f16_t*)p->db);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }

@@ -1012,7 +1012,7 @@ class _LayerNorm(torch.autograd.Function):
         db = torch.empty(d, dtype=bias.dtype, device=dev) if need_b else None
         part = None
         if need_w or need_b:
-            part = torch.empty(L.load().pg_layer_norm_scratch(n, d), dtype=torch.float32, device=dev)
+            part = torch.empty(L.load().pg_layer_norm_scratch(n, d, _DTYPES[t]), dtype=torch.float32, device=dev)
         at = stats.data_ptr()
         _enqueue("pg_layer_norm_bwd", dev, L.PgNormDesc(
             None, None, _addr(weight), _addr(bias), rows.data_ptr(), None, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),

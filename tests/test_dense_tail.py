@@ -84,7 +84,7 @@ def test_library_refuses_bad_arguments(hiplib):
     assert hiplib.pg_layer_norm_fwd(a, None) == -4 and hiplib.pg_layer_norm_bwd(a, None) == -4
     a.d, a.has_drop, a.drop = 8, 1, drop
     assert hiplib.pg_layer_norm_fwd(a, None) == -1                                                         # dropout without a residual
-    assert hiplib.pg_layer_norm_scratch(10, 0) == 0 and hiplib.pg_layer_norm_scratch(10, 8) >= 16
+    assert hiplib.pg_layer_norm_scratch(10, 0, 0) == 0 and hiplib.pg_layer_norm_scratch(10, 8, 0) >= 16
     x = L.PgLinearXentDesc()
     assert hiplib.pg_linear_xent_fwd(None, None) == hiplib.pg_linear_xent_bwd(x, None) == hiplib.pg_linear_xent_fwd(x, None) == -1
     assert hiplib.pg_linear_xent_scratch(-1, 8, 8, 0, 0) == -1 and hiplib.pg_linear_xent_scratch(4, 8, 8, 5, 0) == -1
