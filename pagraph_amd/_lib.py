@@ -228,13 +228,13 @@ _SIGS = {
     "pg_linear_bwd_w": (ctypes.c_int, [ctypes.POINTER(PgLinearBwdDesc), vp]),
     "pg_xent_fwd": (ctypes.c_int, [vp, c_i32, vp, c_i64, c_i32, c_i64, vp, c_i32, vp, vp, vp]),
     "pg_xent_bwd": (ctypes.c_int, [vp, c_i32, c_i64, c_i32, vp, vp, vp, c_i32, vp]),
-    "pg_dropout_apply": (ctypes.c_int, [vp, c_i64, vp, c_i64, c_i64, c_i64, c_i32, ctypes.POINTER(PgDropout), vp, vp]),
-    "pg_layer_norm_fwd": (ctypes.c_int, [ctypes.POINTER(PgNormDesc), vp]),
+    "pg_dropout_apply": (ctypes.c_int, [vp, c_i64, vp, c_i64, c_i64, c_i64, c_i32, vp, vp, vp]),
+    "pg_layer_norm_fwd": (ctypes.c_int, [vp, vp]),
     "pg_layer_norm_scratch": (c_i64, [c_i64, c_i64, c_i32]),
-    "pg_layer_norm_bwd": (ctypes.c_int, [ctypes.POINTER(PgNormDesc), vp]),
+    "pg_layer_norm_bwd": (ctypes.c_int, [vp, vp]),
     "pg_linear_xent_scratch": (c_i64, [c_i64, c_i64, c_i64, c_i32, c_i32]),
-    "pg_linear_xent_fwd": (ctypes.c_int, [ctypes.POINTER(PgLinearXentDesc), vp]),
-    "pg_linear_xent_bwd": (ctypes.c_int, [ctypes.POINTER(PgLinearXentDesc), vp]),
+    "pg_linear_xent_fwd": (ctypes.c_int, [vp, vp]),
+    "pg_linear_xent_bwd": (ctypes.c_int, [vp, vp]),
     "pg_gcn_head_scratch": (c_i64, [c_i64, c_i32, c_i32]),
     "pg_gcn_head_row_len": (c_i32, [c_i32, c_i32]),
     "pg_head": (ctypes.c_int, [ctypes.POINTER(PgHeadDesc), vp]),

@@ -1,6 +1,7 @@
 """autograd wrappers over the HIP aggregation kernels (pagraph_amd/csrc/pg_spmm.hip)."""
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -856,9 +857,11 @@ def gcn_head(indptr, src, h, linear, labels, n_valid, grad_seed=None, ignore_ind
 
 
 # ---- the dense tail of a model: dropout, layer norm with its residual, the loss of a wide class head -------------------------
-# A call costs the host more than most of these kernels cost the card, and a backward pass runs on autograd's own thread: what
-# stands between the arguments and the launch is kept short (descriptors filled positionally, no device switch where none is due:
-# 149 -> 85 us for a forward and backward pass of ops.dropout on small rows, 31 us of them autograd's own).
+# A call costs the host more than most of these kernels cost the card, and a backward pass runs on autograd's own thread, with
+# every Python object it touches in another core's cache: what stands between the arguments and the launch is kept short
+# (descriptors packed in one go — the layout is pg_norm_desc_t's and pg_linear_xent_desc_t's —, no device switch where none is due).
+_NORM_DESC, _XENT_DESC, _DROP_DESC = struct.Struct("16Q10qiifiIIQQQ").pack, struct.Struct("13Q7qii").pack, struct.Struct("IIQQQ").pack
+_NO_DROP = (0, 0, 0, 0, 0)
 _DTYPES = {torch.float32: L.PG_DTYPE_F32, torch.bfloat16: L.PG_DTYPE_BF16, torch.float16: L.PG_DTYPE_F16}
 
 
@@ -876,7 +879,7 @@ def _enqueue(name, device, *args):
 
 
 def _addr(t):
-    return t.data_ptr() if t is not None else None
+    return t.data_ptr() if t is not None else 0
 
 
 def _rows_of(x):
@@ -920,30 +923,32 @@ def _once(name):
         raise L.PgError(f"{name}: a gradient's own graph (create_graph=True) is not supported")
 
 
-def _drop_struct(spec, step_used=None):
-    """the mask's parameters; for a gradient the step is the one the forward's launch noted, not what the counter holds by now"""
-    step = spec.step.data_ptr() if step_used is None and spec.step is not None else step_used
-    return L.PgDropout(spec.threshold, spec.tag, spec.seed, step, spec.step_value)
+def _drop_fields(spec, step_used=0):
+    """pg_dropout_t of a mask; for a gradient the step is the one the forward's launch noted, not what the counter holds by now"""
+    step = spec.step
+    return spec.threshold, spec.tag, spec.seed, 0 if step is None else step_used or step.data_ptr(), spec.step_value & 0xFFFFFFFFFFFFFFFF
 
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, spec):
-        rows = _rows_of(x)
-        y = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
-        used = torch.empty(1, dtype=torch.int64, device=x.device) if spec.step is not None and ctx.needs_input_grad[0] else None
-        _enqueue("pg_dropout_apply", x.device, rows.data_ptr(), _row_stride(rows), y.data_ptr(), rows.size(1), rows.size(0), rows.size(1),
-                 _DTYPES[x.dtype], _drop_struct(spec), _addr(used))
+        rows, dev, t = _rows_of(x), x.device, x.dtype
+        n, d = rows.shape
+        y = torch.empty((n, d), dtype=t, device=dev)
+        used = torch.empty(1, dtype=torch.int64, device=dev) if spec.step is not None and ctx.needs_input_grad[0] else None
+        _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), y.data_ptr(), d, n, d, _DTYPES[t],
+                 _DROP_DESC(*_drop_fields(spec)), _addr(used))
         ctx.spec, ctx.used = spec, used
         return _like(y, x.shape)
 
     @staticmethod
     def backward(ctx, gy):
         _once("dropout")
-        rows = _rows_of(gy)
-        gx = torch.empty(rows.shape, dtype=gy.dtype, device=gy.device)
-        _enqueue("pg_dropout_apply", gy.device, rows.data_ptr(), _row_stride(rows), gx.data_ptr(), rows.size(1), rows.size(0), rows.size(1),
-                 _DTYPES[gy.dtype], _drop_struct(ctx.spec, _addr(ctx.used)), None)
+        rows, dev, t = _rows_of(gy), gy.device, gy.dtype
+        n, d = rows.shape
+        gx = torch.empty((n, d), dtype=t, device=dev)
+        _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), gx.data_ptr(), d, n, d, _DTYPES[t],
+                 _DROP_DESC(*_drop_fields(ctx.spec, _addr(ctx.used))), 0)
         return _like(gx, gy.shape), None
 
 
@@ -973,12 +978,11 @@ class _LayerNorm(torch.autograd.Function):
         stats = torch.empty(2 * n + 2, dtype=torch.float32, device=dev) if grad[0] or grad[1] or grad[2] or grad[3] else None
         at = _addr(stats)
         param = weight if weight is not None else bias
-        _enqueue("pg_layer_norm_fwd", dev, L.PgNormDesc(
-            rows.data_ptr(), _addr(res), _addr(weight), _addr(bias), _addr(total), y.data_ptr(), at, at + 4 * n if at is not None else None,
-            None, None, None, None, None, None, None, at + 8 * n if at is not None else None,
-            n, d, _row_stride(rows), _row_stride(res) if res is not None else 0, d, d, 0, 0, 0, 0,
-            _DTYPES[t], _DTYPES[param.dtype] if param is not None else _DTYPES[t], eps, 1 if spec is not None else 0,
-            _drop_struct(spec) if spec is not None else L.PgDropout()))
+        dt = _DTYPES[t]
+        _enqueue("pg_layer_norm_fwd", dev, _NORM_DESC(
+            rows.data_ptr(), _addr(res), _addr(weight), _addr(bias), _addr(total), y.data_ptr(), at, at + 4 * n if at else 0,
+            0, 0, 0, 0, 0, 0, 0, at + 8 * n if at else 0, n, d, _row_stride(rows), _row_stride(res) if res is not None else 0, d, d, 0, 0, 0, 0,
+            dt, _DTYPES[param.dtype] if param is not None else dt, eps, spec is not None, *(_drop_fields(spec) if spec is not None else _NO_DROP)))
         ctx.eps, ctx.spec = eps, spec
         ctx.set_materialize_grads(False)
         y = _like(y, x.shape)
@@ -1002,7 +1006,7 @@ class _LayerNorm(torch.autograd.Function):
         rows, g = _rows_of(s), _rows_of(gy)
         gs = _rows_of(gsum) if gsum is not None else None
         n, d = rows.shape
-        dev, t = s.device, s.dtype
+        dev, t, dt = s.device, s.dtype, _DTYPES[s.dtype]
         need_w, need_b = need_w and weight is not None, need_b and bias is not None
         dx = torch.empty((n, d), dtype=t, device=dev) if need_x or (need_res and spec is None) else None
         # one gradient for both summands, as of a sum, unless a mask stands before one of them
@@ -1012,14 +1016,13 @@ class _LayerNorm(torch.autograd.Function):
         db = torch.empty(d, dtype=bias.dtype, device=dev) if need_b else None
         part = None
         if need_w or need_b:
-            part = torch.empty(L.load().pg_layer_norm_scratch(n, d, _DTYPES[t]), dtype=torch.float32, device=dev)
+            part = torch.empty(L.load().pg_layer_norm_scratch(n, d, dt), dtype=torch.float32, device=dev)
         at = stats.data_ptr()
-        _enqueue("pg_layer_norm_bwd", dev, L.PgNormDesc(
-            None, None, _addr(weight), _addr(bias), rows.data_ptr(), None, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
-            _addr(dw), _addr(db), _addr(part), None,
-            n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
-            _DTYPES[t], _DTYPES[param.dtype] if param is not None else _DTYPES[t], ctx.eps, 1 if spec is not None else 0,
-            _drop_struct(spec, at + 8 * n if spec.step is not None else None) if spec is not None else L.PgDropout()))
+        _enqueue("pg_layer_norm_bwd", dev, _NORM_DESC(
+            0, 0, _addr(weight), _addr(bias), rows.data_ptr(), 0, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
+            _addr(dw), _addr(db), _addr(part), 0, n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
+            dt, _DTYPES[param.dtype] if param is not None else dt, ctx.eps, spec is not None,
+            *(_drop_fields(spec, at + 8 * n) if spec is not None else _NO_DROP)))
         if need_res:
             dres = _like(dx if spec is None else dres, s.shape)
         return (_like(dx, s.shape) if need_x else None, dw, db, dres, None, None)
@@ -1070,9 +1073,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
             raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)
         at = stats.data_ptr()
-        _enqueue("pg_linear_xent_fwd", dev, L.PgLinearXentDesc(
+        _enqueue("pg_linear_xent_fwd", dev, _XENT_DESC(
             rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
-            None, None, None, None, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
+            0, 0, 0, 0, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
         ctx.save_for_backward(h, weight, bias, labels, stats)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         if reduction == L.PG_XENT_NONE:
@@ -1095,7 +1098,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             g = g.reshape(-1)                        # fp32, as the loss is
             scratch = torch.empty(L.load().pg_linear_xent_scratch(n, K, C, t, 1), dtype=torch.uint8, device=dev)
             at = stats.data_ptr()
-            _enqueue("pg_linear_xent_bwd", dev, L.PgLinearXentDesc(
+            _enqueue("pg_linear_xent_bwd", dev, _XENT_DESC(
                 rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
                 g.data_ptr(), _addr(dh), _addr(dw), _addr(db), scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight),
                 g.stride(0), ctx.ignore_index, t, ctx.reduction))

@@ -71,22 +71,23 @@ def test_refuses_host_tensors(hiplib):
 
 def test_library_refuses_bad_arguments(hiplib):
     from pagraph_amd import _lib as L
+    ref = lambda o: ctypes.addressof(o) if o is not None else None
     drop = L.PgDropout(100, 0, 1, None, 0)
-    call = lambda n=1, d=4, xs=4, ys=4, dt=0, dr=drop: hiplib.pg_dropout_apply(None, xs, None, ys, n, d, dt, dr, None, None)
+    call = lambda n=1, d=4, xs=4, ys=4, dt=0, dr=drop: hiplib.pg_dropout_apply(None, xs, None, ys, n, d, dt, ref(dr), None, None)
     assert call(n=-1) == call(d=0) == call(xs=3) == call(ys=3) == call(dt=3) == call(dr=None) == call() == -1
     assert call(dr=L.PgDropout(0, 0, 1, None, 0)) == -1
     assert call(n=1 << 32) == -4 and call(n=0) == 0
     a = L.PgNormDesc()
-    assert hiplib.pg_layer_norm_fwd(None, None) == -1 and hiplib.pg_layer_norm_fwd(a, None) == -1          # no columns
+    assert hiplib.pg_layer_norm_fwd(None, None) == -1 and hiplib.pg_layer_norm_fwd(ref(a), None) == -1          # no columns
     a.n, a.d, a.x_stride, a.y_stride = 2, 8, 8, 8
-    assert hiplib.pg_layer_norm_fwd(a, None) == -1                                                         # no rows given
+    assert hiplib.pg_layer_norm_fwd(ref(a), None) == -1                                                         # no rows given
     a.d = L.PG_NORM_MAX_COLUMNS + 1
-    assert hiplib.pg_layer_norm_fwd(a, None) == -4 and hiplib.pg_layer_norm_bwd(a, None) == -4
+    assert hiplib.pg_layer_norm_fwd(ref(a), None) == -4 and hiplib.pg_layer_norm_bwd(ref(a), None) == -4
     a.d, a.has_drop, a.drop = 8, 1, drop
-    assert hiplib.pg_layer_norm_fwd(a, None) == -1                                                         # dropout without a residual
+    assert hiplib.pg_layer_norm_fwd(ref(a), None) == -1                                                         # dropout without a residual
     assert hiplib.pg_layer_norm_scratch(10, 0, 0) == 0 and hiplib.pg_layer_norm_scratch(10, 8, 0) >= 16
     x = L.PgLinearXentDesc()
-    assert hiplib.pg_linear_xent_fwd(None, None) == hiplib.pg_linear_xent_bwd(x, None) == hiplib.pg_linear_xent_fwd(x, None) == -1
+    assert hiplib.pg_linear_xent_fwd(None, None) == hiplib.pg_linear_xent_bwd(ref(x), None) == hiplib.pg_linear_xent_fwd(ref(x), None) == -1
     assert hiplib.pg_linear_xent_scratch(-1, 8, 8, 0, 0) == -1 and hiplib.pg_linear_xent_scratch(4, 8, 8, 5, 0) == -1
     assert hiplib.pg_linear_xent_scratch(1 << 31, 8, 1 << 20, 0, 1) == -1                                  # more tiles than a grid has
     assert hiplib.pg_linear_xent_scratch(0, 8, 8, 0, 1) == 0
@@ -111,6 +112,13 @@ def test_descriptors_match_the_header(tmp_path):
         assert got[(cname, "size")] == ctypes.sizeof(cls)
         for f in cls._fields_:
             assert got[(cname, f[0])] == getattr(cls, f[0]).offset, (cname, f[0])
+    # the packed forms ops.py hands over are the same bytes
+    from pagraph_amd import ops
+    drop = (1, 2, 3, 4, 5)
+    ptrs, sizes = tuple(range(10, 26)), tuple(range(-5, 5))
+    assert ops._DROP_DESC(*drop) == bytes(_lib.PgDropout(*drop))
+    assert ops._NORM_DESC(*ptrs, *sizes, 1, 2, 0.5, True, *drop) == bytes(_lib.PgNormDesc(*ptrs, *sizes, 1, 2, 0.5, 1, _lib.PgDropout(*drop)))
+    assert ops._XENT_DESC(*ptrs[:13], *sizes[:7], 1, 2) == bytes(_lib.PgLinearXentDesc(*ptrs[:13], *sizes[:7], 1, 2))
 
 
 # ---- dropout ---------------------------------------------------------------------------------------------------------------
