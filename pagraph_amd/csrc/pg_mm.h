@@ -1,10 +1,11 @@
 // Tiles of matrix products on the matrix cores (gfx950), for operands of 16-bit parts whose reduction range is padded to whole
-// tiles of 64: acc[BM x BN] += sum over parts and k of A(m, k) B(n, k), fp32 accumulation.
+// multiples of 64: acc[BM x BN] += sum over parts and k of A(m, k) B(n, k), fp32 accumulation.
 //
-// Tiles travel from memory into LDS without passing through registers (16 bytes a lane), one tile ahead of the one being
-// multiplied, two buffers, one barrier a step. An operand is stored either way round:
-//   ROWS: p[row][k], k contiguous     -> LDS tile [rows][64], fragments are plain 16-byte reads
-//   COLS: p[k][row], row contiguous   -> LDS tile [64][rows], fragments come from the transposing LDS reads (4 x 16 blocks)
+// Tiles of depth 32 travel from memory into LDS without passing through registers (16 bytes a lane), three tiles ahead of the one
+// being multiplied, four buffers, one barrier a step: a step of a 256 x 256 tile is about 1000 cycles of matrix work, a load that
+// misses the XCD's L2 takes two to three times that. An operand is stored either way round:
+//   ROWS: p[row][k], k contiguous     -> LDS tile [rows][32], fragments are plain 16-byte reads
+//   COLS: p[k][row], row contiguous   -> LDS tile [32][rows], fragments come from the transposing LDS reads (4 x 16 blocks)
 // so that no operand is ever transposed in memory. LDS-direct loads write 64 lanes x 16 bytes contiguously, so the bank swizzle is
 // applied to the address each lane fetches: the 16-byte chunk at position p of a tile row is chunk p ^ swizzle(row).
 #pragma once
@@ -26,7 +27,9 @@ __device__ __forceinline__ f32x16 mma(f16_t, s16x8 a, s16x8 b, f32x16 c) {
 }
 
 enum { ROWS = 0, COLS = 1 };
-constexpr int kDepth = 64;                     // reduction depth of a tile
+constexpr int kDepth = 32;                     // reduction depth of a tile
+constexpr int kPad = 64;                       // what rows of parts are padded to
+constexpr int kBuffers = 4;
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
@@ -59,7 +62,7 @@ struct TileLoad {
     for (int t = 0; t < T; ++t) {
       const int piece = wave * T + t;
       if constexpr (KIND == ROWS) {
-        const int r = piece * 8 + lane / 8, chunk = (lane & 7) ^ ((r >> 1) & 7);
+        const int r = piece * 16 + lane / 4, chunk = (lane & 3) ^ ((r >> 2) & 3);
         const int64_t last = o.rows - 1 - o.r0;
         row[t] = (uint32_t)(r < last ? r : last) * ld2 + chunk * 16;
       } else {
@@ -80,8 +83,8 @@ struct TileLoad {
 #pragma unroll
       for (int t = 0; t < T; ++t) dma16(b + row[t], lds + (wave * T + t) * 512);
     } else {
-      const char* b = base + part * 2 + k0 * ld2;
-      const int64_t left = limit - k0;
+      const int64_t from = k0 < limit ? k0 : limit, left = limit - from;       // (a whole tile may lie behind the last row)
+      const char* b = base + part * 2 + from * ld2;
       const uint32_t last = left < kDepth ? (uint32_t)left : kDepth;
 #pragma unroll
       for (int t = 0; t < T; ++t) dma16(b + ((row[t] < last ? row[t] : last) * ld2 + col[t]), lds + (wave * T + t) * 512);
@@ -90,11 +93,13 @@ struct TileLoad {
 };
 
 // the MFMA operand of rows [rb, rb + 32) at depth 16 kk: lane l holds row rb + l % 32, k = 16 kk + 8 (l / 32) + 0..7
+// (restrict: with alias information on every read the compiler leaves the waits for loads into LDS to wait_loads; without, it
+// waits for all of them before a transposing read)
 template <int KIND, int R>
-__device__ __forceinline__ s16x8 fragment(const short* lds, int rb, int kk, int lane) {
+__device__ __forceinline__ s16x8 fragment(const short* __restrict__ lds, int rb, int kk, int lane) {
   if constexpr (KIND == ROWS) {
     const int r = rb + (lane & 31), chunk = kk * 2 + (lane >> 5);
-    return *reinterpret_cast<const s16x8*>(lds + r * kDepth + ((chunk ^ ((r >> 1) & 7)) << 3));
+    return *reinterpret_cast<const s16x8*>(lds + r * kDepth + ((chunk ^ ((r >> 2) & 3)) << 3));
   } else {
     const int i = lane & 15, g = lane >> 4;
     const int k = kk * 16 + (g >> 1) * 8 + (i >> 2), chunk = (rb >> 3) + (g & 1) * 2 + ((i & 3) >> 1);
@@ -114,66 +119,114 @@ struct Shape {
   static constexpr int TILE = (BM + BN) * kDepth;               // elements of one buffer
 };
 
-template <typename S, int KA, int KB>
-__device__ __forceinline__ void mm_step(const short* __restrict__ cur, short* __restrict__ next, bool more, const TileLoad<KA, S::BM, S::WAVES>& la,
-                                        const TileLoad<KB, S::BN, S::WAVES>& lb, int64_t pa, int64_t pb, int64_t k_next, int wave, int lane,
-                                        f32x16 (&acc)[S::FI][S::FJ]) {
-  if (more) {
-    la.issue(pa, k_next, next, wave);
-    lb.issue(pb, k_next, next + S::BM * kDepth, wave);
-  }
-  const int wm = wave / S::WC, wn = wave % S::WC;
-#pragma unroll
-  for (int kk = 0; kk < kDepth / 16; ++kk) {
-    s16x8 a[S::FI], b[S::FJ];
-#pragma unroll
-    for (int i = 0; i < S::FI; ++i) a[i] = fragment<KA, S::BM>(cur, wm * (S::BM / S::WR) + i * 32, kk, lane);
-#pragma unroll
-    for (int j = 0; j < S::FJ; ++j) b[j] = fragment<KB, S::BN>(cur + S::BM * kDepth, wn * (S::BN / S::WC) + j * 32, kk, lane);
-#pragma unroll
-    for (int i = 0; i < S::FI; ++i)
-#pragma unroll
-      for (int j = 0; j < S::FJ; ++j) acc[i][j] = mma(typename S::E(), a[i], b[j], acc[i][j]);
-  }
+// LDS of a kernel: ONE array of kBuffers tile buffers and `extra` shorts behind them (several variables would carry alias
+// information of their own, see fragment)
+#define PG_MM_LDS(S, name, extra) __shared__ __align__(16) short name[kBuffers * S::TILE + (extra)]
+
+template <int VM>
+__device__ __forceinline__ void wait_loads() {          // at most VM loads of this wave still under way, none of its LDS reads
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((VM & 15) | 7 << 4 | 0 << 8 | (VM >> 4) << 14);
 }
 
-// acc += the product over [k_lo, k_hi), whole tiles. buf0, buf1: S::TILE elements of LDS each; on return every wave may still be
-// reading one of them (synchronise before reusing them).
 template <typename S, int KA, int KB>
-__device__ __forceinline__ void mm_product(const Operand& oa, const Operand& ob, int64_t k_lo, int64_t k_hi, short* buf0, short* buf1,
-                                           f32x16 (&acc)[S::FI][S::FJ]) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+struct Product {
+  static constexpr int LOADS = TileLoad<KA, S::BM, S::WAVES>::T + TileLoad<KB, S::BN, S::WAVES>::T;     // of a wave, per tile
   TileLoad<KA, S::BM, S::WAVES> la;
   TileLoad<KB, S::BN, S::WAVES> lb;
-  la.init(oa, wave, lane);
-  lb.init(ob, wave, lane);
-  const int64_t steps1 = (k_hi - k_lo) / kDepth;
-  const int64_t steps = S::NP == 3 ? 6 * steps1 : steps1;
-  if (steps <= 0) return;
-  // parts of the step's operands: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-  int seg = 0;
-  int64_t k = k_lo;
-  auto part_a = [&]() -> int64_t { return S::NP == 3 ? (seg == 0 ? 2 : seg == 1 || seg == 3 ? 1 : 0) * oa.part : 0; };
-  auto part_b = [&]() -> int64_t { return S::NP == 3 ? (seg == 2 ? 2 : seg == 1 || seg == 4 ? 1 : 0) * ob.part : 0; };
-  auto advance = [&] {
+  int64_t k_lo, k_hi, k, part_a, part_b;
+  int seg, wave, lane;
+
+  // parts of the operands in turn: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+  __device__ __forceinline__ void issue(short* buf) {
+    const int64_t pa = S::NP == 3 ? (seg == 0 ? 2 : seg == 1 || seg == 3 ? 1 : 0) * part_a : 0;
+    const int64_t pb = S::NP == 3 ? (seg == 2 ? 2 : seg == 1 || seg == 4 ? 1 : 0) * part_b : 0;
+    la.issue(pa, k, buf, wave);
+    lb.issue(pb, k, buf + S::BM * kDepth, wave);
     k += kDepth;
     if (S::NP == 3 && k >= k_hi) {
       k = k_lo;
       ++seg;
     }
-  };
-  la.issue(part_a(), k, buf0, wave);
-  lb.issue(part_b(), k, buf0 + S::BM * kDepth, wave);
-  for (int64_t s = 0; s < steps; s += 2) {
-    advance();
-    __syncthreads();                                   // this step's tile has landed, the other buffer's readers are done
-    mm_step<S, KA, KB>(buf0, buf1, s + 1 < steps, la, lb, part_a(), part_b(), k, wave, lane, acc);
-    if (s + 1 < steps) {
-      advance();
-      __syncthreads();
-      mm_step<S, KA, KB>(buf1, buf0, s + 2 < steps, la, lb, part_a(), part_b(), k, wave, lane, acc);
+  }
+  // one step; the caller has waited for this wave's loads of the tile
+  __device__ __forceinline__ void step(const short* cur, short* refill, bool more, f32x16 (&acc)[S::FI][S::FJ]) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();              // every wave's loads of the tile have landed, and all are done with the buffer to refill
+    asm volatile("" ::: "memory");
+    if (more) issue(refill);
+    const int wm = wave / S::WC, wn = wave % S::WC;
+#pragma unroll
+    for (int kk = 0; kk < kDepth / 16; ++kk) {
+      s16x8 a[S::FI], b[S::FJ];
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i) a[i] = fragment<KA, S::BM>(cur, wm * (S::BM / S::WR) + i * 32, kk, lane);
+#pragma unroll
+      for (int j = 0; j < S::FJ; ++j) b[j] = fragment<KB, S::BN>(cur + S::BM * kDepth, wn * (S::BN / S::WC) + j * 32, kk, lane);
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FJ; ++j) acc[i][j] = mma(typename S::E(), a[i], b[j], acc[i][j]);
     }
   }
+};
+
+template <typename S, int KA, int KB>
+__device__ __forceinline__ void mm_run(Product<S, KA, KB>& p, int64_t steps, short* b0, short* b1, short* b2, short* b3, f32x16 (&acc)[S::FI][S::FJ]) {
+  // steps is even: reduction ranges are multiples of kPad
+  constexpr int N = Product<S, KA, KB>::LOADS;
+  p.issue(b0);
+  p.issue(b1);
+  if (steps > 2) p.issue(b2);
+  int64_t left = steps;
+  for (; left >= 8; left -= 4) {
+    wait_loads<2 * N>();
+    p.step(b0, b3, true, acc);
+    wait_loads<2 * N>();
+    p.step(b1, b0, true, acc);
+    wait_loads<2 * N>();
+    p.step(b2, b1, true, acc);
+    wait_loads<2 * N>();
+    p.step(b3, b2, true, acc);
+  }
+  if (left >= 4) {                             // four or six
+    const bool six = left == 6;
+    wait_loads<2 * N>();
+    p.step(b0, b3, true, acc);
+    wait_loads<2 * N>();
+    p.step(b1, b0, six, acc);
+    if (six) wait_loads<2 * N>(); else wait_loads<N>();
+    p.step(b2, b1, six, acc);
+    if (six) wait_loads<2 * N>(); else wait_loads<0>();
+    p.step(b3, b2, false, acc);
+    left -= 4;
+  }
+  if (left == 2) {
+    wait_loads<N>();
+    p.step(b0, b3, false, acc);
+    wait_loads<0>();
+    p.step(b1, b0, false, acc);
+  }
+}
+
+// acc += the product over [k_lo, k_hi), whole tiles. On return every wave may still be reading the buffers (synchronise before
+// reusing them).
+template <typename S, int KA, int KB>
+__device__ __forceinline__ void mm_product(const Operand& oa, const Operand& ob, int64_t k_lo, int64_t k_hi, short* buf,
+                                           f32x16 (&acc)[S::FI][S::FJ]) {
+  Product<S, KA, KB> p;
+  p.lane = threadIdx.x & 63;
+  p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  p.la.init(oa, p.wave, p.lane);
+  p.lb.init(ob, p.wave, p.lane);
+  p.k_lo = p.k = k_lo;
+  p.k_hi = k_hi;
+  p.part_a = oa.part;
+  p.part_b = ob.part;
+  p.seg = 0;
+  const int64_t steps = (S::NP == 3 ? 6 : 1) * ((k_hi - k_lo) / kDepth);
+  if (steps <= 0) return;
+  mm_run<S, KA, KB>(p, steps, buf, buf + S::TILE, buf + 2 * S::TILE, buf + 3 * S::TILE, acc);
 }
 
 // Workgroups go round the 8 XCDs in turn: give each XCD a contiguous run of tiles, so that its own L2 sees a tile's neighbours

@@ -153,9 +153,10 @@ template <typename T, typename S, bool PIECE>
 __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   typedef typename S::E E;
   constexpr int BM = S::BM, BN = S::BN, WM = BM / S::WR, WN = BN / S::WC;
-  __shared__ __align__(16) short buf[2 * S::TILE];
-  __shared__ float2 red[PIECE ? 1 : S::WR][PIECE ? 1 : BN];
-  __shared__ __align__(16) float bias[BM];                   // -inf beyond the last class: its exponentials are 0
+  // behind the tile buffers: the tile's biases, -inf beyond the last class (their exponentials are 0), and the waves' statistics
+  PG_MM_LDS(S, buf, 2 * BM + (PIECE ? 0 : 4 * S::WR * BN));
+  float* bias = reinterpret_cast<float*>(buf + kBuffers * S::TILE);
+  float2(*red)[BN] = reinterpret_cast<float2(*)[BN]>(bias + BM);
   const int64_t row_tiles = ceil_div<int64_t>(a.n, BN), c_tiles = ceil_div<int64_t>(a.c_hi - a.c_lo, BM);
   // an XCD's 32 CUs work on 8 row tiles x 4 class tiles at a time
   const int64_t t = xcd_run(blockIdx.x, row_tiles * c_tiles), group = t / (8 * c_tiles);
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   for (int c = tid; c < BM; c += S::THREADS)
     bias[c] = c0 + c >= a.c_hi ? -INFINITY : a.bias ? (float)((const T*)a.bias)[c0 + c] : 0.f;
   f32x16 acc[S::FI][S::FJ] = {};
-  mm_product<S, ROWS, ROWS>(Operand{a.w, a.w_ld, a.w_part, c0, a.C, 0}, Operand{a.h, a.h_ld, a.h_part, r0, a.h_rows, 0}, 0, a.Kp, buf, buf + S::TILE, acc);
+  mm_product<S, ROWS, ROWS>(Operand{a.w, a.w_ld, a.w_part, c0, a.C, 0}, Operand{a.h, a.h_ld, a.h_part, r0, a.h_rows, 0}, 0, a.Kp, buf, acc);
   const int cw = wm * WM + 4 * (lane >> 5);                  // the lane's first class within the tile
 #pragma unroll
   for (int i = 0; i < S::FI; ++i)
@@ -232,9 +233,8 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
     }
     // [BN rows][BM classes] of one part in the tile buffers, 16-byte chunks swizzled by the row
     constexpr int CH = BM / 8, RP = S::THREADS / CH;
-    static_assert(BM * BN <= S::TILE * 2, "a part of G fits the tile buffers");
-    static_assert(RP * BM * 4 <= 4 * S::TILE, "and so do its column sums");
-    short* stage = buf;
+    static_assert(BM * BN <= kBuffers * S::TILE, "a part of G fits the tile buffers");
+    static_assert(RP * BM * 2 <= kBuffers * S::TILE, "and so do its column sums");
     float sum[8] = {};
 #pragma unroll 1
     for (int part = 0; part < S::NP; ++part) {
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
               acc[i][j][q * 4 + e] -= (float)o[e];
             }
             const int chunk = (wm * WM + i * 32 + 8 * q) / 8;
-            __builtin_memcpy(stage + rl * BM + ((chunk ^ (rl & (CH - 1))) << 3) + 4 * (lane >> 5), o, 8);
+            __builtin_memcpy(buf + rl * BM + ((chunk ^ (rl & (CH - 1))) << 3) + 4 * (lane >> 5), o, 8);
           }
       }
       __syncthreads();
@@ -261,14 +261,14 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
       E* g = (E*)a.g + part * a.g_rows * a.ldg + r0 * a.ldg + (c0 - a.c_lo) + ch * 8;
       for (int rl = tid / CH; rl < BN; rl += RP) {
         E o[8];
-        __builtin_memcpy(o, stage + rl * BM + ((ch ^ (rl & (CH - 1))) << 3), 16);
+        __builtin_memcpy(o, buf + rl * BM + ((ch ^ (rl & (CH - 1))) << 3), 16);
         __builtin_memcpy(g + rl * a.ldg, o, 16);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] += (float)o[e];
       }
     }
     __syncthreads();
-    float* cs = (float*)stage;
+    float* cs = (float*)buf;
 #pragma unroll
     for (int e = 0; e < 8; ++e) cs[(tid / CH) * BM + tid % CH * 8 + e] = sum[e];
     __syncthreads();
@@ -378,16 +378,16 @@ __device__ __forceinline__ void each_output(const f32x16 (&acc)[S::FI][S::FJ], i
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
-  __shared__ __align__(16) short buf[2 * S::TILE];
+  PG_MM_LDS(S, buf, 0);
   const int64_t row_tiles = ceil_div<int64_t>(a.n, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
   const int64_t t = xcd_run(blockIdx.x, row_tiles * k_tiles * a.splits);
   const int64_t kt = t % k_tiles, rt = t / k_tiles % row_tiles, sp = t / k_tiles / row_tiles;
-  const int64_t r0 = rt * S::BM, n0 = kt * S::BN, len = (a.c_hi - a.c_lo + kDepth - 1) / kDepth * kDepth;
+  const int64_t r0 = rt * S::BM, n0 = kt * S::BN, len = (a.c_hi - a.c_lo + kPad - 1) / kPad * kPad;
   const int64_t lo = sp * a.range, hi = lo + a.range < len ? lo + a.range : len;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
   f32x16 acc[S::FI][S::FJ] = {};
   mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
-                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, buf + S::TILE, acc);
+                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, acc);
   const int rl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);       // the lane's first row, first column of the tile
   const int rows = (int)(a.n - r0 < S::BM ? a.n - r0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
   if (a.direct) {
@@ -444,16 +444,16 @@ int lx_sums(const SumArgs& a, const SumArgs& b, const SumArgs& c, const LxArgs& 
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
-  __shared__ __align__(16) short buf[2 * S::TILE];
+  PG_MM_LDS(S, buf, 0);
   const int64_t len = a.c_hi - a.c_lo, c_tiles = ceil_div<int64_t>(len, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
   const int64_t t = xcd_run(blockIdx.x, c_tiles * k_tiles * a.splits);
   const int64_t kt = t % k_tiles, ct = t / k_tiles % c_tiles, sp = t / k_tiles / c_tiles;
-  const int64_t c0 = ct * S::BM, n0 = kt * S::BN, rows = (a.n + kDepth - 1) / kDepth * kDepth;
+  const int64_t c0 = ct * S::BM, n0 = kt * S::BN, rows = (a.n + kPad - 1) / kPad * kPad;
   const int64_t lo = sp * a.range, hi = lo + a.range < rows ? lo + a.range : rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
   f32x16 acc[S::FI][S::FJ] = {};
   mm_product<S, COLS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, c0, a.g_rows, a.ldg},
-                            Operand{a.h, a.h_ld, a.h_part, n0, a.h_rows, a.Kp}, lo, hi, buf, buf + S::TILE, acc);
+                            Operand{a.h, a.h_ld, a.h_part, n0, a.h_rows, a.Kp}, lo, hi, buf, acc);
   const int cl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);
   const int cs = (int)(len - c0 < S::BM ? len - c0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
   if (a.splits > 1) {
@@ -500,7 +500,7 @@ inline void narrow_split(int64_t t, int64_t y_tiles, int32_t* splits, int64_t* r
 inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   LxPlan p{};
   const int64_t np = dtype == PG_DTYPE_F32 ? 3 : 1;
-  p.Kp = up(K, kDepth);
+  p.Kp = up(K, kPad);
   p.h_rows = up(n, 256);
   p.h_bytes = up(np * p.h_rows * p.Kp * 2, 256);
   p.w_bytes = up(np * C * p.Kp * 2, 256);
@@ -540,14 +540,14 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   // splits of the reductions: enough workgroups for the 256 CUs, ranges of at least eight tiles
   const int64_t gm = p.cols == 256 ? 256 : 128;
   auto split = [&](int64_t tiles, int64_t len, int32_t* s, int64_t* range) {
-    int64_t want = ceil_div<int64_t>(gm == 256 ? 256 : 512, tiles), most = len / (8 * kDepth);
+    int64_t want = ceil_div<int64_t>(gm == 256 ? 256 : 512, tiles), most = len / (8 * kPad);
     if (want > most) want = most;
     if (want < 1) want = 1;
-    *range = up(ceil_div<int64_t>(len, want), kDepth);
+    *range = up(ceil_div<int64_t>(len, want), kPad);
     *s = (int32_t)ceil_div<int64_t>(len, *range);
   };
   split(ceil_div<int64_t>(n, gm) * ceil_div<int64_t>(K, p.cols), p.piece, &p.dh_splits, &p.dh_range);
-  split(ceil_div<int64_t>(p.piece, gm) * ceil_div<int64_t>(K, p.cols), up(n, kDepth), &p.dw_splits, &p.dw_range);
+  split(ceil_div<int64_t>(p.piece, gm) * ceil_div<int64_t>(K, p.cols), up(n, kPad), &p.dw_splits, &p.dw_range);
   p.acc_dh = p.dh_splits > 1 || p.pieces > 1 ? up((int64_t)p.dh_splits * n * K * 4, 256) : 0;
   p.acc_dw = p.dw_splits > 1 ? up((int64_t)p.dw_splits * p.piece * K * 4, 256) : 0;
   p.dbp_bytes = up(p.row_tiles * C * 4, 256);
@@ -776,7 +776,7 @@ int lx_args(const pg_linear_xent_desc_t* d, LxArgs* a) {
   if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->lse || !d->flag || !d->scratch))) return PG_ERR_INVALID;
   *a = LxArgs{};
   a->bias = d->bias; a->labels = d->labels;
-  a->n = d->n; a->K = d->K; a->Kp = up(d->K, kDepth); a->C = d->C; a->ignore = d->ignore_index;
+  a->n = d->n; a->K = d->K; a->Kp = up(d->K, kPad); a->C = d->C; a->ignore = d->ignore_index;
   a->lse = d->lse; a->flag = d->flag; a->row_loss = d->row_loss; a->meta = d->meta;
   return PG_OK;
 }
