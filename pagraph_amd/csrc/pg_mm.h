@@ -76,7 +76,11 @@ struct TileLoad {
     base = (const char*)o.p + (KIND == ROWS ? o.r0 * o.ld : o.r0) * 2;
     limit = o.rows - 1;
   }
-  static __device__ __forceinline__ int swz(int k) { return (((k & 3) | ((k >> 1) & 4)) << 1) & (R / 8 - 1); }
+  // COLS: 16 lanes of a transposing read take 32 bytes of four tile rows, their neighbours the next 32 bytes of the same rows: the
+  // four (with the other half-wave's: eight) rows are moved 64 bytes apart in the 256 bytes of banks
+  static __device__ __forceinline__ int swz(int k) {
+    return R >= 256 ? ((k & 3) | ((k >> 1) & 4)) << 2 : R == 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
+  }
   __device__ __forceinline__ void issue(int64_t part, int64_t k0, short* lds, int wave) const {
     if constexpr (KIND == ROWS) {
       const char* b = base + (part + k0) * 2;

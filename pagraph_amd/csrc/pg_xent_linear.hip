@@ -40,16 +40,15 @@ struct LxArgs {
   int64_t ldg, g_rows, c_lo, c_hi;         // the piece's classes
   float* acc;                              // fp32 partial products [split][rows][K]
   float* dbp;                              // [row tiles][C] partial sums of G
+  const float *bias2, *lse2, *rowf2;       // side arrays (SideArgs)
+  const int32_t* lab2;
+  int32_t scaled;
   void *dh, *dw, *db;
   int64_t range;                           // reduction range of one split
   int32_t splits, first, direct;           // direct: one split and one piece, the product itself is the output
 };
 
 __device__ __forceinline__ bool label_ok(int64_t lab, const LxArgs& a) { return lab != a.ignore && lab >= 0 && lab < a.C; }
-// a label's place in the tile of classes [c0, c0 + width), far below 0 elsewhere
-__device__ __forceinline__ int label_in(int64_t lab, int64_t c0, int width) {
-  return lab >= c0 && lab < c0 + width ? (int)(lab - c0) : -(1 << 30);
-}
 __device__ __forceinline__ float out_factor(const LxArgs& a) { return (a.f1 ? *a.f1 : 1.f) * (a.f2 ? *a.f2 : 1.f); }
 
 // rows of T as padded rows of parts: dst [NP][rows_p][ldp]; columns beyond K, rows beyond `rows` and (labels != NULL) rows that do
@@ -61,7 +60,7 @@ struct PackArgs {
   const int64_t* labels;
   int64_t ignore, C;
 };
-// what the narrow form reads beside the operands, padded past the last class / row (see NxArgs): base-2 biases, labels as int32,
+// what the products' epilogues read beside the operands, padded past the last class / row (see NxArgs): base-2 biases, labels as int32,
 // and for the gradients the rows' lse (less the exponent of G's scale) and factors
 struct SideArgs {
   const void* bias;
@@ -153,7 +152,7 @@ template <typename T, typename S, bool PIECE>
 __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   typedef typename S::E E;
   constexpr int BM = S::BM, BN = S::BN, WM = BM / S::WR, WN = BN / S::WC;
-  // behind the tile buffers: the tile's biases, -inf beyond the last class (their exponentials are 0), and the waves' statistics
+  // behind the tile buffers: the tile's biases (base 2, -inf beyond the last class: their exponentials are 0), the waves' statistics
   PG_MM_LDS(S, buf, 2 * BM + (PIECE ? 0 : 4 * S::WR * BN));
   float* bias = reinterpret_cast<float*>(buf + kBuffers * S::TILE);
   float2(*red)[BN] = reinterpret_cast<float2(*)[BN]>(bias + BM);
@@ -163,47 +162,66 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   const int64_t in_group = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8, u = t - group * 8 * c_tiles;
   const int64_t ct = u / in_group, rt = group * 8 + u % in_group, r0 = rt * BN, c0 = a.c_lo + ct * BM;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
-  for (int c = tid; c < BM; c += S::THREADS)
-    bias[c] = c0 + c >= a.c_hi ? -INFINITY : a.bias ? (float)((const T*)a.bias)[c0 + c] : 0.f;
+  for (int c = tid; c < BM; c += S::THREADS) bias[c] = a.bias2[c0 + c];
   f32x16 acc[S::FI][S::FJ] = {};
   mm_product<S, ROWS, ROWS>(Operand{a.w, a.w_ld, a.w_part, c0, a.C, 0}, Operand{a.h, a.h_ld, a.h_part, r0, a.h_rows, 0}, 0, a.Kp, buf, acc);
   const int cw = wm * WM + 4 * (lane >> 5);                  // the lane's first class within the tile
+  int at[S::FJ];                                             // the rows' labels, counted from there
+  float lse[S::FJ];
 #pragma unroll
-  for (int i = 0; i < S::FI; ++i)
+  for (int j = 0; j < S::FJ; ++j) {
+    const int64_t r = r0 + wn * WN + j * 32 + (lane & 31);   // (the side arrays are padded to whole tiles of rows)
+    at[j] = a.lab2[r] - (int)c0 - cw;
+    lse[j] = PIECE ? a.lse2[r] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < S::FI; ++i) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 b = *reinterpret_cast<const float4*>(bias + cw + i * 32 + 8 * q);
 #pragma unroll
       for (int j = 0; j < S::FJ; ++j) {
-        acc[i][j][4 * q] += b.x;
-        acc[i][j][4 * q + 1] += b.y;
-        acc[i][j][4 * q + 2] += b.z;
-        acc[i][j][4 * q + 3] += b.w;
+        acc[i][j][4 * q] = fmaf(acc[i][j][4 * q], kLog2e, b.x);
+        acc[i][j][4 * q + 1] = fmaf(acc[i][j][4 * q + 1], kLog2e, b.y);
+        acc[i][j][4 * q + 2] = fmaf(acc[i][j][4 * q + 2], kLog2e, b.z);
+        acc[i][j][4 * q + 3] = fmaf(acc[i][j][4 * q + 3], kLog2e, b.w);
       }
     }
+#pragma unroll
+    for (int j = 0; j < S::FJ; ++j) {
+      if constexpr (PIECE) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - lse[j]);
+      }
+      if (__any((unsigned)(at[j] - 32 * i) < 32u)) {         // does any of the wave's rows have its label among these 32 classes?
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (at[j] == i * 32 + 8 * (e / 4) + e % 4) {
+            if constexpr (PIECE)
+              acc[i][j][e] -= Mul<T>::G;
+            else
+              a.zlab[r0 + wn * WN + j * 32 + (lane & 31)] = acc[i][j][e];
+          }
+      }
+    }
+  }
   if constexpr (!PIECE) {
 #pragma unroll
     for (int j = 0; j < S::FJ; ++j) {
-      const int rl = wn * WN + j * 32 + (lane & 31);
-      const int64_t r = r0 + rl;
-      const int at = r < a.n ? label_in(a.labels[r], c0, BM) - cw : -1;
       float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          m = fmaxf(m, acc[i][j][e]);
-          if (at == i * 32 + 8 * (e / 4) + e % 4) a.zlab[r] = acc[i][j][e];
-        }
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
       m = fmaxf(m, __shfl_xor(m, 32, kWave));
       const float base = m == -INFINITY ? 0.f : m;         // nothing but -inf so far: every exponential is 0
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - base) * kLog2e);
+        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(acc[i][j][e] - base);
       s += __shfl_xor(s, 32, kWave);
-      if (lane < 32) red[wm][rl] = make_float2(m, s);
+      if (lane < 32) red[wm][wn * WN + j * 32 + lane] = make_float2(m, s);
     }
     __syncthreads();
     for (int rl = tid; rl < BN; rl += S::THREADS)
@@ -213,23 +231,19 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
         for (int i = 1; i < S::WR; ++i) m = fmaxf(m, red[i][rl].x);
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int i = 0; i < S::WR; ++i) s += red[i][rl].y * __builtin_amdgcn_exp2f((red[i][rl].x - base) * kLog2e);
+        for (int i = 0; i < S::WR; ++i) s += red[i][rl].y * __builtin_amdgcn_exp2f(red[i][rl].x - base);
         a.part[(r0 + rl) * a.tiles + ct] = make_float2(m, s);
       }
   } else {
+    if (a.scaled) {                                          // rows with factors of their own
 #pragma unroll
-    for (int j = 0; j < S::FJ; ++j) {
-      const int64_t r = r0 + wn * WN + j * 32 + (lane & 31);
-      const bool in = r < a.n;
-      const int at = in ? label_in(a.labels[r], c0, BM) - cw : -1;
-      const float f = in ? a.rowf[r] * Mul<T>::G : 0.f, lse = in ? a.lse[r] : 0.f;
+      for (int j = 0; j < S::FJ; ++j) {
+        const float f = a.rowf2[r0 + wn * WN + j * 32 + (lane & 31)];
 #pragma unroll
-      for (int i = 0; i < S::FI; ++i)
+        for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f((acc[i][j][e] - lse) * kLog2e) - (at == i * 32 + 8 * (e / 4) + e % 4 ? 1.f : 0.f);
-          acc[i][j][e] = f == 0.f ? 0.f : p * f;
-        }
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = f == 0.f ? 0.f : acc[i][j][e] * f;
+      }
     }
     // [BN rows][BM classes] of one part in the tile buffers, 16-byte chunks swizzled by the row
     constexpr int CH = BM / 8, RP = S::THREADS / CH;
@@ -282,9 +296,8 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   }
 }
 
-// a wave per row: joins the tiles' (narrow form: the splits') statistics. unit: log2(e), or 1 where they are in base 2 already;
-// the lse is kept in the same unit
-__global__ __launch_bounds__(256) void k_lx_rows(LxArgs a, float unit) {
+// a wave per row: joins the tiles' (narrow form: the splits') statistics, in base 2
+__global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   if (r >= a.n) return;
@@ -292,22 +305,22 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a, float unit) {
   for (int64_t t = lane; t < a.tiles; t += 64) {
     const float2 x = a.part[r * a.tiles + t];
     const float mm = fmaxf(m, x.x), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f((m - base) * unit) + x.y * __builtin_amdgcn_exp2f((x.x - base) * unit);
+    s = s * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
     m = mm;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float om = __shfl_xor(m, o, kWave), os = __shfl_xor(s, o, kWave);
     const float mm = fmaxf(m, om), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f((m - base) * unit) + os * __builtin_amdgcn_exp2f((om - base) * unit);
+    s = s * __builtin_amdgcn_exp2f(m - base) + os * __builtin_amdgcn_exp2f(om - base);
     m = mm;
   }
   if (lane == 0) {
-    const float lse = m + (unit == 1.f ? log2f(s) : logf(s));
+    const float lse = m + log2f(s);
     const bool ok = label_ok(a.labels[r], a);
     a.lse[r] = lse;
     a.flag[r] = ok ? 1.f : 0.f;
-    a.row_loss[r] = ok ? (lse - a.zlab[r]) * (unit == 1.f ? 0.693147180559945309417f : 1.f) : 0.f;
+    a.row_loss[r] = ok ? (lse - a.zlab[r]) * 0.693147180559945309417f : 0.f;
   }
 }
 
@@ -385,22 +398,32 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
   const int64_t r0 = rt * S::BM, n0 = kt * S::BN, len = (a.c_hi - a.c_lo + kPad - 1) / kPad * kPad;
   const int64_t lo = sp * a.range, hi = lo + a.range < len ? lo + a.range : len;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
-  f32x16 acc[S::FI][S::FJ] = {};
-  mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
-                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, acc);
   const int rl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);       // the lane's first row, first column of the tile
   const int rows = (int)(a.n - r0 < S::BM ? a.n - r0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
+  float* sum = a.acc + sp * a.n * a.K + r0 * a.K + n0;
+  f32x16 acc[S::FI][S::FJ] = {};
+  if (!a.first) {                              // on top of the earlier pieces' sum (before the product: all loads at once)
+#pragma unroll
+    for (int j = 0; j < S::FJ; ++j) {
+      const int k = kl + 32 * j < cols ? kl + 32 * j : cols - 1;
+#pragma unroll
+      for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int r = rl + i * 32 + 8 * (e / 4) + e % 4;
+          acc[i][j][e] = sum[(r < rows ? r : rows - 1) * a.K + k];
+        }
+    }
+  }
+  mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
+                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, acc);
+  // (rows that do not count leave as zeros, whatever W holds)
   if (a.direct) {
     const float f = out_factor(a) / Mul<T>::G;
     T* out = (T*)a.dh + r0 * a.K + n0;
     each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
   } else {
-    float* out = a.acc + sp * a.n * a.K + r0 * a.K + n0;
-    // (rows that do not count leave as zeros, whatever W holds)
-    if (a.first)
-      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? 0.f : v; });
-    else
-      each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] += a.rowf[r0 + r] == 0.f ? 0.f : v; });
+    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { sum[r * a.K + k] = a.rowf[r0 + r] == 0.f ? 0.f : v; });
   }
 }
 
@@ -504,6 +527,9 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   p.h_rows = up(n, 256);
   p.h_bytes = up(np * p.h_rows * p.Kp * 2, 256);
   p.w_bytes = up(np * C * p.Kp * 2, 256);
+  p.classes_p = up(C, 256) + 64;
+  p.rows_p = p.h_rows + 64;
+  p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
   p.narrow = p.Kp <= (np == 3 ? 128 : 256);
   if (p.narrow) {
     p.xt_stats = 128 * narrow_xb((int)np, (int)p.Kp, NX_STATS);
@@ -516,9 +542,6 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
     p.part_bytes = up(n * p.nx_stats * 8, 256);
     p.acc_dh = p.nx_dh > 1 ? up((int64_t)p.nx_dh * n * K * 4, 256) : 0;
     p.acc_dw = p.nx_dw > 1 ? up((int64_t)p.nx_dw * C * (K + 1) * 4, 256) : 0;
-    p.classes_p = up(C, 256) + 64;
-    p.rows_p = p.h_rows + 64;
-    p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
     return p;
   }
   p.big = n > 128 && C > 128 && p.Kp * np >= 256;
@@ -603,7 +626,7 @@ int launch_narrow(const NxArgs& n, const LxPlan& p, hipStream_t st) {
 }
 
 // the side arrays at s, in the order bias2 | labels | lse | row factors
-inline SideArgs narrow_side(const LxArgs& a, const LxPlan& p, char* s, bool grads) {
+inline SideArgs lx_side_arrays(const LxArgs& a, const LxPlan& p, char* s, bool grads) {
   SideArgs side{};
   const int64_t rows = up(p.rows_p * 4, 256);
   side.bias = a.bias; side.labels = a.labels; side.ignore = a.ignore;
@@ -636,7 +659,7 @@ int narrow_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, c
   a.part = (float2*)s;
   a.zlab = (float*)(s + p.part_bytes);
   char* h = s + p.part_bytes + up(4 * a.n, 256);
-  const SideArgs side = narrow_side(a, p, h + p.h_bytes + p.w_bytes, false);
+  const SideArgs side = lx_side_arrays(a, p, h + p.h_bytes + p.w_bytes, false);
   int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, side, st);
   if (rc != PG_OK) return rc;
   NxArgs n = narrow_args(a, false);
@@ -645,7 +668,7 @@ int narrow_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, c
   rc = launch_narrow<T, NX_STATS>(n, p, st);
   if (rc != PG_OK) return rc;
   a.tiles = p.nx_stats;
-  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a, 1.f);
+  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
@@ -656,7 +679,7 @@ int narrow_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, 
   s += p.acc_dh;
   float* acc_dw = (float*)s;
   s += p.acc_dw;
-  const SideArgs side = narrow_side(a, p, s + p.h_bytes + p.w_bytes, true);
+  const SideArgs side = lx_side_arrays(a, p, s + p.h_bytes + p.w_bytes, true);
   int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, side, st);
   if (rc != PG_OK) return rc;
   SumArgs dh{}, dw{}, db{};
@@ -689,8 +712,10 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   a.part = (float2*)s;
   a.zlab = (float*)(s + p.part_bytes);
   char* h = s + p.part_bytes + up(4 * a.n, 256);
-  const int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, SideArgs{}, st);
+  const SideArgs side = lx_side_arrays(a, p, h + p.h_bytes + p.w_bytes, false);
+  const int rc = lx_operands<T>(a, d, p, h, h + p.h_bytes, false, side, st);
   if (rc != PG_OK) return rc;
+  a.bias2 = side.bias2; a.lab2 = side.lab;
   a.tiles = p.tiles;
   a.c_lo = 0;
   a.c_hi = a.C;
@@ -700,7 +725,7 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   else
     hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, false>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
   PG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a, kLog2e);
+  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
@@ -739,8 +764,11 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   s += p.acc_dw;
   a.dbp = (float*)s;
   s += p.dbp_bytes;
-  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, SideArgs{}, st);
+  const SideArgs side = lx_side_arrays(a, p, s + p.h_bytes + p.w_bytes, true);
+  int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, side, st);
   if (rc != PG_OK) return rc;
+  a.bias2 = side.bias2; a.lab2 = side.lab; a.lse2 = side.lse2; a.rowf2 = side.rowf2;
+  a.scaled = a.rowf != a.flag;
   a.ldg = p.ldg;
   a.g_rows = p.g_rows;
   for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
