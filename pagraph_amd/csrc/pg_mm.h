@@ -40,59 +40,58 @@ __device__ __forceinline__ void dma16(const void* g, void* lds) {
   __builtin_amdgcn_global_load_lds((glb_void*)g, (lds_void*)lds, 16, 0, 0);
 }
 
-// one operand of a tile: R rows of the product from r0 on
+// a value that is the same for all lanes, where the compiler cannot know it (what came out of a division, say): in scalar registers
+// from here on, so that addresses made from it are scalar too
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32;
+}
+
+// one operand of a tile: R rows of the product from r0 on. Memory holds whole tiles of the reduction range
 struct Operand {
   const void* p;
   int64_t ld, part;      // elements between rows, between parts
   int64_t r0;            // first row of the tile (ROWS) / first column (COLS)
-  int64_t rows;          // memory rows that exist: beyond them the last one is read again (its products are dropped or meet zeros)
-  int64_t width;         // COLS: columns that exist (a multiple of 8)
+  int64_t rows;          // ROWS: rows that exist; beyond them the last one is read again (its products are dropped)
+  int64_t width;         // COLS: columns that exist (a multiple of 8); likewise
 };
 
 template <int KIND, int R, int WAVES>
 struct TileLoad {
   static constexpr int T = R * kDepth * 2 / 1024 / WAVES;       // 1 KB pieces per wave
-  uint32_t row[T], col[T];
-  const char* base;
-  uint32_t ld2;
-  int64_t limit;
-  __device__ __forceinline__ void init(const Operand& o, int wave, int lane) {
-    ld2 = (uint32_t)o.ld * 2;
+  uint32_t offset[T];                                           // the lane's, from the tile's first element
+  const char *base, *at;                                        // the tile's at depth 0, the next one to load
+  int64_t step, part;
+  __device__ __forceinline__ void init(const Operand& o, int64_t k_lo, int wave, int lane) {
+    const uint32_t ld2 = (uint32_t)o.ld * 2;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const int piece = wave * T + t;
       if constexpr (KIND == ROWS) {
         const int r = piece * 16 + lane / 4, chunk = (lane & 3) ^ ((r >> 2) & 3);
         const int64_t last = o.rows - 1 - o.r0;
-        row[t] = (uint32_t)(r < last ? r : last) * ld2 + chunk * 16;
+        offset[t] = (uint32_t)(r < last ? r : last) * ld2 + chunk * 16;
       } else {
         constexpr int CH = R / 8, PER = 64 / CH;                 // chunks of a tile row, tile rows of a piece
         const int k = piece * PER + lane / CH, chunk = (lane % CH) ^ swz(k);
         const int64_t last = o.width - 8 - o.r0, c = chunk * 8 < last ? chunk * 8 : last;
-        row[t] = k;
-        col[t] = (uint32_t)(c * 2);
+        offset[t] = k * ld2 + (uint32_t)(c * 2);
       }
     }
-    base = (const char*)o.p + (KIND == ROWS ? o.r0 * o.ld : o.r0) * 2;
-    limit = o.rows - 1;
+    step = KIND == ROWS ? kDepth * 2 : kDepth * o.ld * 2;
+    part = o.part * 2;
+    base = (const char*)o.p + (KIND == ROWS ? (o.r0 * o.ld + k_lo) : (o.r0 + k_lo * o.ld)) * 2;
+  }
+  __device__ __forceinline__ void start(int p) { at = base + p * part; }
+  __device__ __forceinline__ void issue(short* lds, int wave) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) dma16(at + offset[t], lds + (wave * T + t) * 512);
+    at += step;
   }
   // COLS: 16 lanes of a transposing read take 32 bytes of four tile rows, their neighbours the next 32 bytes of the same rows: the
   // four (with the other half-wave's: eight) rows are moved 64 bytes apart in the 256 bytes of banks
   static __device__ __forceinline__ int swz(int k) {
     return R >= 256 ? ((k & 3) | ((k >> 1) & 4)) << 2 : R == 128 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
-  }
-  __device__ __forceinline__ void issue(int64_t part, int64_t k0, short* lds, int wave) const {
-    if constexpr (KIND == ROWS) {
-      const char* b = base + (part + k0) * 2;
-#pragma unroll
-      for (int t = 0; t < T; ++t) dma16(b + row[t], lds + (wave * T + t) * 512);
-    } else {
-      const int64_t from = k0 < limit ? k0 : limit, left = limit - from;       // (a whole tile may lie behind the last row)
-      const char* b = base + part * 2 + from * ld2;
-      const uint32_t last = left < kDepth ? (uint32_t)left : kDepth;
-#pragma unroll
-      for (int t = 0; t < T; ++t) dma16(b + ((row[t] < last ? row[t] : last) * ld2 + col[t]), lds + (wave * T + t) * 512);
-    }
   }
 };
 
@@ -128,88 +127,113 @@ struct Shape {
 #define PG_MM_LDS(S, name, extra) __shared__ __align__(16) short name[kBuffers * S::TILE + (extra)]
 
 template <int VM>
-__device__ __forceinline__ void wait_loads() {          // at most VM loads of this wave still under way, none of its LDS reads
+__device__ __forceinline__ void wait_loads() {          // at most VM loads of this wave still under way
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt((VM & 15) | 7 << 4 | 0 << 8 | (VM >> 4) << 14);
+  __builtin_amdgcn_s_waitcnt((VM & 15) | 7 << 4 | 15 << 8 | (VM >> 4) << 14);
 }
+__device__ __forceinline__ void wait_reads() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14); }      // none of its LDS reads
 
 template <typename S, int KA, int KB>
 struct Product {
   static constexpr int LOADS = TileLoad<KA, S::BM, S::WAVES>::T + TileLoad<KB, S::BN, S::WAVES>::T;     // of a wave, per tile
   TileLoad<KA, S::BM, S::WAVES> la;
   TileLoad<KB, S::BN, S::WAVES> lb;
-  int64_t k_lo, k_hi, k, part_a, part_b;
-  int seg, wave, lane;
+  int seg, seg_steps, seg_left, wave, lane;
 
   // parts of the operands in turn: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+  __device__ __forceinline__ void start() {
+    la.start(S::NP == 3 ? (seg == 0 ? 2 : seg == 1 || seg == 3 ? 1 : 0) : 0);
+    lb.start(S::NP == 3 ? (seg == 2 ? 2 : seg == 1 || seg == 4 ? 1 : 0) : 0);
+  }
   __device__ __forceinline__ void issue(short* buf) {
-    const int64_t pa = S::NP == 3 ? (seg == 0 ? 2 : seg == 1 || seg == 3 ? 1 : 0) * part_a : 0;
-    const int64_t pb = S::NP == 3 ? (seg == 2 ? 2 : seg == 1 || seg == 4 ? 1 : 0) * part_b : 0;
-    la.issue(pa, k, buf, wave);
-    lb.issue(pb, k, buf + S::BM * kDepth, wave);
-    k += kDepth;
-    if (S::NP == 3 && k >= k_hi) {
-      k = k_lo;
+    la.issue(buf, wave);
+    lb.issue(buf + S::BM * kDepth, wave);
+    if (S::NP == 3 && --seg_left == 0) {
+      seg_left = seg_steps;
       ++seg;
+      start();
     }
   }
-  // one step; the caller has waited for this wave's loads of the tile
-  __device__ __forceinline__ void step(const short* cur, short* refill, bool more, f32x16 (&acc)[S::FI][S::FJ]) {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();              // every wave's loads of the tile have landed, and all are done with the buffer to refill
-    asm volatile("" ::: "memory");
-    if (more) issue(refill);
+  struct Fragments {
+    s16x8 a[S::FI], b[S::FJ];
+  };
+  __device__ __forceinline__ void read(const short* tile, int kk, Fragments& f) const {
     const int wm = wave / S::WC, wn = wave % S::WC;
 #pragma unroll
-    for (int kk = 0; kk < kDepth / 16; ++kk) {
-      s16x8 a[S::FI], b[S::FJ];
+    for (int i = 0; i < S::FI; ++i) f.a[i] = fragment<KA, S::BM>(tile, wm * (S::BM / S::WR) + i * 32, kk, lane);
 #pragma unroll
-      for (int i = 0; i < S::FI; ++i) a[i] = fragment<KA, S::BM>(cur, wm * (S::BM / S::WR) + i * 32, kk, lane);
+    for (int j = 0; j < S::FJ; ++j) f.b[j] = fragment<KB, S::BN>(tile + S::BM * kDepth, wn * (S::BN / S::WC) + j * 32, kk, lane);
+  }
+  static __device__ __forceinline__ void multiply(const Fragments& f, f32x16 (&acc)[S::FI][S::FJ]) {
 #pragma unroll
-      for (int j = 0; j < S::FJ; ++j) b[j] = fragment<KB, S::BN>(cur + S::BM * kDepth, wn * (S::BN / S::WC) + j * 32, kk, lane);
+    for (int i = 0; i < S::FI; ++i)
 #pragma unroll
-      for (int i = 0; i < S::FI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FJ; ++j) acc[i][j] = mma(typename S::E(), a[i], b[j], acc[i][j]);
-    }
+      for (int j = 0; j < S::FJ; ++j) acc[i][j] = mma(typename S::E(), f.a[i], f.b[j], acc[i][j]);
+  }
+  // One step. f: the tile's fragments of depth 0, read a step ago; leaves with the next tile's. Reads run behind the matrix
+  // instructions of the half tile before. The caller has waited for this wave's loads of the NEXT tile.
+  template <bool LAST>
+  __device__ __forceinline__ void step(const short* cur, const short* next, short* refill, bool more, Fragments& f, f32x16 (&acc)[S::FI][S::FJ]) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();              // every wave's loads of the next tile have landed, all are done with the buffer to refill
+    asm volatile("" ::: "memory");
+    if (more) issue(refill);
+    // in this order, whatever the scheduler thinks of the registers; the reads waited for were issued half a tile ago
+    Fragments g;
+    wait_reads();
+    read(cur, 1, g);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(f, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    wait_reads();
+    if (!LAST) read(next, 0, f);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(g, acc);
+    __builtin_amdgcn_sched_barrier(0);
   }
 };
 
 template <typename S, int KA, int KB>
-__device__ __forceinline__ void mm_run(Product<S, KA, KB>& p, int64_t steps, short* b0, short* b1, short* b2, short* b3, f32x16 (&acc)[S::FI][S::FJ]) {
+__device__ __forceinline__ void mm_run(Product<S, KA, KB>& p, int steps, short* b0, short* b1, short* b2, short* b3, f32x16 (&acc)[S::FI][S::FJ]) {
   // steps is even: reduction ranges are multiples of kPad
   constexpr int N = Product<S, KA, KB>::LOADS;
+  static_assert(kDepth == 32, "two fragments a tile");
+  typename Product<S, KA, KB>::Fragments f;
   p.issue(b0);
   p.issue(b1);
   if (steps > 2) p.issue(b2);
-  int64_t left = steps;
+  if (steps > 2) wait_loads<2 * N>(); else wait_loads<N>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  p.read(b0, 0, f);
+  int left = steps;
   for (; left >= 8; left -= 4) {
-    wait_loads<2 * N>();
-    p.step(b0, b3, true, acc);
-    wait_loads<2 * N>();
-    p.step(b1, b0, true, acc);
-    wait_loads<2 * N>();
-    p.step(b2, b1, true, acc);
-    wait_loads<2 * N>();
-    p.step(b3, b2, true, acc);
+    wait_loads<N>();
+    p.template step<false>(b0, b1, b3, true, f, acc);
+    wait_loads<N>();
+    p.template step<false>(b1, b2, b0, true, f, acc);
+    wait_loads<N>();
+    p.template step<false>(b2, b3, b1, true, f, acc);
+    wait_loads<N>();
+    p.template step<false>(b3, b0, b2, true, f, acc);
   }
   if (left >= 4) {                             // four or six
     const bool six = left == 6;
-    wait_loads<2 * N>();
-    p.step(b0, b3, true, acc);
-    wait_loads<2 * N>();
-    p.step(b1, b0, six, acc);
-    if (six) wait_loads<2 * N>(); else wait_loads<N>();
-    p.step(b2, b1, six, acc);
-    if (six) wait_loads<2 * N>(); else wait_loads<0>();
-    p.step(b3, b2, false, acc);
+    wait_loads<N>();
+    p.template step<false>(b0, b1, b3, true, f, acc);
+    wait_loads<N>();
+    p.template step<false>(b1, b2, b0, six, f, acc);
+    if (six) wait_loads<N>(); else wait_loads<0>();
+    p.template step<false>(b2, b3, b1, six, f, acc);
+    if (six) wait_loads<N>(); else wait_loads<0>();
+    p.template step<false>(b3, b0, b2, false, f, acc);         // (four: reads a buffer that no load has filled anew; not used)
     left -= 4;
   }
   if (left == 2) {
-    wait_loads<N>();
-    p.step(b0, b3, false, acc);
     wait_loads<0>();
-    p.step(b1, b0, false, acc);
+    p.template step<false>(b0, b1, b3, false, f, acc);
+    p.template step<true>(b1, b2, b0, false, f, acc);
   }
 }
 
@@ -221,21 +245,19 @@ __device__ __forceinline__ void mm_product(const Operand& oa, const Operand& ob,
   Product<S, KA, KB> p;
   p.lane = threadIdx.x & 63;
   p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  p.la.init(oa, p.wave, p.lane);
-  p.lb.init(ob, p.wave, p.lane);
-  p.k_lo = p.k = k_lo;
-  p.k_hi = k_hi;
-  p.part_a = oa.part;
-  p.part_b = ob.part;
+  p.la.init(oa, k_lo, p.wave, p.lane);
+  p.lb.init(ob, k_lo, p.wave, p.lane);
   p.seg = 0;
-  const int64_t steps = (S::NP == 3 ? 6 : 1) * ((k_hi - k_lo) / kDepth);
+  p.seg_steps = p.seg_left = uniform((int)((k_hi - k_lo) / kDepth));
+  p.start();
+  const int steps = (S::NP == 3 ? 6 : 1) * p.seg_steps;
   if (steps <= 0) return;
   mm_run<S, KA, KB>(p, steps, buf, buf + S::TILE, buf + 2 * S::TILE, buf + 3 * S::TILE, acc);
 }
 
 // Workgroups go round the 8 XCDs in turn: give each XCD a contiguous run of tiles, so that its own L2 sees a tile's neighbours
-__device__ __forceinline__ int64_t xcd_run(int64_t b, int64_t total) {
-  const int64_t per = total / 8, rest = total % 8, x = b % 8, i = b / 8;
+__device__ __forceinline__ uint32_t xcd_run(uint32_t b, uint32_t total) {
+  const uint32_t per = total / 8, rest = total % 8, x = b % 8, i = b / 8;
   return x * per + (x < rest ? x : rest) + i;
 }
 

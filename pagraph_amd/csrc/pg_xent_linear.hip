@@ -156,11 +156,12 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
   PG_MM_LDS(S, buf, 2 * BM + (PIECE ? 0 : 4 * S::WR * BN));
   float* bias = reinterpret_cast<float*>(buf + kBuffers * S::TILE);
   float2(*red)[BN] = reinterpret_cast<float2(*)[BN]>(bias + BM);
-  const int64_t row_tiles = ceil_div<int64_t>(a.n, BN), c_tiles = ceil_div<int64_t>(a.c_hi - a.c_lo, BM);
+  const uint32_t row_tiles = (uint32_t)ceil_div<int64_t>(a.n, BN), c_tiles = (uint32_t)ceil_div<int64_t>(a.c_hi - a.c_lo, BM);
   // an XCD's 32 CUs work on 8 row tiles x 4 class tiles at a time
-  const int64_t t = xcd_run(blockIdx.x, row_tiles * c_tiles), group = t / (8 * c_tiles);
-  const int64_t in_group = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8, u = t - group * 8 * c_tiles;
-  const int64_t ct = u / in_group, rt = group * 8 + u % in_group, r0 = rt * BN, c0 = a.c_lo + ct * BM;
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x), group = t / (8 * c_tiles);
+  const uint32_t in_group = row_tiles - group * 8 < 8 ? row_tiles - group * 8 : 8, u = t - group * 8 * c_tiles;
+  const int ct = uniform((int)(u / in_group)), rt = uniform((int)(group * 8 + u % in_group));
+  const int64_t r0 = (int64_t)rt * BN, c0 = a.c_lo + (int64_t)ct * BM;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
   for (int c = tid; c < BM; c += S::THREADS) bias[c] = a.bias2[c0 + c];
   f32x16 acc[S::FI][S::FJ] = {};
@@ -392,10 +393,10 @@ template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
   PG_MM_LDS(S, buf, 0);
-  const int64_t row_tiles = ceil_div<int64_t>(a.n, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
-  const int64_t t = xcd_run(blockIdx.x, row_tiles * k_tiles * a.splits);
-  const int64_t kt = t % k_tiles, rt = t / k_tiles % row_tiles, sp = t / k_tiles / row_tiles;
-  const int64_t r0 = rt * S::BM, n0 = kt * S::BN, len = (a.c_hi - a.c_lo + kPad - 1) / kPad * kPad;
+  const uint32_t row_tiles = (uint32_t)ceil_div<int64_t>(a.n, S::BM), k_tiles = (uint32_t)ceil_div<int64_t>(a.K, S::BN);
+  const uint32_t t = xcd_run(blockIdx.x, gridDim.x);
+  const int kt = uniform((int)(t % k_tiles)), rt = uniform((int)(t / k_tiles % row_tiles)), sp = uniform((int)(t / k_tiles / row_tiles));
+  const int64_t r0 = (int64_t)rt * S::BM, n0 = (int64_t)kt * S::BN, len = (a.c_hi - a.c_lo + kPad - 1) / kPad * kPad;
   const int64_t lo = sp * a.range, hi = lo + a.range < len ? lo + a.range : len;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
   const int rl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);       // the lane's first row, first column of the tile
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
     }
   }
   mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
-                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, a.C - a.c_lo, a.Kp}, lo, hi, buf, acc);
+                            Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, 0, a.Kp}, lo, hi, buf, acc);
   // (rows that do not count leave as zeros, whatever W holds)
   if (a.direct) {
     const float f = out_factor(a) / Mul<T>::G;
@@ -468,15 +469,15 @@ template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
   PG_MM_LDS(S, buf, 0);
-  const int64_t len = a.c_hi - a.c_lo, c_tiles = ceil_div<int64_t>(len, S::BM), k_tiles = ceil_div<int64_t>(a.K, S::BN);
-  const int64_t t = xcd_run(blockIdx.x, c_tiles * k_tiles * a.splits);
-  const int64_t kt = t % k_tiles, ct = t / k_tiles % c_tiles, sp = t / k_tiles / c_tiles;
-  const int64_t c0 = ct * S::BM, n0 = kt * S::BN, rows = (a.n + kPad - 1) / kPad * kPad;
+  const int64_t len = a.c_hi - a.c_lo, rows = (a.n + kPad - 1) / kPad * kPad;
+  const uint32_t c_tiles = (uint32_t)ceil_div<int64_t>(len, S::BM), k_tiles = (uint32_t)ceil_div<int64_t>(a.K, S::BN), t = xcd_run(blockIdx.x, gridDim.x);
+  const int kt = uniform((int)(t % k_tiles)), ct = uniform((int)(t / k_tiles % c_tiles)), sp = uniform((int)(t / k_tiles / c_tiles));
+  const int64_t c0 = (int64_t)ct * S::BM, n0 = (int64_t)kt * S::BN;
   const int64_t lo = sp * a.range, hi = lo + a.range < rows ? lo + a.range : rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / S::WC, wn = wave % S::WC;
   f32x16 acc[S::FI][S::FJ] = {};
-  mm_product<S, COLS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, c0, a.g_rows, a.ldg},
-                            Operand{a.h, a.h_ld, a.h_part, n0, a.h_rows, a.Kp}, lo, hi, buf, acc);
+  mm_product<S, COLS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, c0, 0, a.ldg},
+                            Operand{a.h, a.h_ld, a.h_part, n0, 0, a.Kp}, lo, hi, buf, acc);
   const int cl = wm * WM + 4 * (lane >> 5), kl = wn * WN + (lane & 31);
   const int cs = (int)(len - c0 < S::BM ? len - c0 : S::BM), cols = (int)(a.K - n0 < S::BN ? a.K - n0 : S::BN);
   if (a.splits > 1) {
@@ -494,7 +495,7 @@ inline int64_t up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
 // sizes of one call: everything follows from the shapes, types and alignments of the operands, so that the scratch the caller
 // allocates (for packed operands always) fits the launches
 struct LxPlan {
-  int64_t Kp, h_rows, tiles, row_tiles, piece, ldg, g_rows;
+  int64_t Kp, h_rows, w_rows, tiles, row_tiles, piece, ldg, g_rows;
   int64_t h_bytes, w_bytes, part_bytes, g_bytes, acc_dh, acc_dw, dbp_bytes;
   int32_t dh_splits, dw_splits, pieces;
   int64_t dh_range, dw_range;
@@ -526,7 +527,8 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   p.Kp = up(K, kPad);
   p.h_rows = up(n, 256);
   p.h_bytes = up(np * p.h_rows * p.Kp * 2, 256);
-  p.w_bytes = up(np * C * p.Kp * 2, 256);
+  p.w_rows = up(C, kPad);
+  p.w_bytes = up(np * p.w_rows * p.Kp * 2, 256);
   p.classes_p = up(C, 256) + 64;
   p.rows_p = p.h_rows + 64;
   p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
@@ -593,14 +595,15 @@ int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
     h = PackArgs{d->h, h_dst, d->n, p.h_rows, d->K, d->h_stride, p.Kp, d->labels, d->ignore_index, d->C};
     a.h = h_dst; a.h_ld = p.Kp; a.h_rows = p.h_rows; a.h_part = p.h_rows * p.Kp;
   }
-  if (fits(d->W, d->w_stride)) {
+  // (dh's product reads whole tiles of classes: in the wide form's backward pass only a table of such is used in place)
+  if (fits(d->W, d->w_stride) && (p.narrow || !mask || d->C % kPad == 0)) {
     a.w = d->W; a.w_ld = d->w_stride;
   } else {
-    w = PackArgs{d->W, w_dst, d->C, d->C, d->K, d->w_stride, p.Kp, nullptr, 0, 0};
-    a.w = w_dst; a.w_ld = p.Kp; a.w_part = d->C * p.Kp;
+    w = PackArgs{d->W, w_dst, d->C, p.w_rows, d->K, d->w_stride, p.Kp, nullptr, 0, 0};
+    a.w = w_dst; a.w_ld = p.Kp; a.w_part = p.w_rows * p.Kp;
   }
   if (!h.dst && !w.dst && !side.bias2) return PG_OK;
-  const int64_t most = (w.dst && (!h.dst || d->C > p.h_rows) ? d->C : h.dst ? p.h_rows : 32) * (p.Kp / 8);
+  const int64_t most = (w.dst && (!h.dst || p.w_rows > p.h_rows) ? p.w_rows : h.dst ? p.h_rows : 32) * (p.Kp / 8);
   const int64_t blocks = ceil_div<int64_t>(most, 256);
   if (!h.dst) { h = w; w = PackArgs{}; }
   hipLaunchKernelGGL(k_lx_pack<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), side.bias2 ? 3 : w.dst ? 2 : 1), dim3(256), 0, st, h, w, side);

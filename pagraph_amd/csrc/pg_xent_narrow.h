@@ -209,8 +209,9 @@ __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
   typedef Narrow<T, KP, XB> N;
   __shared__ __align__(16) short buf[2 * N::TILE];
   __shared__ __align__(16) float side[2 * 192];
-  const int64_t x_tiles = ceil_div<int64_t>(a.nx, N::XT), t = xcd_run(blockIdx.x, x_tiles * a.splits);
-  const int64_t xt = t % x_tiles, sp = t / x_tiles;        // an XCD's workgroups walk the same y at the same time
+  const uint32_t x_tiles = (uint32_t)ceil_div<int64_t>(a.nx, N::XT), t = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t xt = uniform((int)(t % x_tiles));
+  const int sp = uniform((int)(t / x_tiles));              // an XCD's workgroups walk the same y at the same time
   const int64_t y_lo = sp * a.range, y_hi = y_lo + a.range < a.ny ? y_lo + a.range : a.ny;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   NarrowState<T, KP, XB, MODE> st;
