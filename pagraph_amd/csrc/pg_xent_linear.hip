@@ -499,7 +499,7 @@ struct LxPlan {
   int64_t h_bytes, w_bytes, part_bytes, g_bytes, acc_dh, acc_dw, dbp_bytes;
   int32_t dh_splits, dw_splits, pieces;
   int64_t dh_range, dw_range;
-  int big, cols;                            // tile shapes: 256 x 256 logits; columns of a gradient tile
+  int big, dh_cols, dw_cols;                // tile shapes: 256 x 256 logits; columns of the gradients' tiles
   // narrow form
   int narrow, xt_stats, xt_grad, yt;
   int32_t nx_stats, nx_dh, nx_dw;           // splits
@@ -546,12 +546,13 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
     p.acc_dw = p.nx_dw > 1 ? up((int64_t)p.nx_dw * C * (K + 1) * 4, 256) : 0;
     return p;
   }
-  p.big = n > 128 && C > 128 && p.Kp * np >= 256;
+  // 256 x 256 tiles need a quarter less LDS traffic and two thirds of the loads of 128 x 128 ones, and fill the card from 256 tiles
+  // on: at half of that 128 x 128 ones, two to a CU, are ahead (fp16 777 x 602 -> 1153, 20 against 70 tiles: logits 22 -> XX us)
+  p.big = ceil_div<int64_t>(n, 256) * ceil_div<int64_t>(C, 256) >= 192;
   const int64_t bm = p.big ? 256 : 128;
   p.tiles = ceil_div<int64_t>(C, bm);
   p.row_tiles = ceil_div<int64_t>(n, bm);
   p.part_bytes = up(n * p.tiles * 8, 256);
-  p.cols = p.Kp >= 256 ? 256 : p.Kp > 64 ? 128 : 64;
   // a piece of G
   p.g_rows = up(n, 256);
   int64_t cols = (int64_t(256) << 20) / (np * 2 * p.g_rows) / 256 * 256;
@@ -560,19 +561,21 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   p.pieces = (int32_t)ceil_div<int64_t>(C, cols);
   p.piece = up(ceil_div<int64_t>(C, p.pieces), 256);
   p.pieces = (int32_t)ceil_div<int64_t>(C, p.piece);
-  p.ldg = p.piece;
+  p.ldg = p.piece + 64;        // (rows a power of two apart would share their memory channels: dh 296 -> 279 us at 8192 x 1024 -> 65536)
   p.g_bytes = up(np * p.g_rows * p.ldg * 2, 256);
-  // splits of the reductions: enough workgroups for the 256 CUs, ranges of at least eight tiles
-  const int64_t gm = p.cols == 256 ? 256 : 128;
-  auto split = [&](int64_t tiles, int64_t len, int32_t* s, int64_t* range) {
-    int64_t want = ceil_div<int64_t>(gm == 256 ? 256 : 512, tiles), most = len / (8 * kPad);
+  // gradient tiles likewise; splits of the reductions: enough workgroups for the 256 CUs, ranges of at least four times 64
+  auto split = [&](int64_t rows, int64_t len, int* cols, int32_t* s, int64_t* range) {
+    const int64_t big = ceil_div<int64_t>(rows, 256) * ceil_div<int64_t>(K, 256);
+    *cols = p.Kp >= 256 && big * (len / 1024) >= 192 ? 256 : p.Kp > 64 ? 128 : 64;
+    const int64_t tiles = *cols == 256 ? big : ceil_div<int64_t>(rows, 128) * ceil_div<int64_t>(K, *cols);
+    int64_t want = ceil_div<int64_t>(*cols == 256 ? 256 : 512, tiles), most = len / (4 * kPad);
     if (want > most) want = most;
     if (want < 1) want = 1;
     *range = up(ceil_div<int64_t>(len, want), kPad);
     *s = (int32_t)ceil_div<int64_t>(len, *range);
   };
-  split(ceil_div<int64_t>(n, gm) * ceil_div<int64_t>(K, p.cols), p.piece, &p.dh_splits, &p.dh_range);
-  split(ceil_div<int64_t>(p.piece, gm) * ceil_div<int64_t>(K, p.cols), up(n, kPad), &p.dw_splits, &p.dw_range);
+  split(n, p.piece, &p.dh_cols, &p.dh_splits, &p.dh_range);
+  split(p.piece, up(n, kPad), &p.dw_cols, &p.dw_splits, &p.dw_range);
   p.acc_dh = p.dh_splits > 1 || p.pieces > 1 ? up((int64_t)p.dh_splits * n * K * 4, 256) : 0;
   p.acc_dw = p.dw_splits > 1 ? up((int64_t)p.dw_splits * p.piece * K * 4, 256) : 0;
   p.dbp_bytes = up(p.row_tiles * C * 4, 256);
@@ -734,24 +737,42 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
 }
 
 template <typename T, typename S>
+int lx_launch_dh(const LxArgs& a, hipStream_t st) {
+  const int64_t tiles = ceil_div<int64_t>(a.n, S::BM) * ceil_div<int64_t>(a.K, S::BN) * a.splits;
+  hipLaunchKernelGGL((k_lx_dh<T, S>), dim3((unsigned)tiles), dim3(S::THREADS), 0, st, a);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+template <typename T, typename S>
+int lx_launch_dw(const LxArgs& a, hipStream_t st) {
+  const int64_t tiles = ceil_div<int64_t>(a.c_hi - a.c_lo, S::BM) * ceil_div<int64_t>(a.K, S::BN) * a.splits;
+  hipLaunchKernelGGL((k_lx_dw<T, S>), dim3((unsigned)tiles), dim3(S::THREADS), 0, st, a);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
+}
+
+// one piece's share of the gradients
+template <typename T>
 int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipStream_t st) {
-  const int64_t k_tiles = ceil_div<int64_t>(a.K, S::BN), len = a.c_hi - a.c_lo;
   if (a.dh) {
     a.acc = acc_dh;
     a.splits = p.dh_splits;
     a.range = p.dh_range;
     a.first = a.c_lo == 0;
     a.direct = p.dh_splits == 1 && p.pieces == 1;
-    hipLaunchKernelGGL((k_lx_dh<T, S>), dim3((unsigned)(ceil_div<int64_t>(a.n, S::BM) * k_tiles * a.splits)), dim3(S::THREADS), 0, st, a);
-    PG_LAUNCH_CHECK();
+    const int rc = p.dh_cols == 256 ? lx_launch_dh<T, BigTile<T>>(a, st) : p.dh_cols == 128 ? lx_launch_dh<T, MidTile<T>>(a, st)
+                                                                                            : lx_launch_dh<T, SlimTile<T>>(a, st);
+    if (rc != PG_OK) return rc;
   }
   if (a.dw) {
     a.acc = acc_dw;
     a.splits = p.dw_splits;
     a.range = p.dw_range;
-    hipLaunchKernelGGL((k_lx_dw<T, S>), dim3((unsigned)(ceil_div<int64_t>(len, S::BM) * k_tiles * a.splits)), dim3(S::THREADS), 0, st, a);
-    PG_LAUNCH_CHECK();
-    if (a.splits > 1) return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, len * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
+    const int rc = p.dw_cols == 256 ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw_cols == 128 ? lx_launch_dw<T, MidTile<T>>(a, st)
+                                                                                            : lx_launch_dw<T, SlimTile<T>>(a, st);
+    if (rc != PG_OK) return rc;
+    if (a.splits > 1)
+      return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, (a.c_hi - a.c_lo) * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
   }
   return PG_OK;
 }
@@ -782,9 +803,7 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
     else
       hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, true>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
     PG_LAUNCH_CHECK();
-    rc = p.cols == 256 ? lx_gradients<T, BigTile<T>>(a, p, acc_dh, acc_dw, st)
-       : p.cols == 128 ? lx_gradients<T, MidTile<T>>(a, p, acc_dh, acc_dw, st)
-                       : lx_gradients<T, SlimTile<T>>(a, p, acc_dh, acc_dw, st);
+    rc = lx_gradients<T>(a, p, acc_dh, acc_dw, st);
     if (rc != PG_OK) return rc;
   }
   const bool direct = p.dh_splits == 1 && p.pieces == 1;

@@ -48,19 +48,26 @@ struct Narrow {
   static_assert(PIECES % WAVES == 0, "whole pieces a wave");
 };
 
+// 16-byte chunk c of tile row y sits at position c ^ nx_swz(y): the 16 rows of a quarter-wave's row reads meet 16 different
+// 16-byte banks, and of the 8 rows x 64 bytes of a transposing read no bank gets more than two
+template <int KP>
+__device__ __forceinline__ int nx_swz(int y) {
+  return KP % 128 == 0 ? (y & 3) << 2 | ((y >> 2) & 3) : ((y >> 1) & 1) << 2 | ((y >> 2) & 1) << 1 | ((y >> 3) & 1);
+}
+
 template <typename N, int KP>
-__device__ __forceinline__ s16x8 nx_rows(const short* part, int yb, int kk, int lane) {
+__device__ __forceinline__ s16x8 nx_rows(const short* __restrict__ part, int yb, int kk, int lane) {
   const int y = yb * 32 + (lane & 31), chunk = kk * 2 + (lane >> 5);
-  return *reinterpret_cast<const s16x8*>(part + y * KP + ((chunk ^ (y & 7)) << 3));
+  return *reinterpret_cast<const s16x8*>(part + y * KP + ((chunk ^ nx_swz<KP>(y)) << 3));
 }
 // columns [32 mb, +32) of the tile, reduction over the 16 y that a lane's G values 8 s .. 8 s + 7 stand for
 template <typename N, int KP>
-__device__ __forceinline__ s16x8 nx_cols(const short* part, int yb, int s, int mb, int lane) {
+__device__ __forceinline__ s16x8 nx_cols(const short* __restrict__ part, int yb, int s, int mb, int lane) {
   const int i = lane & 15, g = lane >> 4, h = g >> 1;
   const int chunk = mb * 4 + (g & 1) * 2 + ((i & 3) >> 1), y = yb * 32 + s * 16 + 4 * h + (i >> 2);
-  const short* p = part + y * KP + ((chunk ^ (4 * h + (i >> 2))) << 3) + (i & 1) * 4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * KP));
+  const short* p = part + y * KP + (i & 1) * 4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + ((chunk ^ nx_swz<KP>(y)) << 3)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 8 * KP + ((chunk ^ nx_swz<KP>(y + 8)) << 3)));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -103,7 +110,7 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
 #pragma unroll
     for (int t = 0; t < N::PER; ++t) {
       const int piece = wave * N::PER + t, part = piece / (N::PIECES / N::NP);
-      const int lin = (piece % (N::PIECES / N::NP)) * 64 + lane, row = lin / N::CH, chunk = (lin % N::CH) ^ (row & 7);
+      const int lin = (piece % (N::PIECES / N::NP)) * 64 + lane, row = lin / N::CH, chunk = (lin % N::CH) ^ nx_swz<KP>(row);
       dma16(base + part * a.y_part * 2 + ((uint32_t)(row < last ? row : last) * ld2 + chunk * 16), next + piece * 512);
     }
     if (wave == 0) {
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
 #pragma unroll
     for (int t2 = 0; t2 < N::PER; ++t2) {
       const int piece = wave * N::PER + t2, part = piece / (N::PIECES / N::NP);
-      const int lin = (piece % (N::PIECES / N::NP)) * 64 + lane, row = lin / N::CH, chunk = (lin % N::CH) ^ (row & 7);
+      const int lin = (piece % (N::PIECES / N::NP)) * 64 + lane, row = lin / N::CH, chunk = (lin % N::CH) ^ nx_swz<KP>(row);
       dma16(base + part * a.y_part * 2 + ((uint32_t)(row < last ? row : last) * (uint32_t)a.y_ld * 2 + chunk * 16), buf + piece * 512);
     }
     if (wave == 0) {

@@ -478,10 +478,21 @@ def test_linear_cross_entropy_reductions(dev, hiplib, t, reduction, bias):
 
 
 @gpu
-@pytest.mark.parametrize("t", [F32, BF16])
-def test_linear_cross_entropy_in_several_pieces(dev, hiplib, t):
-    """n * C past the size of one piece of the vocabulary, its last piece ragged"""
-    check_xent(dev, 4099, 40, 20011, t, ignored=0.05)
+@pytest.mark.parametrize("n,K,C,t", [(4099, 40, 20011, F32), (4099, 40, 20011, BF16), (4099, 131, 11003, F32), (4099, 260, 33001, BF16),
+                                     (300, 300, 9000, F16), (2500, 520, 4097, BF16), (1300, 1030, 2050, F32)])
+def test_linear_cross_entropy_large(dev, hiplib, n, K, C, t):
+    """several splits of the classes and rows, several pieces of the vocabulary with a ragged last one, large and small tiles"""
+    check_xent(dev, n, K, C, t, ignored=0.05)
+
+
+@gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("K", [64, 128, 192, 256, 320])
+def test_linear_cross_entropy_every_row_width(dev, hiplib, K, t):
+    """rows that fill their padding exactly, read in place where the type allows, and one column less"""
+    check_xent(dev, 150, K, 700, t)
+    check_xent(dev, 150, K - 1, 700, t, ignored=0.3)
+    check_xent(dev, 90, K, 321, t, reduction="none")
 
 
 @gpu
