@@ -631,8 +631,8 @@ int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
 /* CrossEntropyLoss(h W^T + bias, labels) for any number of classes without the logits [n, C] in memory (a wide head's counterpart
  * of pg_head + pg_xent_*): h [n, K], W [C, K], bias [C] or NULL, all of `dtype`. Rows whose label is ignore_index or outside
  * [0, C) are not counted, have loss 0 and gradient 0, and do not enter dW / db whatever h holds there.
- * forward:  lse [n], flag [n] (1: counted), row_loss [n], meta[4] = {mean loss (nan when no row counts), 1 / #counted rows (0),
- *           sum, unused}.
+ * forward:  PG_XENT_MEAN / _SUM: *loss (nan for the mean when no row counts); PG_XENT_NONE: row_loss [n]. And what the backward
+ *           pass reads: lse [n], flag [n] (1: counted), meta [1] = 1 / #counted rows (0).
  * backward: given the forward's lse, flag, meta and grad = d objective / d loss (device fp32: one value for PG_XENT_MEAN / _SUM,
  *           [n] with grad_stride for PG_XENT_NONE): dh [n, K], dW [C, K], db [C], dense, each may be NULL. n >= 1.
  * scratch: pg_linear_xent_scratch(n, K, C, dtype, backward) bytes (negative: the sizes are refused). Deterministic.           */
@@ -647,6 +647,7 @@ typedef struct pg_linear_xent_desc {
   float* lse;
   float* flag;
   float* row_loss;
+  float* loss;
   float* meta;
   const float* grad;
   void* dh;

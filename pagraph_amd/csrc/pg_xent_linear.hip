@@ -325,9 +325,9 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
   }
 }
 
-// one block, fixed order: meta = {mean, 1 / counted rows, sum}
+// one block, fixed order: the loss (mean or sum) and meta = 1 / counted rows
 __global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_loss, const float* __restrict__ flag, int64_t n,
-                                                  float* __restrict__ meta) {
+                                                  int mean, float* __restrict__ loss, float* __restrict__ meta) {
   __shared__ float ss[1024];
   __shared__ int sc[1024];
   float s = 0.f;
@@ -347,9 +347,8 @@ __global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    meta[0] = sc[0] > 0 ? ss[0] / (float)sc[0] : NAN;       // as ops.cross_entropy: a mean over no rows
-    meta[1] = sc[0] > 0 ? 1.f / (float)sc[0] : 0.f;
-    meta[2] = ss[0];
+    *loss = !mean ? ss[0] : sc[0] > 0 ? ss[0] / (float)sc[0] : NAN;       // as ops.cross_entropy: a mean over no rows
+    *meta = sc[0] > 0 ? 1.f / (float)sc[0] : 0.f;
   }
 }
 
@@ -827,7 +826,7 @@ int lx_args(const pg_linear_xent_desc_t* d, LxArgs* a) {
   *a = LxArgs{};
   a->bias = d->bias; a->labels = d->labels;
   a->n = d->n; a->K = d->K; a->Kp = up(d->K, kPad); a->C = d->C; a->ignore = d->ignore_index;
-  a->lse = d->lse; a->flag = d->flag; a->row_loss = d->row_loss; a->meta = d->meta;
+  a->lse = d->lse; a->flag = d->flag; a->meta = d->meta;
   return PG_OK;
 }
 
@@ -842,7 +841,7 @@ int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, i
   if (n == 0) return 0;
   const LxPlan p = lx_plan(n, K, C, dtype);
   const int64_t ops = p.h_bytes + p.w_bytes + p.side_bytes;
-  return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + up(4 * n, 256) + ops;
+  return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + 2 * up(4 * n, 256) + ops;
 }
 
 int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
@@ -850,16 +849,22 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   int rc = lx_args(d, &a);
   if (rc != PG_OK) return rc;
   hipStream_t st = as_stream(stream);
+  if (d->reduction < PG_XENT_MEAN || d->reduction > PG_XENT_NONE) return PG_ERR_INVALID;
+  const bool rows = d->reduction == PG_XENT_NONE;
+  if (rows ? a.n > 0 && !d->row_loss : !d->loss) return PG_ERR_INVALID;
   if (a.n > 0) {
-    if (!d->row_loss) return PG_ERR_INVALID;
     const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype);
     char* s = (char*)d->scratch;
+    a.row_loss = rows ? d->row_loss : (float*)s;
+    s += up(4 * a.n, 256);
     rc = d->dtype == PG_DTYPE_F32 ? lx_forward<float>(a, d, p, s, st) : d->dtype == PG_DTYPE_BF16 ? lx_forward<bf16_t>(a, d, p, s, st)
                                                                                                   : lx_forward<f16_t>(a, d, p, s, st);
     if (rc != PG_OK) return rc;
   }
-  hipLaunchKernelGGL(k_lx_mean, dim3(1), dim3(1024), 0, st, a.row_loss, a.flag, a.n, a.meta);
-  PG_LAUNCH_CHECK();
+  if (!rows) {
+    hipLaunchKernelGGL(k_lx_mean, dim3(1), dim3(1024), 0, st, a.row_loss, a.flag, a.n, d->reduction == PG_XENT_MEAN ? 1 : 0, d->loss, a.meta);
+    PG_LAUNCH_CHECK();
+  }
   return PG_OK;
 }
 
@@ -883,7 +888,7 @@ int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   } else {
     a.rowf = a.flag;
     a.f1 = d->grad;
-    a.f2 = d->reduction == PG_XENT_MEAN ? a.meta + 1 : nullptr;
+    a.f2 = d->reduction == PG_XENT_MEAN ? a.meta : nullptr;
   }
   s += up(4 * a.n, 256) + 256;
   return d->dtype == PG_DTYPE_F32 ? lx_backward<float>(a, d, p, s, st) : d->dtype == PG_DTYPE_BF16 ? lx_backward<bf16_t>(a, d, p, s, st)

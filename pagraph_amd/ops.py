@@ -860,7 +860,7 @@ def gcn_head(indptr, src, h, linear, labels, n_valid, grad_seed=None, ignore_ind
 # A call costs the host more than most of these kernels cost the card, and a backward pass runs on autograd's own thread, with
 # every Python object it touches in another core's cache: what stands between the arguments and the launch is kept short
 # (descriptors packed in one go — the layout is pg_norm_desc_t's and pg_linear_xent_desc_t's —, no device switch where none is due).
-_NORM_DESC, _XENT_DESC, _DROP_DESC = struct.Struct("16Q10qiifiIIQQQ").pack, struct.Struct("13Q7qii").pack, struct.Struct("IIQQQ").pack
+_NORM_DESC, _XENT_DESC, _DROP_DESC = struct.Struct("16Q10qiifiIIQQQ").pack, struct.Struct("14Q7qii").pack, struct.Struct("IIQQQ").pack
 _NO_DROP = (0, 0, 0, 0, 0)
 _DTYPES = {torch.float32: L.PG_DTYPE_F32, torch.bfloat16: L.PG_DTYPE_BF16, torch.float16: L.PG_DTYPE_F16}
 
@@ -983,46 +983,44 @@ class _LayerNorm(torch.autograd.Function):
             rows.data_ptr(), _addr(res), _addr(weight), _addr(bias), _addr(total), y.data_ptr(), at, at + 4 * n if at else 0,
             0, 0, 0, 0, 0, 0, 0, at + 8 * n if at else 0, n, d, _row_stride(rows), _row_stride(res) if res is not None else 0, d, d, 0, 0, 0, 0,
             dt, _DTYPES[param.dtype] if param is not None else dt, eps, spec is not None, *(_drop_fields(spec) if spec is not None else _NO_DROP)))
-        ctx.eps, ctx.spec = eps, spec
+        # (what the backward pass can do without looking at a tensor on its own thread it is given here)
+        ctx.eps, ctx.spec, ctx.stats, ctx.param = eps, spec, stats, param.dtype if param is not None else t
+        ctx.scratch = L.load().pg_layer_norm_scratch(n, d, dt) if grad[1] or grad[2] else 0
         ctx.set_materialize_grads(False)
         y = _like(y, x.shape)
         if res is None:
-            ctx.save_for_backward(x, weight, bias, stats)
+            ctx.save_for_backward(x, weight)
             return y
         total = _like(total, x.shape)
-        ctx.save_for_backward(total, weight, bias, stats)
+        ctx.save_for_backward(total, weight)
         return y, total
 
     @staticmethod
     def backward(ctx, gy, gsum=None):
         _once("layer_norm")
-        s, weight, bias, stats = ctx.saved_tensors
+        s, weight = ctx.saved_tensors
         need_x, need_w, need_b, need_res = ctx.needs_input_grad[:4]
         spec = ctx.spec
         if gy is None:
             if gsum is None:
-                return (None,) * 6
+                return None, None, None, None, None, None
             gy = torch.zeros((), dtype=s.dtype, device=s.device).expand(s.shape)      # only the sum was used
         rows, g = _rows_of(s), _rows_of(gy)
         gs = _rows_of(gsum) if gsum is not None else None
         n, d = rows.shape
-        dev, t, dt = s.device, s.dtype, _DTYPES[s.dtype]
-        need_w, need_b = need_w and weight is not None, need_b and bias is not None
+        dev, t, param = s.device, s.dtype, ctx.param
+        dt = _DTYPES[t]
         dx = torch.empty((n, d), dtype=t, device=dev) if need_x or (need_res and spec is None) else None
         # one gradient for both summands, as of a sum, unless a mask stands before one of them
         dres = torch.empty((n, d), dtype=t, device=dev) if need_res and spec is not None else None
-        param = weight if weight is not None else bias
-        dw = torch.empty(d, dtype=weight.dtype, device=dev) if need_w else None
-        db = torch.empty(d, dtype=bias.dtype, device=dev) if need_b else None
-        part = None
-        if need_w or need_b:
-            part = torch.empty(L.load().pg_layer_norm_scratch(n, d, dt), dtype=torch.float32, device=dev)
-        at = stats.data_ptr()
+        dw = torch.empty(d, dtype=param, device=dev) if need_w else None
+        db = torch.empty(d, dtype=param, device=dev) if need_b else None
+        part = torch.empty(ctx.scratch, dtype=torch.float32, device=dev) if need_w or need_b else None
+        at = ctx.stats.data_ptr()
         _enqueue("pg_layer_norm_bwd", dev, _NORM_DESC(
-            0, 0, _addr(weight), _addr(bias), rows.data_ptr(), 0, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
+            0, 0, _addr(weight), 0, rows.data_ptr(), 0, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
             _addr(dw), _addr(db), _addr(part), 0, n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
-            dt, _DTYPES[param.dtype] if param is not None else dt, ctx.eps, spec is not None,
-            *(_drop_fields(spec, at + 8 * n) if spec is not None else _NO_DROP)))
+            dt, _DTYPES[param], ctx.eps, spec is not None, *(_drop_fields(spec, at + 8 * n) if spec is not None else _NO_DROP)))
         if need_res:
             dres = _like(dx if spec is None else dres, s.shape)
         return (_like(dx, s.shape) if need_x else None, dw, db, dres, None, None)
@@ -1067,25 +1065,27 @@ class _LinearCrossEntropy(torch.autograd.Function):
         weight, labels = _table(weight), labels.reshape(-1).contiguous()
         n, K, C = rows.size(0), rows.size(1), weight.size(0)
         dev, t = h.device, _DTYPES[h.dtype]
-        stats = torch.empty(3 * n + 4, dtype=torch.float32, device=dev)           # lse | counted? | row losses | meta
+        each = reduction == L.PG_XENT_NONE
+        loss = torch.empty(h.shape[:-1] if each else (), dtype=torch.float32, device=dev)
+        stats = torch.empty(2 * n + 1, dtype=torch.float32, device=dev)           # lse | counted? | 1 / #counted
         size = L.load().pg_linear_xent_scratch(n, K, C, t, 0)
         if size < 0:
             raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-        at = stats.data_ptr()
+        at, out = stats.data_ptr(), loss.data_ptr()
         _enqueue("pg_linear_xent_fwd", dev, _XENT_DESC(
-            rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
-            0, 0, 0, 0, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
-        ctx.save_for_backward(h, weight, bias, labels, stats)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        if reduction == L.PG_XENT_NONE:
-            return _like(stats[2 * n:3 * n], h.shape[:-1])
-        return stats[3 * n + (0 if reduction == L.PG_XENT_MEAN else 2)]
+            rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, out if each else 0, 0 if each else out,
+            at + 8 * n, 0, 0, 0, 0, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
+        ctx.save_for_backward(h, weight, bias, labels)
+        ctx.stats, ctx.ignore_index, ctx.reduction = stats, ignore_index, reduction
+        grad = ctx.needs_input_grad
+        ctx.scratch = L.load().pg_linear_xent_scratch(n, K, C, t, 1) if grad[0] or grad[1] or grad[2] else 0
+        return loss
 
     @staticmethod
     def backward(ctx, g):
         _once("linear_cross_entropy")
-        h, weight, bias, labels, stats = ctx.saved_tensors
+        h, weight, bias, labels = ctx.saved_tensors
         need_h, need_w, need_b = ctx.needs_input_grad[:3]
         rows = _rows_of(h)
         n, K, C = rows.size(0), rows.size(1), weight.size(0)
@@ -1096,10 +1096,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         db = new((C,), dtype=h.dtype, device=dev) if need_b and bias is not None else None
         if n > 0:
             g = g.reshape(-1)                        # fp32, as the loss is
-            scratch = torch.empty(L.load().pg_linear_xent_scratch(n, K, C, t, 1), dtype=torch.uint8, device=dev)
-            at = stats.data_ptr()
+            scratch = torch.empty(ctx.scratch, dtype=torch.uint8, device=dev)
+            at = ctx.stats.data_ptr()
             _enqueue("pg_linear_xent_bwd", dev, _XENT_DESC(
-                rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, at + 8 * n, at + 12 * n,
+                rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, 0, 0, at + 8 * n,
                 g.data_ptr(), _addr(dh), _addr(dw), _addr(db), scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight),
                 g.stride(0), ctx.ignore_index, t, ctx.reduction))
         return _like(dh, h.shape) if need_h else None, dw, db, None, None, None

@@ -118,7 +118,7 @@ def test_descriptors_match_the_header(tmp_path):
     ptrs, sizes = tuple(range(10, 26)), tuple(range(-5, 5))
     assert ops._DROP_DESC(*drop) == bytes(_lib.PgDropout(*drop))
     assert ops._NORM_DESC(*ptrs, *sizes, 1, 2, 0.5, True, *drop) == bytes(_lib.PgNormDesc(*ptrs, *sizes, 1, 2, 0.5, 1, _lib.PgDropout(*drop)))
-    assert ops._XENT_DESC(*ptrs[:13], *sizes[:7], 1, 2) == bytes(_lib.PgLinearXentDesc(*ptrs[:13], *sizes[:7], 1, 2))
+    assert ops._XENT_DESC(*ptrs[:14], *sizes[:7], 1, 2) == bytes(_lib.PgLinearXentDesc(*ptrs[:14], *sizes[:7], 1, 2))
 
 
 # ---- dropout ---------------------------------------------------------------------------------------------------------------
@@ -605,6 +605,35 @@ def test_linear_cross_entropy_layouts_and_parts(dev, hiplib):
             assert torch.equal(one, want[which])
             for q in leaf:
                 q.requires_grad_(True)
+
+
+@gpu
+def test_outputs_are_the_callers(dev, hiplib):
+    """outputs may be changed in place; inputs that a gradient needs may not (autograd says so); a second pass over a kept graph is
+    the first; a gradient's own graph is refused"""
+    from pagraph_amd import _lib, ops
+    g = gen(14, dev)
+    lin, norm, spec = head(dev, 24, 90, F32, g), torch.nn.LayerNorm(24, device=dev), spec_of(dev, 0.5)
+    lab = torch.randint(0, 90, (40,), generator=g, device=dev)
+    for f in (lambda x: ops.linear_cross_entropy(x, lin, lab), lambda x: ops.linear_cross_entropy(x, lin, lab, reduction="none"),
+              lambda x: ops.layer_norm(x, norm), lambda x: ops.dropout(x, spec), lambda x: ops.layer_norm(x, norm, residual=x, dropout=spec)[0]):
+        x = torch.randn(40, 24, generator=g, device=dev, requires_grad=True)
+        y = f(x)
+        a = torch.autograd.grad(y.sum(), x, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y.sum(), x, retain_graph=True)[0], a)
+        with pytest.raises(_lib.PgError):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+        z = f(x)
+        z.mul_(2.0)
+        assert torch.equal(torch.autograd.grad(z.sum(), x)[0], torch.autograd.grad((2.0 * f(x)).sum(), x)[0])
+    loss = ops.linear_cross_entropy(x, lin, lab)
+    lab.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    y, s = ops.layer_norm(x, norm, residual=x)
+    s.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
 
 
 @gpu
