@@ -2,6 +2,7 @@
 import ctypes
 import os
 import struct
+import weakref
 
 import torch
 
@@ -923,6 +924,30 @@ def _once(name):
         raise L.PgError(f"{name}: a gradient's own graph (create_graph=True) is not supported")
 
 
+# graphs of these operators that were recorded outside a capture and still live: their leaves' gradient accumulators belong to the
+# stream they were recorded on. A backward pass captured on another stream would make autograd wait across the capture's border,
+# which ends the process; the forward inside the capture is refused instead.
+_EAGER_GRAPHS = weakref.WeakSet()
+
+
+def _capture_state(device):
+    return torch._C._cuda_isCurrentStreamCapturing(), torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _watch_graph(name, ctx, device, *inputs):
+    capturing, ctx.stream = _capture_state(device)
+    if not capturing:
+        _EAGER_GRAPHS.add(ctx)
+        return
+    for other in list(_EAGER_GRAPHS):
+        if other.stream != ctx.stream:
+            for fn, _ in other.next_functions:
+                leaf = getattr(fn, "variable", None)
+                if leaf is not None and any(leaf is t for t in inputs):
+                    raise L.PgError(f"{name}: this capture's gradients would meet those of a graph that was recorded on another stream "
+                                    "and is still alive (a loss kept from an eager step?): drop it before the capture")
+
+
 def _drop_fields(spec, step_used=0):
     """pg_dropout_t of a mask; for a gradient the step is the one the forward's launch noted, not what the counter holds by now"""
     step = spec.step
@@ -939,6 +964,8 @@ class _Dropout(torch.autograd.Function):
         _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), y.data_ptr(), d, n, d, _DTYPES[t],
                  _DROP_DESC(*_drop_fields(spec)), _addr(used))
         ctx.spec, ctx.used = spec, used
+        if ctx.needs_input_grad[0]:
+            _watch_graph("dropout", ctx, dev, x)
         return _like(y, x.shape)
 
     @staticmethod
@@ -987,6 +1014,8 @@ class _LayerNorm(torch.autograd.Function):
         ctx.eps, ctx.spec, ctx.stats, ctx.param = eps, spec, stats, param.dtype if param is not None else t
         ctx.scratch = L.load().pg_layer_norm_scratch(n, d, dt) if grad[1] or grad[2] else 0
         ctx.set_materialize_grads(False)
+        if stats is not None:
+            _watch_graph("layer_norm", ctx, dev, x, weight, bias, residual)
         y = _like(y, x.shape)
         if res is None:
             ctx.save_for_backward(x, weight)
@@ -1079,7 +1108,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.save_for_backward(h, weight, bias, labels)
         ctx.stats, ctx.ignore_index, ctx.reduction = stats, ignore_index, reduction
         grad = ctx.needs_input_grad
-        ctx.scratch = L.load().pg_linear_xent_scratch(n, K, C, t, 1) if grad[0] or grad[1] or grad[2] else 0
+        if grad[0] or grad[1] or grad[2]:
+            ctx.scratch = L.load().pg_linear_xent_scratch(n, K, C, t, 1)
+            _watch_graph("linear_cross_entropy", ctx, dev, h, weight, bias)
         return loss
 
     @staticmethod

@@ -121,6 +121,36 @@ def test_descriptors_match_the_header(tmp_path):
     assert ops._XENT_DESC(*ptrs[:14], *sizes[:7], 1, 2) == bytes(_lib.PgLinearXentDesc(*ptrs[:14], *sizes[:7], 1, 2))
 
 
+def test_a_capture_meets_no_living_eager_graph(monkeypatch):
+    """the rule of ops._watch_graph, with the streams made up"""
+    from pagraph_amd import _lib, ops
+    state = {"capturing": False, "stream": 1}
+    monkeypatch.setattr(ops, "_capture_state", lambda device: (state["capturing"], state["stream"]))
+    monkeypatch.setattr(ops, "_EAGER_GRAPHS", type(ops._EAGER_GRAPHS)())
+
+    class F(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            ops._watch_graph("f", ctx, x.device, x, w)
+            return x * w
+
+        @staticmethod
+        def backward(ctx, g):
+            return g, g
+    x, w, v = (torch.ones(3, requires_grad=True) for _ in range(3))
+    kept = F.apply(x, w)
+    assert len(ops._EAGER_GRAPHS) == 1
+    state.update(capturing=True)
+    F.apply(x, w)                                   # the stream the graph was recorded on: autograd has nothing to wait for
+    state.update(stream=2)
+    F.apply(v, v)                                   # other leaves
+    with pytest.raises(_lib.PgError, match="still alive"):
+        F.apply(v, w)
+    del kept
+    assert len(ops._EAGER_GRAPHS) == 0
+    F.apply(x, w)
+
+
 # ---- dropout ---------------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("t", [F32, BF16, F16])
@@ -752,6 +782,33 @@ def test_tail_captured_and_replayed(dev, hiplib):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+@gpu
+def test_capture_is_refused_while_an_eager_graph_lives(dev, hiplib):
+    from pagraph_amd import _lib, ops
+    g = gen(55, dev)
+    lin, x = head(dev, 32, 200, F32, g), torch.randn(50, 32, generator=g, device=dev)
+    lab = torch.randint(0, 200, (50,), generator=g, device=dev)
+
+    def step():
+        loss = ops.linear_cross_entropy(x, lin, lab)
+        return [loss.detach()] + list(torch.autograd.grad(loss, [lin.weight, lin.bias]))
+    want = step()
+    kept = ops.linear_cross_entropy(x, lin, lab)
+    with pytest.raises(_lib.PgError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    torch.cuda.synchronize()
+    del kept
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        step()
 
 
 @gpu
