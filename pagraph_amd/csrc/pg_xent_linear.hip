@@ -10,7 +10,7 @@
 // whole tiles: 16-bit rows that are so already are used in place, others are packed first (k_lx_pack). fp32 values are split
 // into three bf16 parts (x = x0 + x1 + x2 to 24 bits) and six of the nine partial products are summed; what is left out is below
 // 2^-24 of the product — 2.5 PF / 6 where the fp32 matrix instructions reach 0.157 PF.
-// G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-9, fp16 2^-12 relative),
+// G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-8, fp16 2^-11 relative),
 // independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
 // of 2^-28 is still a normal number.
 #include "pg_xent_narrow.h"
@@ -520,7 +520,7 @@ inline void narrow_split(int64_t t, int64_t y_tiles, int32_t* splits, int64_t* r
   *splits = (int32_t)ceil_div<int64_t>(y_tiles, r);
 }
 
-inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
+inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backward) {
   LxPlan p{};
   const int64_t np = dtype == PG_DTYPE_F32 ? 3 : 1;
   p.Kp = up(K, kPad);
@@ -531,7 +531,10 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   p.classes_p = up(C, 256) + 64;
   p.rows_p = p.h_rows + 64;
   p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
-  p.narrow = p.Kp <= (np == 3 ? 128 : 256);
+  // (us, narrow against wide. fp32 6000 -> 50000: 64 columns forward 223, 343, with gradients 1109, 2645; 128: 424, 501 and 1963,
+  // 3464. bf16 8192 -> 65536: 128 columns 188, 264 and 775, 1408; 192: 239, 325 and 1001, 1712; 256: forward 269, 390, but the
+  // gradients alone 1652, 1478, since 256 columns of operands and sums do not fit the registers of a wave)
+  p.narrow = p.Kp <= (np == 3 ? 128 : backward ? 192 : 256);
   if (p.narrow) {
     p.xt_stats = 128 * narrow_xb((int)np, (int)p.Kp, NX_STATS);
     p.xt_grad = 128 * narrow_xb((int)np, (int)p.Kp, NX_DH);
@@ -546,15 +549,16 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype) {
     return p;
   }
   // 256 x 256 tiles need a quarter less LDS traffic and two thirds of the loads of 128 x 128 ones, and fill the card from 256 tiles
-  // on: at half of that 128 x 128 ones, two to a CU, are ahead (fp16 777 x 602 -> 1153, 20 against 70 tiles: logits 22 -> XX us)
+  // on: at half of that 128 x 128 ones, two to a CU, are ahead (fp16 777 x 602 -> 1153, 20 against 70 tiles: logits 22 -> 12.5 us)
   p.big = ceil_div<int64_t>(n, 256) * ceil_div<int64_t>(C, 256) >= 192;
   const int64_t bm = p.big ? 256 : 128;
   p.tiles = ceil_div<int64_t>(C, bm);
   p.row_tiles = ceil_div<int64_t>(n, bm);
   p.part_bytes = up(n * p.tiles * 8, 256);
-  // a piece of G
+  // a piece of G: half a GB (128 MB, 256 MB, half a GB: 4690, 4363, 4280 us at bf16 8192 x 1024 -> 65536, 3005, 2847, 2680 at fp16
+  // 16384 x 512 -> 32768: fewer launches with a ragged end each, and fewer passes over dh's running sum)
   p.g_rows = up(n, 256);
-  int64_t cols = (int64_t(256) << 20) / (np * 2 * p.g_rows) / 256 * 256;
+  int64_t cols = (int64_t(512) << 20) / (np * 2 * p.g_rows) / 256 * 256;
   if (cols < 256) cols = 256;
   if (cols > (1 << 18)) cols = 1 << 18;
   p.pieces = (int32_t)ceil_div<int64_t>(C, cols);
@@ -606,7 +610,7 @@ int lx_operands(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   }
   if (!h.dst && !w.dst && !side.bias2) return PG_OK;
   const int64_t most = (w.dst && (!h.dst || p.w_rows > p.h_rows) ? p.w_rows : h.dst ? p.h_rows : 32) * (p.Kp / 8);
-  const int64_t blocks = ceil_div<int64_t>(most, 256);
+  const int64_t sides = p.classes_p > p.rows_p ? p.classes_p : p.rows_p, blocks = ceil_div<int64_t>(most > sides ? most : sides, 256);
   if (!h.dst) { h = w; w = PackArgs{}; }
   hipLaunchKernelGGL(k_lx_pack<T>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks), side.bias2 ? 3 : w.dst ? 2 : 1), dim3(256), 0, st, h, w, side);
   PG_LAUNCH_CHECK();
@@ -625,7 +629,8 @@ int launch_narrow(const NxArgs& n, const LxPlan& p, hipStream_t st) {
   if (p.Kp == 64) return launch_narrow_kp<T, 64, MODE>(n, st);
   if constexpr (Mul<T>::NP == 1) {
     if (p.Kp == 192) return launch_narrow_kp<T, 192, MODE>(n, st);
-    if (p.Kp == 256) return launch_narrow_kp<T, 256, MODE>(n, st);
+    if constexpr (MODE == NX_STATS)
+      if (p.Kp == 256) return launch_narrow_kp<T, 256, MODE>(n, st);
   }
   return launch_narrow_kp<T, 128, MODE>(n, st);
 }
@@ -770,7 +775,7 @@ int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipSt
     const int rc = p.dw_cols == 256 ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw_cols == 128 ? lx_launch_dw<T, MidTile<T>>(a, st)
                                                                                             : lx_launch_dw<T, SlimTile<T>>(a, st);
     if (rc != PG_OK) return rc;
-    if (a.splits > 1)
+    if (a.splits > 1 && p.pieces > 1)
       return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, (a.c_hi - a.c_lo) * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
   }
   return PG_OK;
@@ -806,7 +811,8 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
     if (rc != PG_OK) return rc;
   }
   const bool direct = p.dh_splits == 1 && p.pieces == 1;
-  return lx_sums<T>(SumArgs{acc_dh, direct ? nullptr : a.dh, a.n * a.K, p.dh_splits}, SumArgs{a.dbp, a.db, a.C, p.row_tiles}, SumArgs{}, a, st);
+  return lx_sums<T>(SumArgs{acc_dh, direct ? nullptr : a.dh, a.n * a.K, p.dh_splits}, SumArgs{a.dbp, a.db, a.C, p.row_tiles},
+                    SumArgs{acc_dw, p.dw_splits > 1 && p.pieces == 1 ? a.dw : nullptr, a.C * a.K, p.dw_splits}, a, st);
 }
 
 // the grids are one-dimensional, and a tile's offsets have 32 bits
@@ -839,7 +845,7 @@ extern "C" {
 int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, int32_t backward) {
   if (lx_check(n, K, C, dtype) != PG_OK) return -1;
   if (n == 0) return 0;
-  const LxPlan p = lx_plan(n, K, C, dtype);
+  const LxPlan p = lx_plan(n, K, C, dtype, backward != 0);
   const int64_t ops = p.h_bytes + p.w_bytes + p.side_bytes;
   return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + 2 * up(4 * n, 256) + ops;
 }
@@ -853,7 +859,7 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   const bool rows = d->reduction == PG_XENT_NONE;
   if (rows ? a.n > 0 && !d->row_loss : !d->loss) return PG_ERR_INVALID;
   if (a.n > 0) {
-    const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype);
+    const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype, false);
     char* s = (char*)d->scratch;
     a.row_loss = rows ? d->row_loss : (float*)s;
     s += up(4 * a.n, 256);
@@ -875,7 +881,7 @@ int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   if (!d->grad || d->reduction < PG_XENT_MEAN || d->reduction > PG_XENT_NONE) return PG_ERR_INVALID;
   if (a.n == 0) return PG_ERR_INVALID;            // no row, no gradient to compute: the caller's zeros
   hipStream_t st = as_stream(stream);
-  const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype);
+  const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype, true);
   char* s = (char*)d->scratch;
   a.dh = d->dh; a.dw = d->dW; a.db = d->db;
   if (d->reduction == PG_XENT_NONE) {

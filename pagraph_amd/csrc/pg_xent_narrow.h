@@ -1,4 +1,5 @@
-// The class head's three passes for narrow rows (K <= 256 after padding): nothing of size [n, C] leaves the registers.
+// The class head's three passes for narrow rows (K padded to 64s: 16-bit rows up to 256, for gradients 192, fp32 rows up to 128):
+// nothing of size [n, C] leaves the registers.
 //
 // One kernel, three roles. A wave keeps 32 XB "x" rows in registers as matrix operands and walks the other side's rows "y", whose
 // tiles all four waves share in LDS:
@@ -10,7 +11,7 @@
 // read from the same LDS tile in the order the lanes hold (the transposing LDS reads pick any four consecutive y). No exchange
 // between lanes, no trip through LDS.
 // 10 n K C operations (2 + 4 + 4) and no G traffic, against 8 n K C and 6 bytes (fp32: 18) per element of [n, C] of the wide form:
-// below some 500 columns (16 bit) the traffic costs more than the repeated product.
+// as long as a wave's registers hold its operand rows and its sums, the traffic costs more than the repeated product.
 // Exponents are kept in base 2: z log2(e) + b log2(e) is one fused multiply-add, and fp16's scale of G, 2^14, rides in the exponent.
 #pragma once
 #include "pg_mm.h"
