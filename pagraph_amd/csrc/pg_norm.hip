@@ -55,6 +55,37 @@ __device__ __forceinline__ void store_piece(T* __restrict__ row, int c, int d, c
   }
 }
 
+// the same piece as it stands in memory: half the registers where a 16-bit row has to be kept, and no wait before its use
+template <typename T, int V>
+struct Raw {
+  uint32_t w[V * sizeof(T)];
+};
+template <typename T, int V, bool RAGGED>
+__device__ __forceinline__ void load_raw(const T* __restrict__ row, int c, int d, Raw<T, V>& raw) {
+  if (c + 4 * V <= d) {
+    __builtin_memcpy(&raw, row + c, sizeof(raw));
+  } else {
+    T t[4 * V];
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) t[i] = RAGGED && c + i < d ? row[c + i] : (T)0.f;
+    __builtin_memcpy(&raw, t, sizeof(raw));
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& raw, float (&v)[4 * V]) {
+  T t[4 * V];
+  __builtin_memcpy(t, &raw, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < 4 * V; ++i) v[i] = (float)t[i];
+}
+
+// the compiler forgets what it has unpacked, instead of keeping it in twice the registers
+template <typename T, int V>
+__device__ __forceinline__ void keep_packed(Raw<T, V>& raw) {
+#pragma unroll
+  for (uint32_t& w : raw.w) asm volatile("" : "+v"(w));
+}
+
 struct UnitMask {
   uint32_t w[4];
 };
@@ -142,6 +173,30 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& turn) 
   }
 }
 
+// which of the workgroup's rows a lane works on: one value a wave from 64 lanes a row on, so that row addresses are scalar
+template <int G>
+__device__ __forceinline__ int row_of_lane() {
+  const int r = threadIdx.x / G;
+  return G >= kWave ? __builtin_amdgcn_readfirstlane(r) : r;
+}
+// A row's number, and in the widest workgroups (128 registers a lane) a lane's, opaque: addresses are made from them where they are
+// used, from a scalar base and a 32-bit offset. The compiler would carry one pointer per operand and piece from row to row in
+// vector registers: forward of 16384 x 256 bf16 14.3 against 12.1 us, backward of 2048 x 16384 151 against 92. fp32 rows have
+// registers for it, or lose more to the order of the loads (6000 x 602 forward 12.7 against 14.9 us).
+template <typename T, int G>
+__device__ __forceinline__ int64_t fresh_row(int64_t r) {
+  if constexpr (sizeof(T) == 4) return r;
+  if constexpr (G >= kWave) asm volatile("" : "+s"(r));
+  else asm volatile("" : "+v"(r));
+  return r;
+}
+template <int G>
+__device__ __forceinline__ int fresh_lane() {
+  int l = threadIdx.x;
+  if constexpr (G == 1024) asm volatile("" : "+v"(l));
+  return l & (G - 1);
+}
+
 template <typename T, int V, bool RAGGED>
 __device__ __forceinline__ void load_param(const void* p, int f32, int c, int d, float fill, float (&v)[4 * V]) {
   if (p == nullptr) {
@@ -160,13 +215,14 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_fwd(NormArgs a) {
   constexpr int B = G > 256 ? G : 256, RPB = B / G, P = 4 * V;
   __shared__ float lds[G > kWave ? 4 * (B / kWave) : 1];
   int turn = 0;
-  const int lane = threadIdx.x % G, d = a.d;
+  const int own = row_of_lane<G>(), d = a.d;
   const float cols = (float)d;
   const uint32_t step = a.drop ? drop_step_of(a.dr) : 0u;
   if (a.drop && a.step_used && blockIdx.x == 0 && threadIdx.x == 0) *a.step_used = step;
   for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.n; rb += (int64_t)gridDim.x * RPB) {
-    const bool on = rb + threadIdx.x / G < a.n;
-    const int64_t r = on ? rb + threadIdx.x / G : a.n - 1;
+    const bool on = rb + own < a.n;
+    const int64_t r = fresh_row<T, G>(on ? rb + own : a.n - 1);
+    const int lane = fresh_lane<G>();
     const T* x = (const T*)a.x + r * a.xs;
     float v[2 * S][P];
 #pragma unroll
@@ -235,68 +291,123 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_fwd(NormArgs a) {
 }
 
 template <typename T, int V, bool RAGGED, int G, int S>
-__global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_bwd(NormArgs a) {
+__global__ __launch_bounds__(G > 256 ? G : 256, G < 1024 ? 3 : 4) void k_norm_bwd(NormArgs a) {
   constexpr int B = G > 256 ? G : 256, RPB = B / G, P = 4 * V;
   constexpr int COLS = RPB > 1 ? 2 * P * G * S : 1;             // the workgroup's sums of dw, db over its row groups
   __shared__ float lds[G > kWave ? 4 * (B / kWave) : 1];
   __shared__ float acc_lds[2 * COLS];
   int turn = 0;
-  const int lane = threadIdx.x % G, d = a.d;
+  const int own = row_of_lane<G>(), d = a.d;
   const float cols = (float)d;
   const uint32_t step = a.drop ? drop_step_of(a.dr) : 0u;
   float aw[2 * S][P] = {}, ab[2 * S][P] = {};
-  for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.n; rb += (int64_t)gridDim.x * RPB) {
-    const bool on = rb + threadIdx.x / G < a.n;
-    const int64_t r = on ? rb + threadIdx.x / G : a.n - 1;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    float xh[2 * S][P], gh[2 * S][P], ds[2 * S][P], sum[2] = {0.f, 0.f};
+  // a row is kept as it was read: xh and gh = gy * w are made from 16-bit pieces twice, fp32 pieces give way to them (KEEP).
+  // AHEAD: the next row is read behind this one's stores, so that all its loads leave together; at the top of the loop the compiler
+  // moves some down to their use (16384 x 2048 bf16 94 against 68 us; fp32 2048 x 16384 143 against 163: no registers to spare).
+  // Reading it earlier, while this row's sums go round the group, takes the registers of a third workgroup on the CU: 73 us.
+  constexpr bool KEEP = sizeof(T) == 4, AHEAD = sizeof(T) == 2 && S == 1;
+  struct Row {
+    Raw<T, V> x[2 * S], g[2 * S], s[2 * S];
+    float mean, rstd;
+  };
+  auto read = [&](int64_t rb, Row& row) {
+    const int64_t at = rb + own, r = fresh_row<T, G>(at < a.n ? at : a.n - 1);
+    const int lane = fresh_lane<G>();
+    row.mean = a.mean[r];
+    row.rstd = a.rstd[r];
 #pragma unroll
     for (int k = 0; k < 2 * S; ++k) {
       const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
-      load_piece<T, V, RAGGED>((const T*)a.x + r * a.xs, c, d, xh[k]);
-      load_piece<T, V, RAGGED>((const T*)a.gy + r * a.gys, c, d, gh[k]);
-      if (a.gs) load_piece<T, V, RAGGED>((const T*)a.gs + r * a.gss, c, d, ds[k]);
+      load_raw<T, V, RAGGED>((const T*)a.x + r * a.xs, c, d, row.x[k]);
+      load_raw<T, V, RAGGED>((const T*)a.gy + r * a.gys, c, d, row.g[k]);
+      if (a.gs) load_raw<T, V, RAGGED>((const T*)a.gs + r * a.gss, c, d, row.s[k]);
     }
+  };
+  auto hats = [&](const Row& row, int k, int c, float (&xh)[P], float (&gy)[P]) {
+    unpack<T, V>(row.x[k], xh);
+    unpack<T, V>(row.g[k], gy);
+    // columns behind the row's end have gy = 0 and must not meet an infinite xh there
+#pragma unroll
+    for (int i = 0; i < P; ++i) xh[i] = (RAGGED ? c + i < d : c < d) ? (xh[i] - row.mean) * row.rstd : 0.f;
+  };
+  const int64_t stride = (int64_t)gridDim.x * RPB;
+  Row row;
+  if constexpr (AHEAD) read((int64_t)blockIdx.x * RPB, row);
+  for (int64_t rb = (int64_t)blockIdx.x * RPB; rb < a.n; rb += stride) {
+    const bool on = rb + own < a.n;
+    const int64_t r = fresh_row<T, G>(on ? rb + own : a.n - 1);
+    if constexpr (!AHEAD) read(rb, row);
+    float sum[2] = {0.f, 0.f};
+    int lane = fresh_lane<G>();
 #pragma unroll
     for (int k = 0; k < 2 * S; ++k) {
       const int c = unit_col<V>(lane + k / 2 * G) + 256 * (k & 1);
-      float w[P];
+      float xh[P], gh[P], w[P];
+      hats(row, k, c, xh, gh);
       load_param<T, V, RAGGED>(a.w, a.w_f32, c, d, 1.f, w);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        // columns behind the row's end have gy = 0 and must not meet an infinite xh there
-        xh[k][i] = (RAGGED ? c + i < d : c < d) ? (xh[k][i] - mean) * rstd : 0.f;
         if (on) {
-          ab[k][i] += gh[k][i];
-          aw[k][i] += gh[k][i] * xh[k][i];
+          ab[k][i] += gh[i];
+          aw[k][i] += gh[i] * xh[i];
         }
-        gh[k][i] *= w[i];
-        sum[0] += gh[k][i];
-        sum[1] += gh[k][i] * xh[k][i];
+        gh[i] *= w[i];
+        sum[0] += gh[i];
+        sum[1] += gh[i] * xh[i];
+      }
+      if constexpr (KEEP) {
+        __builtin_memcpy(&row.x[k], xh, sizeof(xh));
+        __builtin_memcpy(&row.g[k], gh, sizeof(gh));
+      } else {
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     group_sum<G, 2>(sum, lds, turn);
-    if (!on) continue;
-    const float s1 = sum[0] / cols, s2 = sum[1] / cols;
+    lane = fresh_lane<G>();
+    if constexpr (!KEEP) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      UnitMask m[V];
-      if (a.drop) draw_unit<V>(a.dr, step, (uint32_t)r, lane + s * G, m);
+      for (int k = 0; k < 2 * S; ++k) {
+        keep_packed<T, V>(row.x[k]);
+        keep_packed<T, V>(row.g[k]);
+      }
+    }
+    if (on) {
+      const float s1 = sum[0] / cols, s2 = sum[1] / cols;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = 2 * s + h, c = unit_col<V>(lane + s * G) + 256 * h;
-        if (c >= d) continue;
+      for (int s = 0; s < S; ++s) {
+        UnitMask m[V];
+        if (a.drop) draw_unit<V>(a.dr, step, (uint32_t)r, lane + s * G, m);
 #pragma unroll
-        for (int i = 0; i < P; ++i) ds[k][i] = rstd * (gh[k][i] - s1 - xh[k][i] * s2) + (a.gs ? ds[k][i] : 0.f);
-        if (a.dres) store_piece<T, V, RAGGED>((T*)a.dres + r * a.drs, c, d, ds[k]);
-        if (a.dx) {
-          if (a.drop) drop_piece<V>(ds[k], m, h, a.dr.thr, a.dr.scale);
-          store_piece<T, V, RAGGED>((T*)a.dx + r * a.dxs, c, d, ds[k]);
+        for (int h = 0; h < 2; ++h) {
+          const int k = 2 * s + h, c = unit_col<V>(lane + s * G) + 256 * h;
+          if (c >= d) continue;
+          float xh[P], gh[P], ds[P] = {};
+          if constexpr (KEEP) {
+            unpack<T, V>(row.x[k], xh);
+            unpack<T, V>(row.g[k], gh);
+          } else {
+            float w[P];
+            hats(row, k, c, xh, gh);
+            load_param<T, V, RAGGED>(a.w, a.w_f32, c, d, 1.f, w);
+#pragma unroll
+            for (int i = 0; i < P; ++i) gh[i] *= w[i];
+          }
+          if (a.gs) unpack<T, V>(row.s[k], ds);
+#pragma unroll
+          for (int i = 0; i < P; ++i) ds[i] += row.rstd * (gh[i] - s1 - xh[i] * s2);
+          if (a.dres) store_piece<T, V, RAGGED>((T*)a.dres + r * a.drs, c, d, ds);
+          if (a.dx) {
+            if (a.drop) drop_piece<V>(ds, m, h, a.dr.thr, a.dr.scale);
+            store_piece<T, V, RAGGED>((T*)a.dx + r * a.dxs, c, d, ds);
+          }
+          if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+    if (AHEAD && rb + stride < a.n) read(rb + stride, row);
   }
   if (!a.part) return;
+  const int lane = threadIdx.x % G;
   float* out = a.part + (int64_t)blockIdx.x * 2 * d;
   if constexpr (RPB > 1) {
     // lanes G apart in a wave hold the same columns: those first, then the waves (pairs of waves) one after the other
@@ -393,7 +504,7 @@ inline int norm_lanes(int64_t d, int v) {
 
 // workgroups of the backward pass: each leaves one partial row of 2 d floats, so each walks 8 rows at least, which keeps that
 // traffic to a tenth of the rows' own. At most the three a CU holds at once (registers): a second, partly filled round of them
-// took as long as the first (1024 workgroups 117 us, 768 89 us at 16384 x 2048 bf16 with dropout and residual)
+// took as long as the first (1024 workgroups 117 us, 768 89 us at 16384 x 2048 bf16 with dropout and residual, before rows were kept as read)
 inline int64_t norm_bwd_blocks(int64_t n, int64_t d, int32_t dtype) {
   const int g = norm_lanes(d, norm_v(d, dtype)), rpb = g >= 256 ? 1 : 256 / g;
   const int64_t rows = rpb > 8 ? rpb : 8, b = ceil_div<int64_t>(n, rows);
