@@ -353,21 +353,21 @@ __global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_
 }
 
 // incoming gradients of single rows: row factors g / max|g| (G then uses its type's range whatever the caller's scale), the
-// maximum becomes the outputs' factor
+// maximum becomes the outputs' factor. Of the finite ones: an infinite or NaN gradient stays that, in its own row
 __global__ __launch_bounds__(1024) void k_lx_row_factors(const float* __restrict__ g, int64_t gs, const float* __restrict__ flag,
                                                          int64_t n, float* __restrict__ rowf, float* __restrict__ top) {
   __shared__ float ss[1024];
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (flag[i] != 0.f) m = fmaxf(m, fabsf(g[i * gs]));
+    if (flag[i] != 0.f && fabsf(g[i * gs]) < INFINITY) m = fmaxf(m, fabsf(g[i * gs]));
   ss[threadIdx.x] = m;
   __syncthreads();
   for (int o = 512; o > 0; o >>= 1) {
     if ((int)threadIdx.x < o) ss[threadIdx.x] = fmaxf(ss[threadIdx.x], ss[threadIdx.x + o]);
     __syncthreads();
   }
-  m = ss[0];
-  for (int64_t i = threadIdx.x; i < n; i += 1024) rowf[i] = flag[i] != 0.f && m > 0.f ? g[i * gs] / m : 0.f;
+  m = ss[0] > 0.f ? ss[0] : 1.f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) rowf[i] = flag[i] != 0.f ? g[i * gs] / m : 0.f;
   if (threadIdx.x == 0) *top = m;
 }
 

@@ -668,6 +668,31 @@ def test_outputs_are_the_callers(dev, hiplib):
 
 
 @gpu
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("K", [40, 300])
+def test_linear_cross_entropy_gradients_that_are_not_finite(dev, hiplib, K, t):
+    """an infinite or NaN gradient of one row's loss stays with that row, and is not lost where it is the only one"""
+    from pagraph_amd import ops
+    g = gen(17, dev)
+    lin = head(dev, K, 700, t, g)
+    h = torch.randn(60, K, generator=g, device=dev).to(t).requires_grad_()
+    lab = torch.randint(0, 700, (60,), generator=g, device=dev)
+    up = torch.randn(60, generator=g, device=dev)
+    rest = torch.ones(60, dtype=torch.bool, device=dev)
+    rest[7], rest[33] = False, False
+    clean = torch.where(rest, up, torch.zeros_like(up))
+    want, = torch.autograd.grad(ops.linear_cross_entropy(h, lin, lab, reduction="none"), h, clean)
+    for a, b in ((float("nan"), float("inf")), (float("-inf"), float("inf"))):
+        dirty = up.clone()
+        dirty[7], dirty[33] = a, b
+        dh, dw = torch.autograd.grad(ops.linear_cross_entropy(h, lin, lab, reduction="none"), [h, lin.weight], dirty)
+        assert torch.equal(dh[rest], want[rest])
+        assert not torch.isfinite(dh[~rest]).any() and not torch.isfinite(dw).any()
+    dh, = torch.autograd.grad(ops.linear_cross_entropy(h, lin, lab, reduction="none"), h, torch.full_like(up, float("nan")))
+    assert torch.isnan(dh).all()
+
+
+@gpu
 def test_linear_cross_entropy_refusals(dev, hiplib):
     from pagraph_amd import _lib, ops
     h, lin = torch.randn(6, 16, device=dev), torch.nn.Linear(16, 100, device=dev)
