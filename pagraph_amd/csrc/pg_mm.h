@@ -1,9 +1,9 @@
 // Tiles of matrix products on the matrix cores (gfx950), for operands of 16-bit parts whose reduction range is padded to whole
 // multiples of 64: acc[BM x BN] += sum over parts and k of A(m, k) B(n, k), fp32 accumulation.
 //
-// Tiles of depth 32 travel from memory into LDS without passing through registers (16 bytes a lane), three tiles ahead of the one
-// being multiplied, four buffers, one barrier a step: a step of a 256 x 256 tile is about 1000 cycles of matrix work, a load that
-// misses the XCD's L2 takes two to three times that. An operand is stored either way round:
+// Tiles of depth 32 travel from memory into LDS without passing through registers (16 bytes a lane), into NB buffers, NB - 1 tiles
+// ahead of the one being multiplied, one barrier a step: a step of a 256 x 256 tile is about 1000 cycles of matrix work, a load
+// that misses the XCD's L2 takes two to three times that. An operand is stored either way round:
 //   ROWS: p[row][k], k contiguous     -> LDS tile [rows][32], fragments are plain 16-byte reads
 //   COLS: p[k][row], row contiguous   -> LDS tile [32][rows], fragments come from the transposing LDS reads (4 x 16 blocks)
 // so that no operand is ever transposed in memory. LDS-direct loads write 64 lanes x 16 bytes contiguously, so the bank swizzle is
@@ -29,7 +29,6 @@ __device__ __forceinline__ f32x16 mma(f16_t, s16x8 a, s16x8 b, f32x16 c) {
 enum { ROWS = 0, COLS = 1 };
 constexpr int kDepth = 32;                     // reduction depth of a tile
 constexpr int kPad = 64;                       // what rows of parts are padded to
-constexpr int kBuffers = 4;
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void glb_void;
@@ -114,17 +113,17 @@ __device__ __forceinline__ s16x8 fragment(const short* __restrict__ lds, int rb,
 }
 
 // Tile shape: BM x BN by WR x WC waves. NP parts per value: 1, or 3 (fp32 as three bf16 parts, six products, smallest first)
-template <typename E_, int NP_, int BM_, int BN_, int WR_, int WC_>
+template <typename E_, int NP_, int BM_, int BN_, int WR_, int WC_, int NB_>
 struct Shape {
   typedef E_ E;
-  static constexpr int NP = NP_, BM = BM_, BN = BN_, WR = WR_, WC = WC_, WAVES = WR * WC, THREADS = WAVES * 64;
+  static constexpr int NP = NP_, BM = BM_, BN = BN_, WR = WR_, WC = WC_, NB = NB_, WAVES = WR * WC, THREADS = WAVES * 64;
   static constexpr int FI = BM / WR / 32, FJ = BN / WC / 32;    // 32 x 32 blocks of a wave
   static constexpr int TILE = (BM + BN) * kDepth;               // elements of one buffer
 };
 
-// LDS of a kernel: ONE array of kBuffers tile buffers and `extra` shorts behind them (several variables would carry alias
+// LDS of a kernel: ONE array of NB tile buffers and `extra` shorts behind them (several variables would carry alias
 // information of their own, see fragment)
-#define PG_MM_LDS(S, name, extra) __shared__ __align__(16) short name[kBuffers * S::TILE + (extra)]
+#define PG_MM_LDS(S, name, extra) __shared__ __align__(16) short name[S::NB * S::TILE + (extra)]
 
 template <int VM>
 __device__ __forceinline__ void wait_loads() {          // at most VM loads of this wave still under way
@@ -170,14 +169,12 @@ struct Product {
 #pragma unroll
       for (int j = 0; j < S::FJ; ++j) acc[i][j] = mma(typename S::E(), f.a[i], f.b[j], acc[i][j]);
   }
-  // One step. f: the tile's fragments of depth 0, read a step ago; leaves with the next tile's. Reads run behind the matrix
-  // instructions of the half tile before. The caller has waited for this wave's loads of the NEXT tile.
+  // One step. f: the tile's fragments of depth 0, read half a step ago; leaves with the next tile's (LAST: there is none). Reads run
+  // behind the matrix instructions of the half tile before. At the barrier every wave's loads of the next tile have landed (full:
+  // those of the NB - 2 tiles behind it may still be under way) and every wave has its second half of this tile in registers: its
+  // buffer is the one that is filled again, with the tile NB further on.
   template <bool LAST>
-  __device__ __forceinline__ void step(const short* cur, const short* next, short* refill, bool more, Fragments& f, f32x16 (&acc)[S::FI][S::FJ]) {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();              // every wave's loads of the next tile have landed, all are done with the buffer to refill
-    asm volatile("" ::: "memory");
-    if (more) issue(refill);
+  __device__ __forceinline__ void step(short* cur, const short* next, bool full, bool more, Fragments& f, f32x16 (&acc)[S::FI][S::FJ]) {
     // in this order, whatever the scheduler thinks of the registers; the reads waited for were issued half a tile ago
     Fragments g;
     wait_reads();
@@ -186,7 +183,13 @@ struct Product {
     multiply(f, acc);
     __builtin_amdgcn_sched_barrier(0);
     wait_reads();
-    if (!LAST) read(next, 0, f);
+    if constexpr (!LAST) {
+      if (full) wait_loads<(S::NB - 2) * LOADS>(); else wait_loads<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read(next, 0, f);
+      if (more) issue(cur);
+    }
     __builtin_amdgcn_sched_barrier(0);
     multiply(g, acc);
     __builtin_amdgcn_sched_barrier(0);
@@ -194,47 +197,30 @@ struct Product {
 };
 
 template <typename S, int KA, int KB>
-__device__ __forceinline__ void mm_run(Product<S, KA, KB>& p, int steps, short* b0, short* b1, short* b2, short* b3, f32x16 (&acc)[S::FI][S::FJ]) {
+__device__ __forceinline__ void mm_run(Product<S, KA, KB>& p, int steps, short* buf, f32x16 (&acc)[S::FI][S::FJ]) {
   // steps is even: reduction ranges are multiples of kPad
-  constexpr int N = Product<S, KA, KB>::LOADS;
+  constexpr int N = Product<S, KA, KB>::LOADS, NB = S::NB;
   static_assert(kDepth == 32, "two fragments a tile");
   typename Product<S, KA, KB>::Fragments f;
-  p.issue(b0);
-  p.issue(b1);
-  if (steps > 2) p.issue(b2);
-  if (steps > 2) wait_loads<2 * N>(); else wait_loads<N>();
-  asm volatile("" ::: "memory");
+  const int first = steps < NB ? steps : NB;
+  for (int i = 0; i < first; ++i) p.issue(buf + i * S::TILE);
+  if (first == NB) wait_loads<(NB - 1) * N>(); else wait_loads<N>();          // (two or more tiles)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  p.read(b0, 0, f);
+  p.read(buf, 0, f);
   int left = steps;
-  for (; left >= 8; left -= 4) {
-    wait_loads<N>();
-    p.template step<false>(b0, b1, b3, true, f, acc);
-    wait_loads<N>();
-    p.template step<false>(b1, b2, b0, true, f, acc);
-    wait_loads<N>();
-    p.template step<false>(b2, b3, b1, true, f, acc);
-    wait_loads<N>();
-    p.template step<false>(b3, b0, b2, true, f, acc);
+  for (; left >= 2 * NB; left -= NB) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) p.template step<false>(buf + i * S::TILE, buf + (i + 1) % NB * S::TILE, true, true, f, acc);
   }
-  if (left >= 4) {                             // four or six
-    const bool six = left == 6;
-    wait_loads<N>();
-    p.template step<false>(b0, b1, b3, true, f, acc);
-    wait_loads<N>();
-    p.template step<false>(b1, b2, b0, six, f, acc);
-    if (six) wait_loads<N>(); else wait_loads<0>();
-    p.template step<false>(b2, b3, b1, six, f, acc);
-    if (six) wait_loads<N>(); else wait_loads<0>();
-    p.template step<false>(b3, b0, b2, false, f, acc);         // (four: reads a buffer that no load has filled anew; not used)
-    left -= 4;
+  int at = 0;
+#pragma unroll 1
+  for (; left > 1; --left) {
+    const int next = at + 1 == NB ? 0 : at + 1;
+    p.template step<false>(buf + at * S::TILE, buf + next * S::TILE, left >= NB, left > NB, f, acc);
+    at = next;
   }
-  if (left == 2) {
-    wait_loads<0>();
-    p.template step<false>(b0, b1, b3, false, f, acc);
-    p.template step<true>(b1, b2, b0, false, f, acc);
-  }
+  p.template step<true>(buf + at * S::TILE, buf, false, false, f, acc);
 }
 
 // acc += the product over [k_lo, k_hi), whole tiles. On return every wave may still be reading the buffers (synchronise before
@@ -252,7 +238,7 @@ __device__ __forceinline__ void mm_product(const Operand& oa, const Operand& ob,
   p.start();
   const int steps = (S::NP == 3 ? 6 : 1) * p.seg_steps;
   if (steps <= 0) return;
-  mm_run<S, KA, KB>(p, steps, buf, buf + S::TILE, buf + 2 * S::TILE, buf + 3 * S::TILE, acc);
+  mm_run<S, KA, KB>(p, steps, buf, acc);
 }
 
 // Workgroups go round the 8 XCDs in turn: give each XCD a contiguous run of tiles, so that its own L2 sees a tile's neighbours

@@ -149,12 +149,12 @@ __global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1, SideA
 // class = 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4 of its wave's classes, so a row's maximum and sum are taken in registers.
 // PIECE: writes G (through LDS: whole 16-byte pieces of rows) and the column sums of the tile, else the tile's row statistics.
 template <typename T, typename S, bool PIECE>
-__global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
+__global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
   typedef typename S::E E;
   constexpr int BM = S::BM, BN = S::BN, WM = BM / S::WR, WN = BN / S::WC;
   // behind the tile buffers: the tile's biases (base 2, -inf beyond the last class: their exponentials are 0), the waves' statistics
   PG_MM_LDS(S, buf, 2 * BM + (PIECE ? 0 : 4 * S::WR * BN));
-  float* bias = reinterpret_cast<float*>(buf + kBuffers * S::TILE);
+  float* bias = reinterpret_cast<float*>(buf + S::NB * S::TILE);
   float2(*red)[BN] = reinterpret_cast<float2(*)[BN]>(bias + BM);
   const uint32_t row_tiles = (uint32_t)ceil_div<int64_t>(a.n, BN), c_tiles = (uint32_t)ceil_div<int64_t>(a.c_hi - a.c_lo, BM);
   // an XCD's 32 CUs work on 8 row tiles x 4 class tiles at a time
@@ -248,8 +248,8 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_logits(LxArgs a) {
     }
     // [BN rows][BM classes] of one part in the tile buffers, 16-byte chunks swizzled by the row
     constexpr int CH = BM / 8, RP = S::THREADS / CH;
-    static_assert(BM * BN <= kBuffers * S::TILE, "a part of G fits the tile buffers");
-    static_assert(RP * BM * 2 <= kBuffers * S::TILE, "and so do its column sums");
+    static_assert(BM * BN <= S::NB * S::TILE, "a part of G fits the tile buffers");
+    static_assert(RP * BM * 2 <= S::NB * S::TILE, "and so do its column sums");
     float sum[8] = {};
 #pragma unroll 1
     for (int part = 0; part < S::NP; ++part) {
@@ -389,7 +389,7 @@ __device__ __forceinline__ void each_output(const f32x16 (&acc)[S::FI][S::FJ], i
 
 // dh: acc[split][r][k] (+)= sum over the split's classes of G[r][c] W[c][k]
 template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS) void k_lx_dh(LxArgs a) {
+__global__ __launch_bounds__(S::THREADS, 2) void k_lx_dh(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
   PG_MM_LDS(S, buf, 0);
   const uint32_t row_tiles = (uint32_t)ceil_div<int64_t>(a.n, S::BM), k_tiles = (uint32_t)ceil_div<int64_t>(a.K, S::BN);
@@ -465,7 +465,7 @@ int lx_sums(const SumArgs& a, const SumArgs& b, const SumArgs& c, const LxArgs& 
 
 // dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]
 template <typename T, typename S>
-__global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
+__global__ __launch_bounds__(S::THREADS, 2) void k_lx_dw(LxArgs a) {
   constexpr int WM = S::BM / S::WR, WN = S::BN / S::WC;
   PG_MM_LDS(S, buf, 0);
   const int64_t len = a.c_hi - a.c_lo, rows = (a.n + kPad - 1) / kPad * kPad;
@@ -491,6 +491,9 @@ __global__ __launch_bounds__(S::THREADS) void k_lx_dw(LxArgs a) {
 
 inline int64_t up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
 
+// tile shapes (BM x BN): one workgroup of 256 x 256 tiles fills a CU's LDS or registers, two of the others do
+enum { BIG = 0, TALL = 1, MID = 2 };
+
 // sizes of one call: everything follows from the shapes, types and alignments of the operands, so that the scratch the caller
 // allocates (for packed operands always) fits the launches
 struct LxPlan {
@@ -498,7 +501,7 @@ struct LxPlan {
   int64_t h_bytes, w_bytes, part_bytes, g_bytes, acc_dh, acc_dw, dbp_bytes;
   int32_t dh_splits, dw_splits, pieces;
   int64_t dh_range, dw_range;
-  int big, dh_cols, dw_cols;                // tile shapes: 256 x 256 logits; columns of the gradients' tiles
+  int logits, dh, dw;                       // tile shapes
   // narrow form
   int narrow, xt_stats, xt_grad, yt;
   int32_t nx_stats, nx_dh, nx_dw;           // splits
@@ -549,11 +552,15 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
     return p;
   }
   // 256 x 256 tiles need a quarter less LDS traffic and two thirds of the loads of 128 x 128 ones, and fill the card from 256 tiles
-  // on: at half of that 128 x 128 ones, two to a CU, are ahead (fp16 777 x 602 -> 1153, 20 against 70 tiles: logits 22 -> 12.5 us)
-  p.big = ceil_div<int64_t>(n, 256) * ceil_div<int64_t>(C, 256) >= 192;
-  const int64_t bm = p.big ? 256 : 128;
-  p.tiles = ceil_div<int64_t>(C, bm);
-  p.row_tiles = ceil_div<int64_t>(n, bm);
+  // on: at half of that 128 x 128 ones, two to a CU, are ahead (fp16 777 x 602 -> 1153, 20 against 70 tiles: logits 22 -> 12.5 us).
+  // 256 x 128 tiles, two to a CU, hide one tile's exponentials behind the other's products, which pays while the exponentials are
+  // a good part of a tile (us with gradients, 256 x 256 against 256 x 128: bf16 8192 x 320 -> 65536 2125, 2050; 8192 x 512 -> 32768
+  // 1259, 1188; 8192 x 768 -> 32768 1971, 1936; 8192 x 1024 -> 65536 4204, 4288; fp32, six products a tile: 4096 x 1024 -> 16384
+  // 2849, 3059)
+  const bool big = ceil_div<int64_t>(n, 256) * ceil_div<int64_t>(C, 256) >= 192;
+  p.logits = !big ? MID : np == 1 && p.Kp <= 768 ? TALL : BIG;
+  p.tiles = ceil_div<int64_t>(C, big ? 256 : 128);
+  p.row_tiles = ceil_div<int64_t>(n, p.logits == BIG ? 256 : 128);
   p.part_bytes = up(n * p.tiles * 8, 256);
   // a piece of G: half a GB (128 MB, 256 MB, half a GB: 4690, 4363, 4280 us at bf16 8192 x 1024 -> 65536, 3005, 2847, 2680 at fp16
   // 16384 x 512 -> 32768: fewer launches with a ragged end each, and fewer passes over dh's running sum)
@@ -566,28 +573,36 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
   p.pieces = (int32_t)ceil_div<int64_t>(C, p.piece);
   p.ldg = p.piece + 64;        // (rows a power of two apart would share their memory channels: dh 296 -> 279 us at 8192 x 1024 -> 65536)
   p.g_bytes = up(np * p.g_rows * p.ldg * 2, 256);
-  // gradient tiles likewise; splits of the reductions: enough workgroups for the 256 CUs, ranges of at least four times 64
-  auto split = [&](int64_t rows, int64_t len, int* cols, int32_t* s, int64_t* range) {
-    const int64_t big = ceil_div<int64_t>(rows, 256) * ceil_div<int64_t>(K, 256);
-    *cols = p.Kp >= 256 && big * (len / 1024) >= 192 ? 256 : p.Kp > 64 ? 128 : 64;
-    const int64_t tiles = *cols == 256 ? big : ceil_div<int64_t>(rows, 128) * ceil_div<int64_t>(K, *cols);
-    int64_t want = ceil_div<int64_t>(*cols == 256 ? 256 : 512, tiles), most = len / (4 * kPad);
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    *range = up(ceil_div<int64_t>(len, want), kPad);
+  // A gradient's tiles and the splits of its reduction: the cheapest by a count of rounds of workgroups over the card, in units of a
+  // round of 256 x 256 tiles. For the same product 256 x 128 tiles take 1.13 times as long as those and 128 x 128 ones 1.31 times
+  // (bf16 8192 x 1024 -> 65536 gradients 2069, 2342, 2714 us; fp32 4096 x 1024 -> 16384 1474, 1662, 1943), but they leave less of
+  // the card idle: bf16 3000 x 300 -> 40000 with gradients 538 us with 256 x 256 alone, 494 so; fp16 777 x 602 -> 1153 165, 143
+  auto split = [&](int64_t rows, int64_t len, int* shape, int32_t* s, int64_t* range) {
+    const struct { int64_t bm, bn, slots; double unit; } shapes[] = {{256, 256, 256, 1.}, {256, 128, 512, 1.13}, {128, 128, 512, 0.65}};
+    // a split's partial result, written and read at 5 TB/s, in units of a round
+    const double extra = (double)rows * (double)K / (double)len * 6.7e-5 / (np == 3 ? 6. : 1.);
+    double best = 1e30;
+    for (int i = BIG; i <= MID; ++i) {
+      const int64_t tiles = ceil_div<int64_t>(rows, shapes[i].bm) * ceil_div<int64_t>(K, shapes[i].bn);
+      for (int64_t k = 1; k <= 64 && (k == 1 || k * 4 * kPad <= len); ++k) {
+        const double cost = shapes[i].unit * (double)ceil_div<int64_t>(tiles * k, shapes[i].slots) / (double)k + (k > 1 ? extra * (double)k : 0.);
+        if (cost < best * 0.999) { best = cost; *shape = i; *s = (int32_t)k; }
+      }
+    }
+    *range = up(ceil_div<int64_t>(len, *s), kPad);
     *s = (int32_t)ceil_div<int64_t>(len, *range);
   };
-  split(n, p.piece, &p.dh_cols, &p.dh_splits, &p.dh_range);
-  split(p.piece, up(n, kPad), &p.dw_cols, &p.dw_splits, &p.dw_range);
+  split(n, p.piece, &p.dh, &p.dh_splits, &p.dh_range);
+  split(p.piece, up(n, kPad), &p.dw, &p.dw_splits, &p.dw_range);
   p.acc_dh = p.dh_splits > 1 || p.pieces > 1 ? up((int64_t)p.dh_splits * n * K * 4, 256) : 0;
   p.acc_dw = p.dw_splits > 1 ? up((int64_t)p.dw_splits * p.piece * K * 4, 256) : 0;
   p.dbp_bytes = up(p.row_tiles * C * 4, 256);
   return p;
 }
 
-template <typename T> using BigTile = Shape<typename Mul<T>::E, Mul<T>::NP, 256, 256, 2, 4>;
-template <typename T> using MidTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128, 128, 2, 2>;
-template <typename T> using SlimTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128, 64, 2, 2>;
+template <typename T> using BigTile = Shape<typename Mul<T>::E, Mul<T>::NP, 256, 256, 2, 4, 4>;
+template <typename T> using TallTile = Shape<typename Mul<T>::E, Mul<T>::NP, 256, 128, 2, 2, 3>;
+template <typename T> using MidTile = Shape<typename Mul<T>::E, Mul<T>::NP, 128, 128, 2, 2, 4>;
 
 // operands in parts: in place where they are padded 16-bit rows already, else packed into h_dst / w_dst by one launch
 template <typename T>
@@ -716,6 +731,20 @@ int narrow_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, 
   return lx_sums<T>(dh, dw, db, a, st);
 }
 
+template <typename T, bool PIECE>
+void lx_launch_logits(const LxArgs& a, const LxPlan& p, dim3 grid, hipStream_t st) {
+  if (p.logits == BIG) {
+    hipLaunchKernelGGL((k_lx_logits<T, BigTile<T>, PIECE>), grid, dim3(BigTile<T>::THREADS), 0, st, a);
+    return;
+  }
+  if constexpr (Mul<T>::NP == 1)
+    if (p.logits == TALL) {
+      hipLaunchKernelGGL((k_lx_logits<T, TallTile<T>, PIECE>), grid, dim3(TallTile<T>::THREADS), 0, st, a);
+      return;
+    }
+  hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, PIECE>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
+}
+
 template <typename T>
 int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char* s, hipStream_t st) {
   if (p.narrow) return narrow_forward<T>(a, d, p, s, st);
@@ -730,10 +759,7 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   a.c_lo = 0;
   a.c_hi = a.C;
   const dim3 grid((unsigned)(p.tiles * p.row_tiles));
-  if (p.big)
-    hipLaunchKernelGGL((k_lx_logits<T, BigTile<T>, false>), grid, dim3(BigTile<T>::THREADS), 0, st, a);
-  else
-    hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, false>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
+  lx_launch_logits<T, false>(a, p, grid, st);
   PG_LAUNCH_CHECK();
   hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
@@ -764,16 +790,16 @@ int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipSt
     a.range = p.dh_range;
     a.first = a.c_lo == 0;
     a.direct = p.dh_splits == 1 && p.pieces == 1;
-    const int rc = p.dh_cols == 256 ? lx_launch_dh<T, BigTile<T>>(a, st) : p.dh_cols == 128 ? lx_launch_dh<T, MidTile<T>>(a, st)
-                                                                                            : lx_launch_dh<T, SlimTile<T>>(a, st);
+    const int rc = p.dh == BIG ? lx_launch_dh<T, BigTile<T>>(a, st) : p.dh == TALL ? lx_launch_dh<T, TallTile<T>>(a, st)
+                                                                                                          : lx_launch_dh<T, MidTile<T>>(a, st);
     if (rc != PG_OK) return rc;
   }
   if (a.dw) {
     a.acc = acc_dw;
     a.splits = p.dw_splits;
     a.range = p.dw_range;
-    const int rc = p.dw_cols == 256 ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw_cols == 128 ? lx_launch_dw<T, MidTile<T>>(a, st)
-                                                                                            : lx_launch_dw<T, SlimTile<T>>(a, st);
+    const int rc = p.dw == BIG ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw == TALL ? lx_launch_dw<T, TallTile<T>>(a, st)
+                                                                                                          : lx_launch_dw<T, MidTile<T>>(a, st);
     if (rc != PG_OK) return rc;
     if (a.splits > 1 && p.pieces > 1)
       return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, (a.c_hi - a.c_lo) * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
@@ -801,11 +827,8 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   a.g_rows = p.g_rows;
   for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
     a.c_hi = a.c_lo + p.piece < a.C ? a.c_lo + p.piece : a.C;
-    const dim3 grid((unsigned)(ceil_div<int64_t>(a.c_hi - a.c_lo, p.big ? 256 : 128) * p.row_tiles));
-    if (p.big)
-      hipLaunchKernelGGL((k_lx_logits<T, BigTile<T>, true>), grid, dim3(BigTile<T>::THREADS), 0, st, a);
-    else
-      hipLaunchKernelGGL((k_lx_logits<T, MidTile<T>, true>), grid, dim3(MidTile<T>::THREADS), 0, st, a);
+    const dim3 grid((unsigned)(ceil_div<int64_t>(a.c_hi - a.c_lo, p.logits == MID ? 128 : 256) * p.row_tiles));
+    lx_launch_logits<T, true>(a, p, grid, st);
     PG_LAUNCH_CHECK();
     rc = lx_gradients<T>(a, p, acc_dh, acc_dw, st);
     if (rc != PG_OK) return rc;
