@@ -510,7 +510,8 @@ def test_linear_cross_entropy_reductions(dev, hiplib, t, reduction, bias):
 @gpu
 @pytest.mark.parametrize("n,K,C,t", [(4099, 40, 20011, F32), (4099, 40, 20011, BF16), (4099, 131, 11003, F32), (4099, 260, 33001, BF16),
                                      (300, 300, 9000, F16), (2500, 520, 4097, BF16), (1300, 1030, 2050, F32),
-                                     (8201, 131, 11003, F32), (8201, 260, 33001, BF16)])
+                                     (8201, 131, 11003, F32), (8201, 260, 33001, BF16), (4099, 1030, 8200, BF16), (3000, 1030, 6001, F16),
+                                     (8201, 300, 11003, F32)])
 def test_linear_cross_entropy_large(dev, hiplib, n, K, C, t):
     """several splits of the classes and rows, several pieces of the vocabulary with a ragged last one, large and small tiles"""
     check_xent(dev, n, K, C, t, ignored=0.05)
