@@ -4,14 +4,16 @@
 // function of (row, column, seed, tag, step), is never stored, and is the one the fused aggregations draw for the same row — the
 // backward pass draws it again. One Philox4x32-10 call makes eight 16-bit words: the columns 4p..4p+3 and 4p+256..4p+259 of one
 // row, so a thread owns those eight columns ("a pair of pieces") and no word is drawn twice. Ten rounds of two 32x32 products are
-// what the ALU pays; the bound is HBM (each element read once, written once).
+// what the ALU pays; the bound is HBM (each element read once, written once): 16384 x 2048 bf16 26 us = 5.1 TB/s, 6000 x 602 fp32
+// 10 us = 2.9 TB/s (rows of no whole 16-byte pieces; the launch is a fifth of it).
 //
 // Layer norm: s = dropout(x) + residual, y = (s - mean) * rstd * w + b, biased variance. A row lives in the registers of G lanes
 // (S pairs of pieces each), so mean and variance are two exact passes over registers and the row is read once. Backward:
 //   gh = gy * w, xh = (s - mean) * rstd, ds = rstd * (gh - mean(gh) - xh * mean(gh * xh)) + gs
 // in one pass over (gy, s, gs); dw = sum_r gy * xh and db = sum_r gy accumulate in registers over the rows a group walks, are
 // added up inside the workgroup and leave as one partial row per workgroup, which a second launch sums in a fixed order
-// (deterministic: no atomics). Bound: HBM.
+// (deterministic: no atomics). Bound: HBM: 16384 x 2048 bf16 with dropout and residual forward 58 us = 4.6 TB/s, backward 68 to 73 us
+// = 4.6 to 4.9 TB/s; 6000 x 602 fp32 with residual 13 and 17 us. Rows above 8192 columns spill in the backward pass.
 #include "pg_elem.h"
 
 namespace pg {

@@ -8,11 +8,14 @@
 //
 // All three products run on one tile engine (pg_mm.h) with fp32 accumulation. Its operands are 16-bit parts in rows padded to
 // whole tiles: 16-bit rows that are so already are used in place, others are packed first (k_lx_pack). fp32 values are split
-// into three bf16 parts (x = x0 + x1 + x2 to 24 bits) and six of the nine partial products are summed; what is left out is below
-// 2^-24 of the product — 2.5 PF / 6 where the fp32 matrix instructions reach 0.157 PF.
+// into three bf16 parts (x = x0 + x1 + x2 exactly, each at most 2^-8 of the one before) and six of the nine partial products are
+// summed; the three left out, x1 y2 + x2 y1 + x2 y2, are below 2^-22.9 of the product. 2.5 PF / 6 where the fp32 matrix
+// instructions reach 0.157 PF.
 // G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-8, fp16 2^-11 relative),
 // independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
 // of 2^-28 is still a normal number.
+// Measured at bf16 8192 x 1024 -> 65536 (2 n K C = 1.1 TFLOP a product; the library's 16384^3 product reaches 1.59 PF): statistics
+// 1.02 ms, G 1.23 ms, dh 0.98 ms, dW 0.90 ms, that is 1.08, 0.90, 1.12, 1.22 PF, 4.1 ms with gradients.
 #include "pg_xent_narrow.h"
 
 namespace pg {
@@ -147,6 +150,7 @@ __global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1, SideA
 
 // One BM-class x BN-row tile of logits; a lane holds one row's classes in registers: row = 32 j + lane % 32 of its wave's rows,
 // class = 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4 of its wave's classes, so a row's maximum and sum are taken in registers.
+// The tile's exponentials and its LDS trip follow its product, some 8000 cycles behind 33 000 (K = 1024): what bounds it.
 // PIECE: writes G (through LDS: whole 16-byte pieces of rows) and the column sums of the tile, else the tile's row statistics.
 template <typename T, typename S, bool PIECE>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
@@ -387,6 +391,7 @@ __device__ __forceinline__ void each_output(const f32x16 (&acc)[S::FI][S::FJ], i
     }
 }
 
+// G [rows x classes] W: G's rows are read as they stand, W through the transposing reads. Bound by the matrix instructions.
 // dh: acc[split][r][k] (+)= sum over the split's classes of G[r][c] W[c][k]
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dh(LxArgs a) {
@@ -463,6 +468,7 @@ int lx_sums(const SumArgs& a, const SumArgs& b, const SumArgs& c, const LxArgs& 
   return PG_OK;
 }
 
+// G^T h, both through the transposing reads (neither is ever transposed in memory). Bound by the matrix instructions.
 // dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dw(LxArgs a) {

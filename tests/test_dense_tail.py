@@ -423,7 +423,7 @@ def xent_reference(h, lin, lab, up):
     lse = top + torch.log(torch.exp(z - top).sum(1, keepdim=True))
     zero = torch.zeros(n, dtype=torch.float64, device=h.device)
     loss = torch.where(ok, (lse - z.gather(1, at)).view(-1), zero)
-    # a logit: K products, each exact to 2^-22 at worst (fp32 in three bf16 parts drops x1 y2 + x2 y1 + x2 y2 < 2^-24 |x y|, 16-bit
+    # a logit: K products, each exact to 2^-22 at worst (fp32 in three bf16 parts drops x1 y2 + x2 y1 + x2 y2 < 2^-22.9 |x y|, 16-bit
     # products are exact), K + 8 additions
     mag = H.abs() @ W.abs().t() + torch.where(torch.isfinite(b), b.abs(), torch.zeros_like(b))
     ez = (K + 16) * E * (mag.amax(1) if n else zero) if n else zero
