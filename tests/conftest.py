@@ -175,9 +175,14 @@ def run_group(cmd, timeout, **kw):
 
 @pytest.fixture(autouse=True)
 def _host_tables_go_with_their_test(request):
-    """A full-size test's page-locked table (24 GB, 32 GB as allocated) hangs in reference cycles behind it; where a second one is
-    more than the machine will lock, the next such test fails on it. Collected here, its block serves the next one."""
+    """A full-size test's page-locked table (24 GB, 32 GB as allocated) hangs in reference cycles behind it, and then in torch's cache:
+    where a second one is more than the machine will lock, the next such test, or the benchmark that a later one starts, fails on
+    it. Collected and given back here."""
     yield
     if "full_size" in request.node.name:
         import gc
+        import torch
         gc.collect()
+        if torch.cuda.is_available() and hasattr(torch._C, "_host_emptyCache"):
+            torch.cuda.synchronize()
+            torch._C._host_emptyCache()
