@@ -935,6 +935,8 @@ def _capture_state(device):
 
 
 def _watch_graph(name, ctx, device, *inputs):
+    if not ctx.next_functions:                       # gradients are off: no graph is recorded
+        return
     capturing, ctx.stream = _capture_state(device)
     if not capturing:
         _EAGER_GRAPHS.add(ctx)

@@ -839,6 +839,32 @@ def test_capture_is_refused_while_an_eager_graph_lives(dev, hiplib):
 
 
 @gpu
+def test_capture_without_gradients_beside_an_eager_graph(dev, hiplib):
+    """an evaluation that records no graph may be captured whatever graphs of the same parameters live"""
+    from pagraph_amd import ops
+    g = gen(56, dev)
+    lin, norm = head(dev, 32, 200, F32, g), torch.nn.LayerNorm(32, device=dev)
+    x = torch.randn(50, 32, generator=g, device=dev, requires_grad=True)
+    lab = torch.randint(0, 200, (50,), generator=g, device=dev)
+    spec = spec_of(dev, 0.3)
+
+    def run():
+        return ops.linear_cross_entropy(ops.layer_norm(ops.dropout(x, spec), norm), lin, lab)
+    kept = run()
+    with torch.no_grad():
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, kept)
+    assert len(torch.autograd.grad(kept, [x, lin.weight, lin.bias, norm.weight, norm.bias])) == 5
+
+
+@gpu
 def test_two_streams_at_once(dev, hiplib):
     """two steps on two streams at the same time share nothing"""
     g = gen(44, dev)
