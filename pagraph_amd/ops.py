@@ -935,8 +935,6 @@ def _capture_state(device):
 
 
 def _watch_graph(name, ctx, device, *inputs):
-    if not ctx.next_functions:                       # gradients are off: no graph is recorded
-        return
     capturing, ctx.stream = _capture_state(device)
     if not capturing:
         _EAGER_GRAPHS.add(ctx)
@@ -956,17 +954,26 @@ def _drop_fields(spec, step_used=0):
     return spec.threshold, spec.tag, spec.seed, 0 if step is None else step_used or step.data_ptr(), spec.step_value & 0xFFFFFFFFFFFFFFFF
 
 
+_NO_GRAD = (False,) * 6
+
+
+def _needs_grad(ctx):
+    """ctx.needs_input_grad, all False where gradients are off and no graph is recorded"""
+    return ctx.needs_input_grad if ctx.next_functions else _NO_GRAD
+
+
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, spec):
         rows, dev, t = _rows_of(x), x.device, x.dtype
         n, d = rows.shape
         y = torch.empty((n, d), dtype=t, device=dev)
-        used = torch.empty(1, dtype=torch.int64, device=dev) if spec.step is not None and ctx.needs_input_grad[0] else None
+        grad = _needs_grad(ctx)[0]
+        used = torch.empty(1, dtype=torch.int64, device=dev) if grad and spec.step is not None else None
         _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), y.data_ptr(), d, n, d, _DTYPES[t],
                  _DROP_DESC(*_drop_fields(spec)), _addr(used))
         ctx.spec, ctx.used = spec, used
-        if ctx.needs_input_grad[0]:
+        if grad:
             _watch_graph("dropout", ctx, dev, x)
         return _like(y, x.shape)
 
@@ -1003,7 +1010,7 @@ class _LayerNorm(torch.autograd.Function):
         y = torch.empty((n, d), dtype=t, device=dev)
         total = torch.empty((n, d), dtype=t, device=dev) if res is not None else None
         # mean | rstd | the step the mask was drawn with
-        grad = ctx.needs_input_grad
+        grad = _needs_grad(ctx)
         stats = torch.empty(2 * n + 2, dtype=torch.float32, device=dev) if grad[0] or grad[1] or grad[2] or grad[3] else None
         at = _addr(stats)
         param = weight if weight is not None else bias
@@ -1109,7 +1116,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             at + 8 * n, 0, 0, 0, 0, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
         ctx.save_for_backward(h, weight, bias, labels)
         ctx.stats, ctx.ignore_index, ctx.reduction = stats, ignore_index, reduction
-        grad = ctx.needs_input_grad
+        grad = _needs_grad(ctx)
         if grad[0] or grad[1] or grad[2]:
             ctx.scratch = L.load().pg_linear_xent_scratch(n, K, C, t, 1)
             _watch_graph("linear_cross_entropy", ctx, dev, h, weight, bias)
