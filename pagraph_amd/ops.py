@@ -1059,9 +1059,11 @@ class _LayerNorm(torch.autograd.Function):
             0, 0, _addr(weight), 0, rows.data_ptr(), 0, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
             _addr(dw), _addr(db), _addr(part), 0, n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
             dt, _DTYPES[param], ctx.eps, spec is not None, *(_drop_fields(spec, at + 8 * n) if spec is not None else _NO_DROP)))
+        if dx is not None:
+            dx = _like(dx, s.shape)
         if need_res:
-            dres = _like(dx if spec is None else dres, s.shape)
-        return (_like(dx, s.shape) if need_x else None, dw, db, dres, None, None)
+            dres = dx if spec is None else _like(dres, s.shape)          # (one tensor, not two views of it: autograd counts references)
+        return (dx if need_x else None, dw, db, dres, None, None)
 
 
 def layer_norm(x, module, residual=None, dropout=None):

@@ -839,6 +839,25 @@ def test_capture_is_refused_while_an_eager_graph_lives(dev, hiplib):
 
 
 @gpu
+def test_both_summands_keep_gradients_of_their_own(dev, hiplib):
+    """x and the residual get the same values in different memory, also where rows have leading dimensions"""
+    from pagraph_amd import ops
+    norm = torch.nn.LayerNorm(24, device=dev)
+    for shape in ((6, 24), (2, 3, 24), (2, 1, 3, 24)):
+        x = torch.randn(shape, device=dev, requires_grad=True)
+        r = torch.randn(shape, device=dev, requires_grad=True)
+        once = None
+        for k in range(3):
+            y, total = ops.layer_norm(x, norm, residual=r)
+            (y * y * y + total).sum().backward()
+            if once is None:
+                once = x.grad.clone()
+                assert x.grad.data_ptr() != r.grad.data_ptr()
+            want = once if k == 0 else want + once
+            assert torch.equal(x.grad, want) and torch.equal(r.grad, want)
+
+
+@gpu
 def test_capture_without_gradients_beside_an_eager_graph(dev, hiplib):
     """an evaluation that records no graph may be captured whatever graphs of the same parameters live"""
     from pagraph_amd import ops
