@@ -897,10 +897,6 @@ def _row_stride(x):
     return x.stride(0) if x.size(0) > 1 else x.size(1)
 
 
-def _like(rows, shape):
-    return rows if rows.shape == shape else rows.view(shape)
-
-
 def _need_rows(name, x):
     if not x.is_cuda or x.dtype not in _DTYPES or x.dim() < 1 or x.size(-1) == 0:
         raise L.PgError(f"{name} needs fp32, bf16 or fp16 CUDA rows [..., d] with d >= 1 (no CPU fallback)")
@@ -967,7 +963,7 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, spec):
         rows, dev, t = _rows_of(x), x.device, x.dtype
         n, d = rows.shape
-        y = torch.empty((n, d), dtype=t, device=dev)
+        y = torch.empty(x.shape, dtype=t, device=dev)             # (in x's shape: a view made in here could not be changed in place)
         grad = _needs_grad(ctx)[0]
         used = torch.empty(1, dtype=torch.int64, device=dev) if grad and spec.step is not None else None
         _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), y.data_ptr(), d, n, d, _DTYPES[t],
@@ -975,17 +971,17 @@ class _Dropout(torch.autograd.Function):
         ctx.spec, ctx.used = spec, used
         if grad:
             _watch_graph("dropout", ctx, dev, x)
-        return _like(y, x.shape)
+        return y
 
     @staticmethod
     def backward(ctx, gy):
         _once("dropout")
         rows, dev, t = _rows_of(gy), gy.device, gy.dtype
         n, d = rows.shape
-        gx = torch.empty((n, d), dtype=t, device=dev)
+        gx = torch.empty(gy.shape, dtype=t, device=dev)
         _enqueue("pg_dropout_apply", dev, rows.data_ptr(), _row_stride(rows), gx.data_ptr(), d, n, d, _DTYPES[t],
                  _DROP_DESC(*_drop_fields(ctx.spec, _addr(ctx.used))), 0)
-        return _like(gx, gy.shape), None
+        return gx, None
 
 
 def dropout(x, spec):
@@ -1007,8 +1003,8 @@ class _LayerNorm(torch.autograd.Function):
         n, d = rows.shape
         res = _rows_of(residual) if residual is not None else None
         dev, t = x.device, x.dtype
-        y = torch.empty((n, d), dtype=t, device=dev)
-        total = torch.empty((n, d), dtype=t, device=dev) if res is not None else None
+        y = torch.empty(x.shape, dtype=t, device=dev)
+        total = torch.empty(x.shape, dtype=t, device=dev) if res is not None else None
         # mean | rstd | the step the mask was drawn with
         grad = _needs_grad(ctx)
         stats = torch.empty(2 * n + 2, dtype=torch.float32, device=dev) if grad[0] or grad[1] or grad[2] or grad[3] else None
@@ -1025,11 +1021,9 @@ class _LayerNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if stats is not None:
             _watch_graph("layer_norm", ctx, dev, x, weight, bias, residual)
-        y = _like(y, x.shape)
         if res is None:
             ctx.save_for_backward(x, weight)
             return y
-        total = _like(total, x.shape)
         ctx.save_for_backward(total, weight)
         return y, total
 
@@ -1048,9 +1042,9 @@ class _LayerNorm(torch.autograd.Function):
         n, d = rows.shape
         dev, t, param = s.device, s.dtype, ctx.param
         dt = _DTYPES[t]
-        dx = torch.empty((n, d), dtype=t, device=dev) if need_x or (need_res and spec is None) else None
+        dx = torch.empty(s.shape, dtype=t, device=dev) if need_x or (need_res and spec is None) else None
         # one gradient for both summands, as of a sum, unless a mask stands before one of them
-        dres = torch.empty((n, d), dtype=t, device=dev) if need_res and spec is not None else None
+        dres = torch.empty(s.shape, dtype=t, device=dev) if need_res and spec is not None else None
         dw = torch.empty(d, dtype=param, device=dev) if need_w else None
         db = torch.empty(d, dtype=param, device=dev) if need_b else None
         part = torch.empty(ctx.scratch, dtype=torch.float32, device=dev) if need_w or need_b else None
@@ -1059,10 +1053,8 @@ class _LayerNorm(torch.autograd.Function):
             0, 0, _addr(weight), 0, rows.data_ptr(), 0, at, at + 4 * n, g.data_ptr(), _addr(gs), _addr(dx), _addr(dres),
             _addr(dw), _addr(db), _addr(part), 0, n, d, 0, 0, _row_stride(rows), 0, _row_stride(g), _row_stride(gs) if gs is not None else 0, d, d,
             dt, _DTYPES[param], ctx.eps, spec is not None, *(_drop_fields(spec, at + 8 * n) if spec is not None else _NO_DROP)))
-        if dx is not None:
-            dx = _like(dx, s.shape)
-        if need_res:
-            dres = dx if spec is None else _like(dres, s.shape)          # (one tensor, not two views of it: autograd counts references)
+        if need_res and spec is None:
+            dres = dx                                # (one tensor, not two views of it: autograd counts references)
         return (dx if need_x else None, dw, db, dres, None, None)
 
 
@@ -1133,7 +1125,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         n, K, C = rows.size(0), rows.size(1), weight.size(0)
         dev, t = h.device, _DTYPES[h.dtype]
         new = torch.zeros if n == 0 else torch.empty
-        dh = new((n, K), dtype=h.dtype, device=dev) if need_h else None
+        dh = new(h.shape, dtype=h.dtype, device=dev) if need_h else None
         dw = new((C, K), dtype=h.dtype, device=dev) if need_w else None
         db = new((C,), dtype=h.dtype, device=dev) if need_b and bias is not None else None
         if n > 0:
@@ -1144,7 +1136,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 rows.data_ptr(), weight.data_ptr(), _addr(bias), labels.data_ptr(), at, at + 4 * n, 0, 0, at + 8 * n,
                 g.data_ptr(), _addr(dh), _addr(dw), _addr(db), scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight),
                 g.stride(0), ctx.ignore_index, t, ctx.reduction))
-        return _like(dh, h.shape) if need_h else None, dw, db, None, None, None
+        return dh, dw, db, None, None, None
 
 
 def _table(weight):

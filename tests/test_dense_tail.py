@@ -839,6 +839,21 @@ def test_capture_is_refused_while_an_eager_graph_lives(dev, hiplib):
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(24,), (5, 24), (2, 3, 24)])
+def test_outputs_of_any_rank_may_be_changed_in_place(dev, hiplib, shape):
+    from pagraph_amd import ops
+    norm, spec = torch.nn.LayerNorm(24, device=dev), spec_of(dev, 0.5)
+    for f in (lambda x: ops.dropout(x, spec), lambda x: ops.layer_norm(x, norm), lambda x: ops.layer_norm(x, norm, residual=x)[0]):
+        x = torch.randn(shape, device=dev, requires_grad=True)
+        y = f(x)
+        assert y.shape == x.shape
+        want, = torch.autograd.grad((3.0 * f(x)).sum(), x)
+        y.mul_(3.0)
+        got, = torch.autograd.grad(y.sum(), x)
+        assert got.shape == x.shape and torch.equal(got, want)
+
+
+@gpu
 def test_both_summands_keep_gradients_of_their_own(dev, hiplib):
     """x and the residual get the same values in different memory, also where rows have leading dimensions"""
     from pagraph_amd import ops
