@@ -5,7 +5,7 @@
 // backward pass draws it again. One Philox4x32-10 call makes eight 16-bit words: the columns 4p..4p+3 and 4p+256..4p+259 of one
 // row, so a thread owns those eight columns ("a pair of pieces") and no word is drawn twice. Ten rounds of two 32x32 products are
 // what the ALU pays; the bound is HBM (each element read once, written once): 16384 x 2048 bf16 26 us = 5.1 TB/s, 6000 x 602 fp32
-// 10 us = 2.9 TB/s (rows of no whole 16-byte pieces; the launch is a fifth of it).
+// 8.2 us = 3.5 TB/s (rows of no whole 16-byte pieces).
 //
 // Layer norm: s = dropout(x) + residual, y = (s - mean) * rstd * w + b, biased variance. A row lives in the registers of G lanes
 // (S pairs of pieces each), so mean and variance are two exact passes over registers and the row is read once. Backward:
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_
     const int rows = n - r0 < rows_per_block ? (int)(n - r0) : rows_per_block;
     const int total = rows * units;
     for (int i = threadIdx.x; i < total; i += 256) {
-      // (several rows per block only while rows * units <= 1024: the quotient in floating point is then exact)
+      // (several rows per block only while rows * units <= 512: the quotient in floating point is then exact)
       const int lr = rows_per_block > 1 ? (int)(((float)i + 0.5f) * inv_units) : 0;
       const int u = i - lr * units, c0 = unit_col<V>(u), c1 = c0 + 256;
       const int64_t r = r0 + lr;
@@ -553,7 +553,10 @@ int dispatch_norm(const NormArgs& a, int64_t bwd, hipStream_t st) {
 
 template <typename T>
 void launch_dropout(const void* x, int64_t xs, void* y, int64_t ys, int64_t n, int64_t d, const DropArgs& dr, uint64_t* used, hipStream_t st) {
-  const int v = sizeof(T) == 2 && d % 8 == 0 ? 2 : 1, units = (row_pairs(d) + v - 1) / v, rows = units >= 512 ? 1 : 1024 / units;
+  // one unit a thread where a row has at most 128 of them, two up to 255 (fewer idle threads): with four, too few workgroups for the
+  // card on short batches (6000 x 602 fp32 8.6 against 7.2 us, 65536 x 17 fp16 6.7 against 4.6, 16384 x 2048 bf16 22.2 and 22.4)
+  const int v = sizeof(T) == 2 && d % 8 == 0 ? 2 : 1, units = (row_pairs(d) + v - 1) / v;
+  const int rows = units >= 256 ? 1 : units > 128 ? 512 / units : 256 / units;
   const int64_t blocks = ceil_div<int64_t>(n, rows);
   const dim3 grid((unsigned)(blocks > 65536 ? 65536 : blocks));
   const float inv = 1.f / (float)units;
