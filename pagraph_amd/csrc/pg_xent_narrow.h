@@ -217,6 +217,13 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
   }
 }
 
+// every wave's share of the next tile has landed and none still reads the buffer that is filled next. A barrier alone promises only
+// the second: a wave's loads into LDS are its own to wait for
+__device__ __forceinline__ void next_tile() {
+  wait_loads<0>();
+  __syncthreads();
+}
+
 template <typename T, int KP, int XB, int MODE>
 __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
   typedef Narrow<T, KP, XB> N;
@@ -278,10 +285,10 @@ __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
       }
     }
     for (int64_t y = y_lo; y < y_hi; y += 2 * N::YT) {
-      __syncthreads();
+      next_tile();
       nx_step<T, KP, XB, MODE>(buf, side, buf + N::TILE, side + 192, y + N::YT < y_hi, a, y, y + N::YT, wave, lane, st);
       if (y + N::YT < y_hi) {
-        __syncthreads();
+        next_tile();
         nx_step<T, KP, XB, MODE>(buf + N::TILE, side + 192, buf, side, y + 2 * N::YT < y_hi, a, y + N::YT, y + 2 * N::YT, wave, lane, st);
       }
     }
