@@ -632,8 +632,9 @@ int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
  * of pg_head + pg_xent_*): h [n, K], W [C, K], bias [C] or NULL, all of `dtype`. Rows whose label is ignore_index or outside
  * [0, C) are not counted, have loss 0 and gradient 0, and do not enter dW / db whatever h holds there.
  * forward:  PG_XENT_MEAN / _SUM: *loss (nan for the mean when no row counts); PG_XENT_NONE: row_loss [n]. And what the backward
- *           pass reads: lse [n], flag [n] (1: counted), meta [1] = 1 / #counted rows (0).
- * backward: given the forward's lse, flag, meta and grad = d objective / d loss (device fp32: one value for PG_XENT_MEAN / _SUM,
+ *           pass reads: top [n], a row's largest logit times log2(e); sum [n], its sum of exponentials over that one (0: the row is not
+ *           counted); meta [1] = 1 / #counted rows (0).
+ * backward: given the forward's top, sum, meta and grad = d objective / d loss (device fp32: one value for PG_XENT_MEAN / _SUM,
  *           [n] with grad_stride for PG_XENT_NONE): dh [n, K], dW [C, K], db [C], dense, each may be NULL. n >= 1.
  * scratch: pg_linear_xent_scratch(n, K, C, dtype, backward) bytes (negative: the sizes are refused). Deterministic.           */
 #define PG_XENT_MEAN 0
@@ -644,8 +645,8 @@ typedef struct pg_linear_xent_desc {
   const void* W;
   const void* bias;
   const int64_t* labels;
-  float* lse;
-  float* flag;
+  float* top;
+  float* sum;
   float* row_loss;
   float* loss;
   float* meta;

@@ -118,7 +118,7 @@ class PgNormDesc(ctypes.Structure):
 
 
 class PgLinearXentDesc(ctypes.Structure):
-    _fields_ = [(n, vp) for n in ("h", "W", "bias", "labels", "lse", "flag", "row_loss", "loss", "meta", "grad", "dh", "dW", "db", "scratch")] + \
+    _fields_ = [(n, vp) for n in ("h", "W", "bias", "labels", "top", "sum", "row_loss", "loss", "meta", "grad", "dh", "dW", "db", "scratch")] + \
                [(n, c_i64) for n in ("n", "K", "C", "h_stride", "w_stride", "grad_stride", "ignore_index")] + \
                [("dtype", c_i32), ("reduction", c_i32)]
 

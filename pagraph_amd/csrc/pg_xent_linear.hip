@@ -1,6 +1,6 @@
 // Softmax cross entropy of a class head z = h W^T + b of any width, without its logits:
-//   lse_r = log sum_c exp z_rc,  loss_r = lse_r - z_r,label,
-//   G = (exp(z - lse) - onehot(label)) * (row factor),  dh = G W,  dW = G^T h,  db = sum_r G.
+//   m_r = max_c z_rc,  s_r = sum_c exp(z_rc - m_r),  loss_r = m_r - z_r,label + log s_r,
+//   G = (exp(z - m) / s - onehot(label)) * (row factor),  dh = G W,  dW = G^T h,  db = sum_r G.
 // The logits [n, C] exist only as tiles in registers. Forward: every workgroup leaves (maximum, sum of exponentials) of its tile's
 // rows, a second launch joins them. Backward: the logits are computed again in pieces of the vocabulary; a piece's G leaves in
 // 16-bit parts and feeds the two gradient products before the next piece overwrites it. 8 n K C operations instead of the 6 n K C
@@ -34,16 +34,16 @@ struct LxArgs {
   const int64_t* labels;
   int64_t n, K, Kp, C, ignore;             // Kp: K padded to whole tiles
   float2* part;                            // [n][tiles] maximum, sum of exponentials
-  float *zlab, *lse, *row_loss, *flag, *meta;
+  float *zlab, *top, *sum, *row_loss, *meta;
   int64_t tiles;
   // backward
-  const float* rowf;                       // row factors: flag, or the normalised incoming gradients
+  const float* rowf;                       // row factors: the normalised incoming gradients (NULL: 1 for rows that count)
   const float *f1, *f2;                    // the outputs' factor = *f1 * *f2 (NULL = 1)
   void* g;                                 // a piece of G: [parts][g_rows][ldg], zeros beyond n and beyond c_hi
   int64_t ldg, g_rows, c_lo, c_hi;         // the piece's classes
   float* acc;                              // fp32 partial products [split][rows][K]
   float* dbp;                              // [row tiles][C] partial sums of G
-  const float *bias2, *lse2, *rowf2;       // side arrays (SideArgs)
+  const float *bias2, *top2, *inv2, *rowf2;        // side arrays (SideArgs)
   const int32_t* lab2;
   int32_t scaled;
   void *dh, *dw, *db;
@@ -64,12 +64,14 @@ struct PackArgs {
   int64_t ignore, C;
 };
 // what the products' epilogues read beside the operands, padded past the last class / row (see NxArgs): base-2 biases, labels as int32,
-// and for the gradients the rows' lse (less the exponent of G's scale) and factors
+// and for the gradients the rows' largest logits, the inverses of their sums (times G's scale) and their factors. The two stay apart:
+// in one number, log2 of the sum would be lost beside a large logit (rows of nothing but masked classes: exponentials of 1 each
+// instead of one C-th)
 struct SideArgs {
   const void* bias;
-  float *bias2, *lse2, *rowf2;             // bias2 == NULL: nothing to do; lse2 == NULL: no gradients
+  float *bias2, *top2, *inv2, *rowf2;      // bias2 == NULL: nothing to do; top2 == NULL: no gradients
   int32_t* lab;
-  const float *lse, *rowf;
+  const float *top, *sum, *rowf;
   const int64_t* labels;
   int64_t n, rows_p, C, classes_p, ignore;
 };
@@ -80,7 +82,7 @@ __device__ __forceinline__ void lx_side(const SideArgs& a) {
       float b = i < a.C ? 0.f : -INFINITY;
       if (i < a.C && a.bias) {
         b = (float)((const T*)a.bias)[i];
-        // (a finite lowest value stays finite: a row of nothing else is uniform, not empty)
+        // (a finite lowest value stays finite: a row of nothing else is uniform, as in natural units)
         b = b == -INFINITY ? b : b * kLog2e < -3.402823466e38f ? -3.402823466e38f : b * kLog2e;
       }
       a.bias2[i] = b;
@@ -88,9 +90,10 @@ __device__ __forceinline__ void lx_side(const SideArgs& a) {
     if (i < a.rows_p) {
       const int64_t lab = i < a.n ? a.labels[i] : -1;
       const bool ok = i < a.n && lab != a.ignore && lab >= 0 && lab < a.C;
-      if (a.lse2) {
-        const float f = ok ? a.rowf[i] : 0.f;
-        a.lse2[i] = f != 0.f ? a.lse[i] - __builtin_log2f(Mul<T>::G) : INFINITY;       // rows without a gradient: exponentials of 0
+      if (a.top2) {
+        const float f = !ok ? 0.f : a.rowf ? a.rowf[i] : 1.f;
+        a.top2[i] = f != 0.f ? a.top[i] : INFINITY;          // rows without a gradient: exponentials of 0
+        a.inv2[i] = f != 0.f ? Mul<T>::G / a.sum[i] : 0.f;
         a.rowf2[i] = f;
         a.lab[i] = f != 0.f ? (int32_t)lab : -1;
       } else {
@@ -172,12 +175,13 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
   mm_product<S, ROWS, ROWS>(Operand{a.w, a.w_ld, a.w_part, c0, a.C, 0}, Operand{a.h, a.h_ld, a.h_part, r0, a.h_rows, 0}, 0, a.Kp, buf, acc);
   const int cw = wm * WM + 4 * (lane >> 5);                  // the lane's first class within the tile
   int at[S::FJ];                                             // the rows' labels, counted from there
-  float lse[S::FJ];
+  float top[S::FJ], inv[S::FJ];
 #pragma unroll
   for (int j = 0; j < S::FJ; ++j) {
     const int64_t r = r0 + wn * WN + j * 32 + (lane & 31);   // (the side arrays are padded to whole tiles of rows)
     at[j] = a.lab2[r] - (int)c0 - cw;
-    lse[j] = PIECE ? a.lse2[r] : 0.f;
+    top[j] = PIECE ? a.top2[r] : 0.f;
+    inv[j] = PIECE ? a.inv2[r] : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < S::FI; ++i) {
@@ -196,7 +200,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
     for (int j = 0; j < S::FJ; ++j) {
       if constexpr (PIECE) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - lse[j]);
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - top[j]) * inv[j];
       }
       if (__any((unsigned)(at[j] - 32 * i) < 32u)) {         // does any of the wave's rows have its label among these 32 classes?
 #pragma unroll
@@ -321,16 +325,15 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
     m = mm;
   }
   if (lane == 0) {
-    const float lse = m + log2f(s);
     const bool ok = label_ok(a.labels[r], a);
-    a.lse[r] = lse;
-    a.flag[r] = ok ? 1.f : 0.f;
-    a.row_loss[r] = ok ? (lse - a.zlab[r]) * 0.693147180559945309417f : 0.f;
+    a.top[r] = m;
+    a.sum[r] = !ok ? 0.f : s > 0.f ? s : NAN;               // (a row of nothing but -inf counts, and its loss is NaN)
+    a.row_loss[r] = ok ? ((m - a.zlab[r]) + log2f(s)) * 0.693147180559945309417f : 0.f;
   }
 }
 
 // one block, fixed order: the loss (mean or sum) and meta = 1 / counted rows
-__global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_loss, const float* __restrict__ flag, int64_t n,
+__global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_loss, const float* __restrict__ sum, int64_t n,
                                                   int mean, float* __restrict__ loss, float* __restrict__ meta) {
   __shared__ float ss[1024];
   __shared__ int sc[1024];
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_
   int c = 0;
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
     s += row_loss[i];
-    c += flag[i] != 0.f;
+    c += sum[i] != 0.f;
   }
   ss[threadIdx.x] = s;
   sc[threadIdx.x] = c;
@@ -358,12 +361,12 @@ __global__ __launch_bounds__(1024) void k_lx_mean(const float* __restrict__ row_
 
 // incoming gradients of single rows: row factors g / max|g| (G then uses its type's range whatever the caller's scale), the
 // maximum becomes the outputs' factor. Of the finite ones: an infinite or NaN gradient stays that, in its own row
-__global__ __launch_bounds__(1024) void k_lx_row_factors(const float* __restrict__ g, int64_t gs, const float* __restrict__ flag,
+__global__ __launch_bounds__(1024) void k_lx_row_factors(const float* __restrict__ g, int64_t gs, const float* __restrict__ sum,
                                                          int64_t n, float* __restrict__ rowf, float* __restrict__ top) {
   __shared__ float ss[1024];
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (flag[i] != 0.f && fabsf(g[i * gs]) < INFINITY) m = fmaxf(m, fabsf(g[i * gs]));
+    if (sum[i] != 0.f && fabsf(g[i * gs]) < INFINITY) m = fmaxf(m, fabsf(g[i * gs]));
   ss[threadIdx.x] = m;
   __syncthreads();
   for (int o = 512; o > 0; o >>= 1) {
@@ -371,7 +374,7 @@ __global__ __launch_bounds__(1024) void k_lx_row_factors(const float* __restrict
     __syncthreads();
   }
   m = ss[0] > 0.f ? ss[0] : 1.f;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) rowf[i] = flag[i] != 0.f ? g[i * gs] / m : 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) rowf[i] = sum[i] != 0.f ? g[i * gs] / m : 0.f;
   if (threadIdx.x == 0) *top = m;
 }
 
@@ -426,9 +429,9 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dh(LxArgs a) {
   if (a.direct) {
     const float f = out_factor(a) / Mul<T>::G;
     T* out = (T*)a.dh + r0 * a.K + n0;
-    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
+    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf2[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
   } else {
-    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { sum[r * a.K + k] = a.rowf[r0 + r] == 0.f ? 0.f : v; });
+    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { sum[r * a.K + k] = a.rowf2[r0 + r] == 0.f ? 0.f : v; });
   }
 }
 
@@ -539,7 +542,7 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
   p.w_bytes = up(np * p.w_rows * p.Kp * 2, 256);
   p.classes_p = up(C, 256) + 64;
   p.rows_p = p.h_rows + 64;
-  p.side_bytes = up(p.classes_p * 4, 256) + 3 * up(p.rows_p * 4, 256);
+  p.side_bytes = up(p.classes_p * 4, 256) + 4 * up(p.rows_p * 4, 256);
   // (us, narrow against wide. fp32 6000 -> 50000: 64 columns forward 223, 343, with gradients 1109, 2645; 128: 424, 501 and 1963,
   // 3464. bf16 8192 -> 65536: 128 columns 188, 264 and 775, 1408; 192: 239, 325 and 1001, 1712; 256: forward 269, 390, but the
   // gradients alone 1652, 1478, since 256 columns of operands and sums do not fit the registers of a wave)
@@ -656,7 +659,7 @@ int launch_narrow(const NxArgs& n, const LxPlan& p, hipStream_t st) {
   return launch_narrow_kp<T, 128, MODE>(n, st);
 }
 
-// the side arrays at s, in the order bias2 | labels | lse | row factors
+// the side arrays at s, in the order bias2 | labels | largest logits | inverse sums | row factors
 inline SideArgs lx_side_arrays(const LxArgs& a, const LxPlan& p, char* s, bool grads) {
   SideArgs side{};
   const int64_t rows = up(p.rows_p * 4, 256);
@@ -665,9 +668,10 @@ inline SideArgs lx_side_arrays(const LxArgs& a, const LxPlan& p, char* s, bool g
   side.bias2 = (float*)s;
   side.lab = (int32_t*)(s + up(p.classes_p * 4, 256));
   if (grads) {
-    side.lse2 = (float*)((char*)side.lab + rows);
-    side.rowf2 = (float*)((char*)side.lab + 2 * rows);
-    side.lse = a.lse; side.rowf = a.rowf;
+    side.top2 = (float*)((char*)side.lab + rows);
+    side.inv2 = (float*)((char*)side.lab + 2 * rows);
+    side.rowf2 = (float*)((char*)side.lab + 3 * rows);
+    side.top = a.top; side.sum = a.sum; side.rowf = a.rowf;
   }
   return side;
 }
@@ -716,7 +720,7 @@ int narrow_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, 
   SumArgs dh{}, dw{}, db{};
   if (a.dh) {
     NxArgs n = narrow_args(a, false);
-    n.side0 = side.bias2; n.xa = side.lse2; n.xb = side.rowf2; n.xlab = side.lab;
+    n.side0 = side.bias2; n.xa = side.top2; n.xi = side.inv2; n.xb = side.rowf2; n.xlab = side.lab;
     n.splits = p.nx_dh; n.range = p.rs_dh; n.acc = acc_dh; n.out = a.dh;
     rc = launch_narrow<T, NX_DH>(n, p, st);
     if (rc != PG_OK) return rc;
@@ -724,8 +728,8 @@ int narrow_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, 
   }
   if (a.dw || a.db) {
     NxArgs n = narrow_args(a, true);
-    n.side0 = side.lse2; n.side1 = (const float*)side.lab; n.side2 = side.rowf2; n.xa = side.bias2;
-    n.scaled = a.rowf != a.flag;
+    n.side0 = side.top2; n.side1 = (const float*)side.lab; n.side2 = side.rowf2; n.side3 = side.inv2; n.xa = side.bias2;
+    n.scaled = a.rowf != nullptr;
     n.splits = p.nx_dw; n.range = p.rs_dw; n.acc = acc_dw; n.accb = acc_dw + (int64_t)p.nx_dw * a.C * a.K; n.out = a.dw; n.outb = a.db;
     rc = launch_narrow<T, NX_DW>(n, p, st);
     if (rc != PG_OK) return rc;
@@ -827,8 +831,8 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   const SideArgs side = lx_side_arrays(a, p, s + p.h_bytes + p.w_bytes, true);
   int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, side, st);
   if (rc != PG_OK) return rc;
-  a.bias2 = side.bias2; a.lab2 = side.lab; a.lse2 = side.lse2; a.rowf2 = side.rowf2;
-  a.scaled = a.rowf != a.flag;
+  a.bias2 = side.bias2; a.lab2 = side.lab; a.top2 = side.top2; a.inv2 = side.inv2; a.rowf2 = side.rowf2;
+  a.scaled = a.rowf != nullptr;
   a.ldg = p.ldg;
   a.g_rows = p.g_rows;
   for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
@@ -857,11 +861,11 @@ int lx_args(const pg_linear_xent_desc_t* d, LxArgs* a) {
   const int rc = lx_check(d->n, d->K, d->C, d->dtype);
   if (rc != PG_OK) return rc;
   if ((d->h_stride < d->K && d->h_stride != 0) || d->w_stride < d->K) return PG_ERR_INVALID;
-  if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->lse || !d->flag || !d->scratch))) return PG_ERR_INVALID;
+  if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->top || !d->sum || !d->scratch))) return PG_ERR_INVALID;
   *a = LxArgs{};
   a->bias = d->bias; a->labels = d->labels;
   a->n = d->n; a->K = d->K; a->Kp = up(d->K, kPad); a->C = d->C; a->ignore = d->ignore_index;
-  a->lse = d->lse; a->flag = d->flag; a->meta = d->meta;
+  a->top = d->top; a->sum = d->sum; a->meta = d->meta;
   return PG_OK;
 }
 
@@ -897,7 +901,7 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
     if (rc != PG_OK) return rc;
   }
   if (!rows) {
-    hipLaunchKernelGGL(k_lx_mean, dim3(1), dim3(1024), 0, st, a.row_loss, a.flag, a.n, d->reduction == PG_XENT_MEAN ? 1 : 0, d->loss, a.meta);
+    hipLaunchKernelGGL(k_lx_mean, dim3(1), dim3(1024), 0, st, a.row_loss, a.sum, a.n, d->reduction == PG_XENT_MEAN ? 1 : 0, d->loss, a.meta);
     PG_LAUNCH_CHECK();
   }
   return PG_OK;
@@ -916,12 +920,11 @@ int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   if (d->reduction == PG_XENT_NONE) {
     float* rowf = (float*)s;
     float* top = (float*)(s + up(4 * a.n, 256));
-    hipLaunchKernelGGL(k_lx_row_factors, dim3(1), dim3(1024), 0, st, d->grad, d->grad_stride, a.flag, a.n, rowf, top);
+    hipLaunchKernelGGL(k_lx_row_factors, dim3(1), dim3(1024), 0, st, d->grad, d->grad_stride, a.sum, a.n, rowf, top);
     PG_LAUNCH_CHECK();
     a.rowf = rowf;
     a.f1 = top;
   } else {
-    a.rowf = a.flag;
     a.f1 = d->grad;
     a.f2 = d->reduction == PG_XENT_MEAN ? a.meta : nullptr;
   }

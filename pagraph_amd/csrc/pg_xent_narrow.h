@@ -27,8 +27,9 @@ struct NxArgs {
   const void *x, *y;               // parts of rows of KP elements
   int64_t x_ld, x_part, x_rows, y_ld, y_part, y_rows;
   int64_t nx, ny, K;               // rows that count
-  const float *side0, *side1, *side2;      // per y: STATS, DH: bias (base 2); DW: lse, labels, row factors. Padded past ny
-  const float *xa, *xb;            // per x: DH: lse, row factor; DW: bias (base 2)
+  const float *side0, *side1, *side2, *side3;      // per y: STATS, DH: bias (base 2); DW: largest logits, labels, row factors, inverse
+                                   // sums. Padded past ny
+  const float *xa, *xi, *xb;       // per x: DH: largest logit, inverse sum, row factor; DW: bias (base 2)
   const int32_t* xlab;             // per x: STATS, DH: labels (-1: none)
   float2* part;                    // STATS: [x][splits]
   float* zlab;
@@ -96,7 +97,7 @@ struct NarrowState {
   s16x8 xf[XB][N::KK][N::NP];
   f32x16 out[MODE == NX_STATS ? 1 : N::KB][XB];
   float m[XB], s[XB];                      // STATS: running maximum, sum; DW: s = column sum of G
-  float xa[XB];
+  float xa[XB], xi[XB];
   int xl[XB];                              // STATS, DH: the lane's label; DW: the lane's class
   float zl[XB];
 };
@@ -123,7 +124,8 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
       __builtin_amdgcn_global_load_lds((glb_void*)(a.side0 + y_next + lane), (lds_void*)side_next, 4, 0, 0);
       if constexpr (MODE == NX_DW) {
         __builtin_amdgcn_global_load_lds((glb_void*)(a.side1 + y_next + lane), (lds_void*)(side_next + 64), 4, 0, 0);
-        if (a.scaled) __builtin_amdgcn_global_load_lds((glb_void*)(a.side2 + y_next + lane), (lds_void*)(side_next + 128), 4, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void*)(a.side3 + y_next + lane), (lds_void*)(side_next + 128), 4, 0, 0);
+        if (a.scaled) __builtin_amdgcn_global_load_lds((glb_void*)(a.side2 + y_next + lane), (lds_void*)(side_next + 192), 4, 0, 0);
       }
     }
   }
@@ -169,7 +171,7 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
       } else {
         if constexpr (MODE == NX_DH) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) z[b][e] = __builtin_amdgcn_exp2f(fmaf(z[b][e], L2E, sv[e]) - st.xa[b]);
+          for (int e = 0; e < 16; ++e) z[b][e] = __builtin_amdgcn_exp2f(fmaf(z[b][e], L2E, sv[e]) - st.xa[b]) * st.xi[b];
           const int at = st.xl[b] - (int)(y0 + yb * 32) - h4;
           if (__any((unsigned)at < 32u)) {
 #pragma unroll
@@ -177,7 +179,13 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) z[b][e] = __builtin_amdgcn_exp2f(fmaf(z[b][e], L2E, st.xa[b]) - sv[e]);
+          for (int q = 0; q < 4; ++q) {
+            const float4 v = *reinterpret_cast<const float4*>(side + 128 + yb * 32 + 8 * q + h4);
+            const float inv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              z[b][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(z[b][4 * q + e], L2E, st.xa[b]) - sv[4 * q + e]) * inv[e];
+          }
           // the wave's classes are 32 in a row: does any of the block's rows have one of them as its label?
           const int* lab = reinterpret_cast<const int*>(side + 64) + yb * 32;
           if (__any((unsigned)(lab[lane & 31] - (st.xl[b] - (lane & 31))) < 32u)) {
@@ -187,7 +195,7 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
           if (a.scaled) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float f = side[128 + yb * 32 + 8 * (e / 4) + h4 + e % 4];
+              const float f = side[192 + yb * 32 + 8 * (e / 4) + h4 + e % 4];
               z[b][e] = f == 0.f ? 0.f : z[b][e] * f;
             }
           }
@@ -228,7 +236,7 @@ template <typename T, int KP, int XB, int MODE>
 __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
   typedef Narrow<T, KP, XB> N;
   __shared__ __align__(16) short buf[2 * N::TILE];
-  __shared__ __align__(16) float side[2 * 192];
+  __shared__ __align__(16) float side[2 * 256];
   const uint32_t x_tiles = (uint32_t)ceil_div<int64_t>(a.nx, N::XT), t = xcd_run(blockIdx.x, gridDim.x);
   const int64_t xt = uniform((int)(t % x_tiles));
   const int sp = uniform((int)(t / x_tiles));              // an XCD's workgroups walk the same y at the same time
@@ -254,6 +262,7 @@ __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
     } else if constexpr (MODE == NX_DH) {
       const bool counts = in && a.xb[x[b]] != 0.f;
       st.xa[b] = counts ? a.xa[x[b]] : INFINITY;           // rows that do not count: every exponential is 0
+      st.xi[b] = counts ? a.xi[x[b]] : 0.f;
       st.xl[b] = counts ? a.xlab[x[b]] : -1;
     } else {
       st.xa[b] = a.xa[x[b]];                               // (padded past the last class)
@@ -281,15 +290,16 @@ __global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
       __builtin_amdgcn_global_load_lds((glb_void*)(a.side0 + y_lo + lane), (lds_void*)side, 4, 0, 0);
       if constexpr (MODE == NX_DW) {
         __builtin_amdgcn_global_load_lds((glb_void*)(a.side1 + y_lo + lane), (lds_void*)(side + 64), 4, 0, 0);
-        if (a.scaled) __builtin_amdgcn_global_load_lds((glb_void*)(a.side2 + y_lo + lane), (lds_void*)(side + 128), 4, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_void*)(a.side3 + y_lo + lane), (lds_void*)(side + 128), 4, 0, 0);
+        if (a.scaled) __builtin_amdgcn_global_load_lds((glb_void*)(a.side2 + y_lo + lane), (lds_void*)(side + 192), 4, 0, 0);
       }
     }
     for (int64_t y = y_lo; y < y_hi; y += 2 * N::YT) {
       next_tile();
-      nx_step<T, KP, XB, MODE>(buf, side, buf + N::TILE, side + 192, y + N::YT < y_hi, a, y, y + N::YT, wave, lane, st);
+      nx_step<T, KP, XB, MODE>(buf, side, buf + N::TILE, side + 256, y + N::YT < y_hi, a, y, y + N::YT, wave, lane, st);
       if (y + N::YT < y_hi) {
         next_tile();
-        nx_step<T, KP, XB, MODE>(buf + N::TILE, side + 192, buf, side, y + 2 * N::YT < y_hi, a, y + N::YT, y + 2 * N::YT, wave, lane, st);
+        nx_step<T, KP, XB, MODE>(buf + N::TILE, side + 256, buf, side, y + 2 * N::YT < y_hi, a, y + N::YT, y + 2 * N::YT, wave, lane, st);
       }
     }
   }

@@ -1099,7 +1099,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dev, t = h.device, _DTYPES[h.dtype]
         each = reduction == L.PG_XENT_NONE
         loss = torch.empty(h.shape[:-1] if each else (), dtype=torch.float32, device=dev)
-        stats = torch.empty(2 * n + 1, dtype=torch.float32, device=dev)           # lse | counted? | 1 / #counted
+        stats = torch.empty(2 * n + 1, dtype=torch.float32, device=dev)           # largest logits | sums | 1 / #counted
         size = L.load().pg_linear_xent_scratch(n, K, C, t, 0)
         if size < 0:
             raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")

@@ -31,3 +31,35 @@ def test_rows_in_another_order_give_the_same_values(dev, hiplib, n, K, C, t):
     for k in range(4):
         order = torch.randperm(n, generator=g, device=dev)
         assert all(torch.equal(a, b[order]) for a, b in zip(values(order), want)), k
+
+
+# ---- masks of the type's lowest value ----------------------------------------------------------------------------------------
+@gpu
+@TYPES
+@pytest.mark.parametrize("K,n,C", [(24, 70, 520), (300, 70, 520), (300, 2100, 7000)])
+def test_a_head_of_nothing_but_masked_classes_is_uniform(dev, hiplib, K, n, C, t):
+    """every class masked by the type's lowest value: no logit is larger than another, so each class has one C-th (beside the lowest
+    value of fp32 and bf16 any h W is lost, in fp16 it is not: its weight is 0)"""
+    from pagraph_amd import ops
+    g = gen(71, dev)
+    lin = head(dev, K, C, t, g)
+    with torch.no_grad():
+        lin.bias.fill_(torch.finfo(t).min)
+        if t == F16:
+            lin.weight.zero_()
+    h = torch.randn(n, K, generator=g, device=dev).to(t).requires_grad_()
+    lab = torch.randint(0, C, (n,), generator=g, device=dev)
+    each = ops.linear_cross_entropy(h, lin, lab, reduction="none")
+    want = torch.full((n,), float(C), dtype=torch.float64, device=dev).log()
+    # log2 of a whole number times ln 2: three roundings
+    assert ((each.double() - want).abs() <= 4 * 2.0 ** -24 * want).all()
+    dh, dw, db = torch.autograd.grad(each.sum(), [h, lin.weight, lin.bias])
+    G = torch.full((n, C), 1.0 / C, dtype=torch.float64, device=dev)
+    G.scatter_add_(1, lab.view(-1, 1), torch.full((n, 1), -1.0, dtype=torch.float64, device=dev))
+    W, H = lin.weight.detach().double(), h.detach().double()
+    # an element of G is off by its rounding to t (fp32: a few roundings), a sum by one rounding an addition, a result by half a step
+    eg = torch.finfo(t).eps / 2 + 8 * 2.0 ** -24
+    half, least = torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal
+    for got, ref, size, adds in ((dh, G @ W, G.abs() @ W.abs(), C), (dw, G.t() @ H, G.abs().t() @ H.abs(), n), (db, G.sum(0), G.abs().sum(0), n)):
+        bound = size * (eg + (adds + 32) * 2.0 ** -24) + half * ref.abs() * 1.01 + least
+        assert ((got.double() - ref).abs() <= bound).all()
