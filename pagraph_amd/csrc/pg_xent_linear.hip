@@ -20,7 +20,8 @@
 
 namespace pg {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
+constexpr float kLowest = -3.402823466e38f;                // what a finite logit is at least, in base 2
 
 // how an operand type is multiplied: the parts' type and number, G's scale
 template <typename T> struct Mul;
@@ -83,7 +84,7 @@ __device__ __forceinline__ void lx_side(const SideArgs& a) {
       if (i < a.C && a.bias) {
         b = (float)((const T*)a.bias)[i];
         // (a finite lowest value stays finite: a row of nothing else is uniform, as in natural units)
-        b = b == -INFINITY ? b : b * kLog2e < -3.402823466e38f ? -3.402823466e38f : b * kLog2e;
+        b = b == -INFINITY ? b : b * kLog2e < kLowest ? kLowest : b * kLog2e;
       }
       a.bias2[i] = b;
     }
@@ -306,6 +307,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
 }
 
 // a wave per row: joins the tiles' (narrow form: the splits') statistics, in base 2
+template <typename T>
 __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
@@ -328,7 +330,15 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
     const bool ok = label_ok(a.labels[r], a);
     a.top[r] = m;
     a.sum[r] = !ok ? 0.f : s > 0.f ? s : NAN;               // (a row of nothing but -inf counts, and its loss is NaN)
-    a.row_loss[r] = ok ? ((m - a.zlab[r]) + log2f(s)) * 0.693147180559945309417f : 0.f;
+    float loss = 0.f;
+    if (ok) {
+      const float z = a.zlab[r];
+      loss = ((m - z) + log2f(s)) * kLn2;
+      // the label's own class is masked by a finite bias that base 2 cannot hold (lx_side), another class is not: beside such a
+      // bias h W is lost, the logit is the bias
+      if (z == kLowest && m > kLowest) loss = (m + log2f(s)) * kLn2 - (float)((const T*)a.bias)[a.labels[r]];
+    }
+    a.row_loss[r] = loss;
   }
 }
 
@@ -703,7 +713,7 @@ int narrow_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, c
   rc = launch_narrow<T, NX_STATS>(n, p, st);
   if (rc != PG_OK) return rc;
   a.tiles = p.nx_stats;
-  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_lx_rows<T>, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }
@@ -771,7 +781,7 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   const dim3 grid((unsigned)(p.tiles * p.row_tiles));
   lx_launch_logits<T, false>(a, p, grid, st);
   PG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_lx_rows, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(k_lx_rows<T>, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
   PG_LAUNCH_CHECK();
   return PG_OK;
 }

@@ -63,3 +63,29 @@ def test_a_head_of_nothing_but_masked_classes_is_uniform(dev, hiplib, K, n, C, t
     for got, ref, size, adds in ((dh, G @ W, G.abs() @ W.abs(), C), (dw, G.t() @ H, G.abs().t() @ H.abs(), n), (db, G.sum(0), G.abs().sum(0), n)):
         bound = size * (eg + (adds + 32) * 2.0 ** -24) + half * ref.abs() * 1.01 + least
         assert ((got.double() - ref).abs() <= bound).all()
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("K", [24, 300])
+def test_a_label_whose_class_is_masked_by_the_lowest_value(dev, hiplib, K, t):
+    """its loss is the mask's size, finite as in natural units, and its row pulls the masked class alone"""
+    from pagraph_amd import ops
+    g = gen(72, dev)
+    n, C = 60, 400
+    lin = head(dev, K, C, t, g)
+    low = torch.finfo(t).min
+    with torch.no_grad():
+        lin.bias[100:130] = low
+    h = torch.randn(n, K, generator=g, device=dev).to(t).requires_grad_()
+    lab = torch.randint(130, C, (n,), generator=g, device=dev)
+    lab[::4] = 107
+    each = ops.linear_cross_entropy(h, lin, lab, reduction="none")
+    z = h.detach().double() @ lin.weight.detach().double().t() + lin.bias.detach().double()
+    want = torch.logsumexp(z, 1) - z.gather(1, lab.view(-1, 1)).view(-1)
+    # logits of some 2 sqrt(K) at most beside the mask: (K + 16) roundings of a sum of absolute products, some of the mask's own size
+    mag = (h.detach().double().abs() @ lin.weight.detach().double().abs().t()).amax(1) + 2.0
+    bound = (2 * (K + 16) * mag + 400) * 2.0 ** -24 + torch.where(lab == 107, 16 * 2.0 ** -24 * abs(low), 0.0)
+    assert ((each.double() - want).abs() <= bound).all()
+    db, = torch.autograd.grad(each.sum(), lin.bias)
+    assert db[107] == -15 and (db[100:107] == 0).all() and (db[108:130] == 0).all()
