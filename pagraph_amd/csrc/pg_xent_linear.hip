@@ -201,7 +201,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
     for (int j = 0; j < S::FJ; ++j) {
       if constexpr (PIECE) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(acc[i][j][e] - top[j]) * inv[j];
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = lx_exp(acc[i][j][e] - top[j]) * inv[j];
       }
       if (__any((unsigned)(at[j] - 32 * i) < 32u)) {         // does any of the wave's rows have its label among these 32 classes?
 #pragma unroll

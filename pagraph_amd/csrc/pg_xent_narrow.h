@@ -42,6 +42,11 @@ struct NxArgs {
 
 template <typename T> struct Mul;      // pg_xent_linear.hip
 
+// 2^v of a logit less its row's largest one. A row without a gradient (ignored, or behind the last one) has the inverse sum 0 and
+// must not reach dW with the NaN that an infinite weight makes of its zeros: the smaller of NaN and 0 is 0. In rows that count, the
+// inverse sum itself is NaN then
+__device__ __forceinline__ float lx_exp(float v) { return __builtin_amdgcn_exp2f(fminf(v, 0.f)); }
+
 // 32-row blocks a wave keeps: two where the registers allow, each read of the other side's tile then feeds two products. Not in
 // fp32: its six products a read keep the matrix units busy, and two blocks leave two waves of three (6000 x 64 -> 50000 with
 // gradients 1244 against 1080 us)
@@ -184,7 +189,7 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
             const float inv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              z[b][4 * q + e] = __builtin_amdgcn_exp2f(fmaf(z[b][4 * q + e], L2E, st.xa[b]) - sv[4 * q + e]) * inv[e];
+              z[b][4 * q + e] = lx_exp(fmaf(z[b][4 * q + e], L2E, st.xa[b]) - sv[4 * q + e]) * inv[e];
           }
           // the wave's classes are 32 in a row: does any of the block's rows have one of them as its label?
           const int* lab = reinterpret_cast<const int*>(side + 64) + yb * 32;

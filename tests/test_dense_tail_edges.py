@@ -89,3 +89,30 @@ def test_a_label_whose_class_is_masked_by_the_lowest_value(dev, hiplib, K, t):
     assert ((each.double() - want).abs() <= bound).all()
     db, = torch.autograd.grad(each.sum(), lin.bias)
     assert db[107] == -15 and (db[100:107] == 0).all() and (db[108:130] == 0).all()
+
+
+# ---- infinite weights ----------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("K,n,C", [(40, 67, 400), (64, 128, 400), (300, 67, 400), (256, 1100, 9000)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_class_taken_out_by_infinite_weights(dev, hiplib, reduction, K, n, C, t):
+    """a class whose weights are -inf where h is positive has the logit -inf: the rest of the head is as without it, and rows that do
+    not count (ignored ones, and those a tile has behind the last row) bring no NaN into the head's gradients"""
+    from pagraph_amd import ops
+    g = gen(73, dev)
+    lin = head(dev, K, C, t, g)
+    h = (torch.rand(n, K, generator=g, device=dev) + 0.5).to(t)
+    lab = torch.randint(10, C, (n,), generator=g, device=dev)
+    lab[::5] = -100
+    h[::5] = 0.0
+    up = torch.randn(n, generator=g, device=dev) if reduction == "none" else torch.ones((), device=dev)
+    out = []
+    for by_weight in (True, False):
+        with torch.no_grad():
+            lin.bias[3] = 0.5 if by_weight else float("-inf")
+            lin.weight[3] = float("-inf") if by_weight else 0.0
+        loss = ops.linear_cross_entropy(h, lin, lab, reduction=reduction)
+        out.append([loss.detach()] + list(torch.autograd.grad(loss, [lin.weight, lin.bias], up)))
+    assert all(torch.isfinite(v).all() for v in out[0])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
