@@ -46,7 +46,7 @@ struct LxArgs {
   float* dbp;                              // [row tiles][C] partial sums of G
   const float *bias2, *top2, *inv2, *rowf2;        // side arrays (SideArgs)
   const int32_t* lab2;
-  int32_t scaled;
+  int32_t scaled, late;                    // G carries the row factors; dh's rows get them behind the product
   void *dh, *dw, *db;
   int64_t range;                           // reduction range of one split
   int32_t splits, first, direct;           // direct: one split and one piece, the product itself is the output
@@ -435,14 +435,31 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dh(LxArgs a) {
   }
   mm_product<S, ROWS, COLS>(Operand{a.g, a.ldg, a.g_rows * a.ldg, r0, a.g_rows, 0},
                             Operand{(const short*)a.w + a.c_lo * a.w_ld, a.w_ld, a.w_part, n0, 0, a.Kp}, lo, hi, buf, acc);
-  // (rows that do not count leave as zeros, whatever W holds)
-  if (a.direct) {
-    const float f = out_factor(a) / Mul<T>::G;
-    T* out = (T*)a.dh + r0 * a.K + n0;
-    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { out[r * a.K + k] = a.rowf2[r0 + r] == 0.f ? (T)0.f : (T)(v * f); });
-  } else {
-    each_output<S>(acc, rl, kl, rows, cols, [&](int r, int k, float v) { sum[r * a.K + k] = a.rowf2[r0 + r] == 0.f ? 0.f : v; });
-  }
+  // (rows that do not count leave as zeros, whatever W holds; the row factors are padded to whole tiles)
+  const float f = a.direct ? out_factor(a) / Mul<T>::G : 1.f;
+  const bool late = a.late && a.c_hi == a.C;               // behind the last piece's share
+  T* out = (T*)a.dh + r0 * a.K + n0;
+#pragma unroll
+  for (int i = 0; i < S::FI; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 v4 = *reinterpret_cast<const float4*>(a.rowf2 + r0 + rl + i * 32 + 8 * q);
+      const float rf[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rl + i * 32 + 8 * q + e;
+        if (r >= rows) continue;
+        const float fr = late ? rf[e] * f : f;
+#pragma unroll
+        for (int j = 0; j < S::FJ; ++j) {
+          const int k = kl + 32 * j;
+          if (k >= cols) continue;
+          const float v = rf[e] == 0.f ? 0.f : acc[i][j][4 * q + e] * fr;
+          if (a.direct) out[r * a.K + k] = (T)v;
+          else sum[r * a.K + k] = v;
+        }
+      }
+    }
 }
 
 // partial sums added in order: out[i] = (sum over splits of acc[split][i]) * factor. Up to three such sums a launch
@@ -801,30 +818,31 @@ int lx_launch_dw(const LxArgs& a, hipStream_t st) {
   return PG_OK;
 }
 
-// one piece's share of the gradients
+// one piece's G, and its share of the gradients
 template <typename T>
-int lx_gradients(LxArgs& a, const LxPlan& p, float* acc_dh, float* acc_dw, hipStream_t st) {
-  if (a.dh) {
-    a.acc = acc_dh;
-    a.splits = p.dh_splits;
-    a.range = p.dh_range;
-    a.first = a.c_lo == 0;
-    a.direct = p.dh_splits == 1 && p.pieces == 1;
-    const int rc = p.dh == BIG ? lx_launch_dh<T, BigTile<T>>(a, st) : p.dh == TALL ? lx_launch_dh<T, TallTile<T>>(a, st)
-                                                                                                          : lx_launch_dh<T, MidTile<T>>(a, st);
-    if (rc != PG_OK) return rc;
-  }
-  if (a.dw) {
-    a.acc = acc_dw;
-    a.splits = p.dw_splits;
-    a.range = p.dw_range;
-    const int rc = p.dw == BIG ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw == TALL ? lx_launch_dw<T, TallTile<T>>(a, st)
-                                                                                                          : lx_launch_dw<T, MidTile<T>>(a, st);
-    if (rc != PG_OK) return rc;
-    if (a.splits > 1 && p.pieces > 1)
-      return lx_sums<T>(SumArgs{acc_dw, (T*)a.dw + a.c_lo * a.K, (a.c_hi - a.c_lo) * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
-  }
+int lx_piece(const LxArgs& a, const LxPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(ceil_div<int64_t>(a.c_hi - a.c_lo, p.logits == MID ? 128 : 256) * p.row_tiles));
+  lx_launch_logits<T, true>(a, p, grid, st);
+  PG_LAUNCH_CHECK();
   return PG_OK;
+}
+template <typename T>
+int lx_piece_dh(LxArgs& a, const LxPlan& p, float* acc, hipStream_t st) {
+  a.acc = acc;
+  a.splits = p.dh_splits;
+  a.range = p.dh_range;
+  a.first = a.c_lo == 0;
+  a.direct = p.dh_splits == 1 && p.pieces == 1;
+  return p.dh == BIG ? lx_launch_dh<T, BigTile<T>>(a, st) : p.dh == TALL ? lx_launch_dh<T, TallTile<T>>(a, st) : lx_launch_dh<T, MidTile<T>>(a, st);
+}
+template <typename T>
+int lx_piece_dw(LxArgs& a, const LxPlan& p, float* acc, hipStream_t st) {
+  a.acc = acc;
+  a.splits = p.dw_splits;
+  a.range = p.dw_range;
+  const int rc = p.dw == BIG ? lx_launch_dw<T, BigTile<T>>(a, st) : p.dw == TALL ? lx_launch_dw<T, TallTile<T>>(a, st) : lx_launch_dw<T, MidTile<T>>(a, st);
+  if (rc != PG_OK || a.splits == 1 || p.pieces == 1) return rc;
+  return lx_sums<T>(SumArgs{acc, (T*)a.dw + a.c_lo * a.K, (a.c_hi - a.c_lo) * a.K, a.splits}, SumArgs{}, SumArgs{}, a, st);
 }
 
 template <typename T>
@@ -842,16 +860,30 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
   int rc = lx_operands<T>(a, d, p, s, s + p.h_bytes, true, side, st);
   if (rc != PG_OK) return rc;
   a.bias2 = side.bias2; a.lab2 = side.lab; a.top2 = side.top2; a.inv2 = side.inv2; a.rowf2 = side.rowf2;
-  a.scaled = a.rowf != nullptr;
   a.ldg = p.ldg;
   a.g_rows = p.g_rows;
+  // Rows with factors of their own in fp16: below 2^-14 of the largest one, G times its factor begins to leave the type's range, and
+  // dh, which has the row to itself, would lose those bits. Its G carries no factors, its rows get them behind the product. dW and
+  // db sum over the rows, largest ones beside them: their G carries the factors, and is made a second time where both are wanted
+  const bool scaled = a.rowf != nullptr, head = a.dw || a.db;
+  a.late = scaled && Mul<T>::G != 1.f;
   for (a.c_lo = 0; a.c_lo < a.C; a.c_lo = a.c_hi) {
     a.c_hi = a.c_lo + p.piece < a.C ? a.c_lo + p.piece : a.C;
-    const dim3 grid((unsigned)(ceil_div<int64_t>(a.c_hi - a.c_lo, p.logits == MID ? 128 : 256) * p.row_tiles));
-    lx_launch_logits<T, true>(a, p, grid, st);
-    PG_LAUNCH_CHECK();
-    rc = lx_gradients<T>(a, p, acc_dh, acc_dw, st);
-    if (rc != PG_OK) return rc;
+    if (a.dh) {
+      a.scaled = scaled && !a.late;
+      rc = lx_piece<T>(a, p, st);
+      if (rc == PG_OK) rc = lx_piece_dh<T>(a, p, acc_dh, st);
+      if (rc != PG_OK) return rc;
+    }
+    if (head && (!a.dh || a.late)) {
+      a.scaled = scaled;
+      rc = lx_piece<T>(a, p, st);
+      if (rc != PG_OK) return rc;
+    }
+    if (a.dw) {
+      rc = lx_piece_dw<T>(a, p, acc_dw, st);
+      if (rc != PG_OK) return rc;
+    }
   }
   const bool direct = p.dh_splits == 1 && p.pieces == 1;
   return lx_sums<T>(SumArgs{acc_dh, direct ? nullptr : a.dh, a.n * a.K, p.dh_splits}, SumArgs{a.dbp, a.db, a.C, p.row_tiles},

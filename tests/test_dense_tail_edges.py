@@ -116,3 +116,35 @@ def test_a_class_taken_out_by_infinite_weights(dev, hiplib, reduction, K, n, C, 
         out.append([loss.detach()] + list(torch.autograd.grad(loss, [lin.weight, lin.bias], up)))
     assert all(torch.isfinite(v).all() for v in out[0])
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+# ---- gradients of single rows far apart ----------------------------------------------------------------------------------------
+@gpu
+@TYPES
+@pytest.mark.parametrize("n,K,C", [(61, 40, 512), (61, 300, 512), (2100, 300, 7000), (2100, 800, 7000)])
+def test_rows_whose_gradients_are_far_below_the_largest(dev, hiplib, n, K, C, t):
+    """a row's gradient is as exact however large another row's is. h is orthogonal to every class: all probabilities are 1 / C, a
+    rounding of them that is the same for all would show in dh = up * (mean of W's rows - W[label])"""
+    from pagraph_amd import ops
+    g = gen(74, dev)
+    lin = head(dev, K, C, t, g)
+    with torch.no_grad():
+        lin.weight.copy_(1.0 + (torch.arange(C, device=dev) % 2).to(t).view(C, 1) * torch.ones(K, device=dev, dtype=t))        # rows of 1, of 2
+        lin.bias.zero_()
+    h = torch.tensor([1.0, -1.0], device=dev).repeat(n, K // 2).to(t).requires_grad_()
+    lab = torch.randint(0, C, (n,), generator=g, device=dev)
+    # (exponents that leave dh, of fp16 too, its normal range: 2^13 to 2^-13 times 1/2)
+    up = torch.exp2(13.0 - 26.0 * torch.rand(n, generator=g, device=dev))
+    up[0] = 2.0 ** 13
+    dh, db = torch.autograd.grad(ops.linear_cross_entropy(h, lin, lab, reduction="none"), [h, lin.bias], up)
+    own = lin.weight.detach().double()[lab, 0]
+    want = up.double() * (1.5 - own)
+    # an element of G is off by half a step of its type (fp32: a few roundings): C of 1 / C with weights of 1.5 on average, and the
+    # label's 1 / C - 1 with its weight, that is 1.5 + own in all; C additions; the result's own half step
+    half = torch.finfo(t).eps / 2
+    bound = up.double() * (1.5 + own) * ((half if t != F32 else 8 * 2.0 ** -24) + (C + 32) * 2.0 ** -24) + half * want.abs() * 1.01 + 2.0 ** -25
+    assert ((dh.double() - want.view(n, 1)).abs() <= bound.view(n, 1)).all()
+    G = (up.double() / C).sum() - torch.zeros(C, dtype=torch.float64, device=dev).index_add_(0, lab, up.double())
+    # (a sum over the rows: half a step of G's type of each, fp16 G's smallest step 2^-24 of the largest row times 2^14)
+    eb = (up.double().sum() + up.double().sum() / C) * (half + (n + 40) * 2.0 ** -24) + n * 2.0 ** 13 * 2.0 ** -38
+    assert ((db.double() - G).abs() <= eb + half * G.abs() * 1.01).all()
