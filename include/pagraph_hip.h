@@ -630,7 +630,8 @@ int64_t pg_layer_norm_scratch(int64_t n, int64_t d, int32_t dtype);
 int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
 /* CrossEntropyLoss(h W^T + bias, labels) for any number of classes without the logits [n, C] in memory (a wide head's counterpart
  * of pg_head + pg_xent_*): h [n, K], W [C, K], bias [C] or NULL, all of `dtype`. Rows whose label is ignore_index or outside
- * [0, C) are not counted, have loss 0 and gradient 0, and do not enter dW / db whatever h holds there.
+ * [0, C) are not counted, have loss 0 and gradient 0, and do not enter dW / db whatever h holds there. In fp32 (three bf16 parts a
+ * value) an infinite element of h or W makes NaN of every logit it enters, also where the product itself would be infinite.
  * forward:  PG_XENT_MEAN / _SUM: *loss (nan for the mean when no row counts); PG_XENT_NONE: row_loss [n]. And what the backward
  *           pass reads: top [n], a row's largest logit times log2(e); sum [n], its sum of exponentials over that one (0: the row is not
  *           counted); meta [1] = 1 / #counted rows (0).

@@ -10,7 +10,7 @@
 // whole tiles: 16-bit rows that are so already are used in place, others are packed first (k_lx_pack). fp32 values are split
 // into three bf16 parts (x = x0 + x1 + x2 exactly, each at most 2^-8 of the one before) and six of the nine partial products are
 // summed; the three left out, x1 y2 + x2 y1 + x2 y2, are below 2^-22.9 of the product. 2.5 PF / 6 where the fp32 matrix
-// instructions reach 0.157 PF.
+// instructions reach 0.157 PF. An infinite element has parts that are NaN, and so are the logits it enters.
 // G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-8, fp16 2^-11 relative),
 // independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
 // of 2^-28 is still a normal number.
@@ -22,6 +22,7 @@ namespace pg {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kLowest = -3.402823466e38f;                // what a finite logit is at least, in base 2
+constexpr float kTopBf16 = 3.38953139e38f;                 // bf16's largest
 
 // how an operand type is multiplied: the parts' type and number, G's scale
 template <typename T> struct Mul;
@@ -144,6 +145,8 @@ __global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1, SideA
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           o[i] = (E)x[i];
+          // (a finite value above bf16's largest would round to infinity: its first part is the largest)
+          if (p == 0 && fabsf(x[i]) < INFINITY && fabsf((float)o[i]) == INFINITY) o[i] = (E)copysignf(kTopBf16, x[i]);
           x[i] -= (float)o[i];                       // exact
         }
         __builtin_memcpy(d + p * a.rows_p * a.ldp, o, sizeof(o));

@@ -1148,7 +1148,8 @@ def linear_cross_entropy(h, module, labels, ignore_index=-100, reduction="mean")
     any width, without the logits: h [..., K] (fp32, bf16 or fp16, the module's type), labels int64 of h's leading shape. Forward
     and backward walk the classes in pieces; the loss is fp32: the mean over the counted rows, their sum, or (reduction "none") one
     loss a row. As in ops.cross_entropy a label that is ignore_index or outside [0, C) is not counted: loss 0, no gradient,
-    whatever its row of h holds. Logits are held times log2(e), above 2.3e38 they are infinite; a bias of the type's lowest value masks
+    whatever its row of h holds. In fp32 an infinite element of h or the weight makes NaN of the logits it enters (mask a class by its
+    bias, which may be -inf). Logits are held times log2(e), above 2.3e38 they are infinite; a bias of the type's lowest value masks
     its class as it does there. Deterministic. Heads of <= 64 classes behind an aggregation: gcn_head / sage_head."""
     w, b = module.weight, module.bias
     _need_rows("linear_cross_entropy", h)

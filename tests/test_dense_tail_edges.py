@@ -148,3 +148,58 @@ def test_rows_whose_gradients_are_far_below_the_largest(dev, hiplib, n, K, C, t)
     # (a sum over the rows: half a step of G's type of each, fp16 G's smallest step 2^-24 of the largest row times 2^14)
     eb = (up.double().sum() + up.double().sum() / C) * (half + (n + 40) * 2.0 ** -24) + n * 2.0 ** 13 * 2.0 ** -38
     assert ((db.double() - G).abs() <= eb + half * G.abs() * 1.01).all()
+
+
+# ---- the ends of fp32 ----------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("K", [8, 300])
+@pytest.mark.parametrize("big", [3.4e38, -3.4028234e38, 3.3895e38, 3.392e38])
+def test_fp32_values_above_the_largest_of_bf16(dev, hiplib, K, big):
+    """fp32 is multiplied in three bf16 parts; a finite value whose rounding to bf16 is infinite is finite all the same, in h and in
+    the head. Weights of whole numbers times 2^-124 have one part, logits are some 16 times those numbers"""
+    from pagraph_amd import ops
+    g = gen(75, dev)
+    n, C = 50, 200
+    lin = head(dev, K, C, F32, g, bias=False)
+    h = torch.zeros(n, K, device=dev)
+    h[:, 0] = big
+    with torch.no_grad():
+        lin.weight.zero_()
+        lin.weight[:, 0] = torch.randint(-8, 9, (C,), generator=g, device=dev).float() * 2.0 ** -124
+    lab = torch.randint(0, C, (n,), generator=g, device=dev)
+    for x, m in ((h, lin), (lin.weight.detach()[:n] * 1.0, torch.nn.Linear(K, C, bias=False, device=dev))):
+        if m is not lin:
+            with torch.no_grad():
+                m.weight.zero_()
+                m.weight[:, 0] = big
+                m.weight[::2, 0] *= 0.5
+        x = x.detach().requires_grad_()
+        each = ops.linear_cross_entropy(x, m, lab, reduction="none")
+        z = x.detach().double() @ m.weight.detach().double().t()
+        want = torch.logsumexp(z, 1) - z.gather(1, lab.view(-1, 1)).view(-1)
+        # |z| <= 128: one product of three parts, the logit's rounding in base 2, the sum's; 400 as everywhere for the exponentials
+        assert ((each.double() - want).abs() <= (8 * 128 + 400) * 2.0 ** -24).all()
+        dx, = torch.autograd.grad(each.sum(), x)
+        assert torch.isfinite(dx).all()
+
+
+@gpu
+@pytest.mark.parametrize("K", [40, 300])
+def test_fp32_infinities_stay_with_their_rows(dev, hiplib, K):
+    """an infinite element of a row makes that row's loss NaN and no other's"""
+    from pagraph_amd import ops
+    g = gen(76, dev)
+    lin = head(dev, K, 500, F32, g)
+    h = torch.randn(90, K, generator=g, device=dev)
+    lab = torch.randint(0, 500, (90,), generator=g, device=dev)
+    bad = h.clone()
+    bad[11, 3], bad[64, K - 1] = float("inf"), float("-inf")
+    rest = torch.ones(90, dtype=torch.bool, device=dev)
+    rest[11], rest[64] = False, False
+    out = []
+    for x in (h, bad):
+        x = x.requires_grad_()
+        each = ops.linear_cross_entropy(x, lin, lab, reduction="none")
+        out.append((each.detach(), torch.autograd.grad(each.sum(), x)[0]))
+    assert all(torch.equal(a[rest], b[rest]) for a, b in zip(*out))
+    assert torch.isnan(out[1][0][~rest]).all() and torch.isnan(out[1][1][~rest]).all()
