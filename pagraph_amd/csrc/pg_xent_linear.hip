@@ -313,36 +313,43 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-  if (r >= a.n) return;
-  float m = -INFINITY, s = 0.f;
-  for (int64_t t = lane; t < a.tiles; t += 64) {
-    const float2 x = a.part[r * a.tiles + t];
-    const float mm = fmaxf(m, x.x), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
-    m = mm;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float om = __shfl_xor(m, o, kWave), os = __shfl_xor(s, o, kWave);
-    const float mm = fmaxf(m, om), base = mm == -INFINITY ? 0.f : mm;
-    s = s * __builtin_amdgcn_exp2f(m - base) + os * __builtin_amdgcn_exp2f(om - base);
-    m = mm;
-  }
-  if (lane == 0) {
-    const bool ok = label_ok(a.labels[r], a);
-    a.top[r] = m;
-    a.sum[r] = !ok ? 0.f : s > 0.f ? s : NAN;               // (a row of nothing but -inf counts, and its loss is NaN)
-    float loss = 0.f;
-    if (ok) {
-      const float z = a.zlab[r];
-      loss = ((m - z) + log2f(s)) * kLn2;
-      // the label's own class is masked by a finite bias that base 2 cannot hold (lx_side), another class is not: beside such a
-      // bias h W is lost, the logit is the bias
-      if (z == kLowest && m > kLowest) loss = (m + log2f(s)) * kLn2 - (float)((const T*)a.bias)[a.labels[r]];
+  for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; r < a.n; r += (int64_t)gridDim.x * 4) {
+    float m = -INFINITY, s = 0.f;
+    for (int64_t t = lane; t < a.tiles; t += 64) {
+      const float2 x = a.part[r * a.tiles + t];
+      const float mm = fmaxf(m, x.x), base = mm == -INFINITY ? 0.f : mm;
+      s = s * __builtin_amdgcn_exp2f(m - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+      m = mm;
     }
-    a.row_loss[r] = loss;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const float om = __shfl_xor(m, o, kWave), os = __shfl_xor(s, o, kWave);
+      const float mm = fmaxf(m, om), base = mm == -INFINITY ? 0.f : mm;
+      s = s * __builtin_amdgcn_exp2f(m - base) + os * __builtin_amdgcn_exp2f(om - base);
+      m = mm;
+    }
+    if (lane == 0) {
+      const bool ok = label_ok(a.labels[r], a);
+      a.top[r] = m;
+      a.sum[r] = !ok ? 0.f : s > 0.f ? s : NAN;             // (a row of nothing but -inf counts, and its loss is NaN)
+      float loss = 0.f;
+      if (ok) {
+        const float z = a.zlab[r];
+        loss = ((m - z) + log2f(s)) * kLn2;
+        // the label's own class is masked by a finite bias that base 2 cannot hold (lx_side), another class is not: beside such a
+        // bias h W is lost, the logit is the bias
+        if (z == kLowest && m > kLowest) loss = (m + log2f(s)) * kLn2 - (float)((const T*)a.bias)[a.labels[r]];
+      }
+      a.row_loss[r] = loss;
+    }
   }
+}
+template <typename T>
+int lx_rows(const LxArgs& a, hipStream_t st) {
+  const int64_t blocks = ceil_div<int64_t>(a.n, 4);
+  hipLaunchKernelGGL(k_lx_rows<T>, dim3((unsigned)(blocks > 65536 ? 65536 : blocks)), dim3(256), 0, st, a);
+  PG_LAUNCH_CHECK();
+  return PG_OK;
 }
 
 // one block, fixed order: the loss (mean or sum) and meta = 1 / counted rows
@@ -529,6 +536,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dw(LxArgs a) {
 }
 
 inline int64_t up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads < (int64_t(1) << 32); }
 
 // tile shapes (BM x BN): one workgroup of 256 x 256 tiles fills a CU's LDS or registers, two of the others do
 enum { BIG = 0, TALL = 1, MID = 2 };
@@ -546,6 +554,7 @@ struct LxPlan {
   int32_t nx_stats, nx_dh, nx_dw;           // splits
   int64_t rs_stats, rs_dh, rs_dw;           // their ranges
   int64_t classes_p, rows_p, side_bytes;
+  bool fits;                                // every launch has fewer than 2^32 threads
 };
 
 // splits of the narrow form's y for t tiles of x: every CU gets the same number of workgroups, or nearly, and at least two of them
@@ -588,6 +597,8 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
     p.part_bytes = up(n * p.nx_stats * 8, 256);
     p.acc_dh = p.nx_dh > 1 ? up((int64_t)p.nx_dh * n * K * 4, 256) : 0;
     p.acc_dw = p.nx_dw > 1 ? up((int64_t)p.nx_dw * C * (K + 1) * 4, 256) : 0;
+    p.fits = backward ? launchable(ceil_div<int64_t>(n, p.xt_grad) * p.nx_dh, 256) && launchable(ceil_div<int64_t>(C, p.xt_grad) * p.nx_dw, 256)
+                      : launchable(ceil_div<int64_t>(n, p.xt_stats) * p.nx_stats, 256);
     return p;
   }
   // 256 x 256 tiles need a quarter less LDS traffic and two thirds of the loads of 128 x 128 ones, and fill the card from 256 tiles
@@ -616,6 +627,7 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
   // round of 256 x 256 tiles. For the same product 256 x 128 tiles take 1.13 times as long as those and 128 x 128 ones 1.31 times
   // (bf16 8192 x 1024 -> 65536 gradients 2069, 2342, 2714 us; fp32 4096 x 1024 -> 16384 1474, 1662, 1943), but they leave less of
   // the card idle: bf16 3000 x 300 -> 40000 with gradients 538 us with 256 x 256 alone, 494 so; fp16 777 x 602 -> 1153 165, 143
+  p.fits = launchable((backward ? ceil_div<int64_t>(p.piece, big ? 256 : 128) : p.tiles) * p.row_tiles, p.logits == BIG ? 512 : 256);
   auto split = [&](int64_t rows, int64_t len, int* shape, int32_t* s, int64_t* range) {
     const struct { int64_t bm, bn, slots; double unit; } shapes[] = {{256, 256, 256, 1.}, {256, 128, 512, 1.13}, {128, 128, 512, 0.65}};
     // a split's partial result, written and read at 5 TB/s, in units of a round
@@ -630,6 +642,8 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
     }
     *range = up(ceil_div<int64_t>(len, *s), kPad);
     *s = (int32_t)ceil_div<int64_t>(len, *range);
+    if (backward)
+      p.fits = p.fits && launchable(ceil_div<int64_t>(rows, shapes[*shape].bm) * ceil_div<int64_t>(K, shapes[*shape].bn) * *s, *shape == BIG ? 512 : 256);
   };
   split(n, p.piece, &p.dh, &p.dh_splits, &p.dh_range);
   split(p.piece, up(n, kPad), &p.dw, &p.dw_splits, &p.dw_range);
@@ -733,9 +747,7 @@ int narrow_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, c
   rc = launch_narrow<T, NX_STATS>(n, p, st);
   if (rc != PG_OK) return rc;
   a.tiles = p.nx_stats;
-  hipLaunchKernelGGL(k_lx_rows<T>, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
-  PG_LAUNCH_CHECK();
-  return PG_OK;
+  return lx_rows<T>(a, st);
 }
 
 template <typename T>
@@ -801,9 +813,7 @@ int lx_forward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char*
   const dim3 grid((unsigned)(p.tiles * p.row_tiles));
   lx_launch_logits<T, false>(a, p, grid, st);
   PG_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_lx_rows<T>, dim3((unsigned)ceil_div<int64_t>(a.n, 4)), dim3(256), 0, st, a);
-  PG_LAUNCH_CHECK();
-  return PG_OK;
+  return lx_rows<T>(a, st);
 }
 
 template <typename T, typename S>
@@ -893,7 +903,7 @@ int lx_backward(LxArgs& a, const pg_linear_xent_desc_t* d, const LxPlan& p, char
                     SumArgs{acc_dw, p.dw_splits > 1 && p.pieces == 1 ? a.dw : nullptr, a.C * a.K, p.dw_splits}, a, st);
 }
 
-// the grids are one-dimensional, and a tile's offsets have 32 bits
+// a tile's offsets have 32 bits (that the launches fit their grids: LxPlan::fits)
 inline int lx_check(int64_t n, int64_t K, int64_t C, int32_t dtype) {
   if (n < 0 || K <= 0 || C <= 0 || dtype < PG_DTYPE_F32 || dtype > PG_DTYPE_F16) return PG_ERR_INVALID;
   if (n > (int64_t(1) << 31) || K > (int64_t(1) << 20) || C > (int64_t(1) << 31)) return PG_ERR_UNSUPPORTED;
@@ -924,6 +934,7 @@ int64_t pg_linear_xent_scratch(int64_t n, int64_t K, int64_t C, int32_t dtype, i
   if (lx_check(n, K, C, dtype) != PG_OK) return -1;
   if (n == 0) return 0;
   const LxPlan p = lx_plan(n, K, C, dtype, backward != 0);
+  if (!p.fits) return -1;
   const int64_t ops = p.h_bytes + p.w_bytes + p.side_bytes;
   return backward ? p.g_bytes + p.acc_dh + p.acc_dw + p.dbp_bytes + ops + up(4 * n, 256) + 256 : p.part_bytes + 2 * up(4 * n, 256) + ops;
 }
@@ -938,6 +949,7 @@ int pg_linear_xent_fwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   if (rows ? a.n > 0 && !d->row_loss : !d->loss) return PG_ERR_INVALID;
   if (a.n > 0) {
     const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype, false);
+    if (!p.fits) return PG_ERR_UNSUPPORTED;
     char* s = (char*)d->scratch;
     a.row_loss = rows ? d->row_loss : (float*)s;
     s += up(4 * a.n, 256);
@@ -960,6 +972,7 @@ int pg_linear_xent_bwd(const pg_linear_xent_desc_t* d, pg_stream_t stream) {
   if (a.n == 0) return PG_ERR_INVALID;            // no row, no gradient to compute: the caller's zeros
   hipStream_t st = as_stream(stream);
   const LxPlan p = lx_plan(a.n, a.K, a.C, d->dtype, true);
+  if (!p.fits) return PG_ERR_UNSUPPORTED;
   char* s = (char*)d->scratch;
   a.dh = d->dh; a.dw = d->dW; a.db = d->db;
   if (d->reduction == PG_XENT_NONE) {

@@ -1098,11 +1098,13 @@ class _LinearCrossEntropy(torch.autograd.Function):
         n, K, C = rows.size(0), rows.size(1), weight.size(0)
         dev, t = h.device, _DTYPES[h.dtype]
         each = reduction == L.PG_XENT_NONE
+        grad = _needs_grad(ctx)
+        grad = grad[0] or grad[1] or grad[2]
+        size, ctx.scratch = (L.load().pg_linear_xent_scratch(n, K, C, t, k) if k == 0 or grad else 0 for k in (0, 1))
+        if size < 0 or ctx.scratch < 0:
+            raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
         loss = torch.empty(h.shape[:-1] if each else (), dtype=torch.float32, device=dev)
         stats = torch.empty(2 * n + 1, dtype=torch.float32, device=dev)           # largest logits | sums | 1 / #counted
-        size = L.load().pg_linear_xent_scratch(n, K, C, t, 0)
-        if size < 0:
-            raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)
         at, out = stats.data_ptr(), loss.data_ptr()
         _enqueue("pg_linear_xent_fwd", dev, _XENT_DESC(
@@ -1110,9 +1112,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             at + 8 * n, 0, 0, 0, 0, scratch.data_ptr(), n, K, C, _row_stride(rows), _row_stride(weight), 0, ignore_index, t, reduction))
         ctx.save_for_backward(h, weight, bias, labels)
         ctx.stats, ctx.ignore_index, ctx.reduction = stats, ignore_index, reduction
-        grad = _needs_grad(ctx)
-        if grad[0] or grad[1] or grad[2]:
-            ctx.scratch = L.load().pg_linear_xent_scratch(n, K, C, t, 1)
+        if grad:
             _watch_graph("linear_cross_entropy", ctx, dev, h, weight, bias)
         return loss
 

@@ -203,3 +203,37 @@ def test_fp32_infinities_stay_with_their_rows(dev, hiplib, K):
         out.append((each.detach(), torch.autograd.grad(each.sum(), x)[0]))
     assert all(torch.equal(a[rest], b[rest]) for a, b in zip(*out))
     assert torch.isnan(out[1][0][~rest]).all() and torch.isnan(out[1][1][~rest]).all()
+
+
+# ---- sizes that no launch fits, and those that need more than one round of it -----------------------------------------------------
+def test_sizes_beyond_a_launch_are_refused_before_anything_is_allocated(hiplib):
+    """a launch has fewer than 2^32 threads: what needs more is refused by the call that sizes the workspace"""
+    from pagraph_amd import _lib as L
+    scratch = hiplib.pg_linear_xent_scratch
+    for back in (0, 1):
+        # logits: tiles of 256 x 128 and 256 threads, of 256 x 256 and 512 threads; a piece of the classes at a time for gradients
+        assert scratch(1 << 20, 512, 1 << 18, L.PG_DTYPE_BF16, back) > 0
+        assert scratch(1 << 18, 1024, 1 << 20, L.PG_DTYPE_BF16, back) > 0
+        assert (scratch(1 << 20, 512, 1 << 20, L.PG_DTYPE_BF16, back) < 0) == (back == 0)
+        assert (scratch(1 << 22, 1024, 1 << 17, L.PG_DTYPE_BF16, back) < 0) == (back == 0)
+        # narrow: 128 rows and 256 threads a workgroup
+        assert scratch((1 << 31) - 128, 64, 61, L.PG_DTYPE_F32, back) > 0
+        assert scratch(1 << 31, 64, 61, L.PG_DTYPE_F32, back) < 0
+    # dh's tiles: 4 to each 256 rows, of 512 threads
+    assert scratch(1 << 28, 1024, 128, L.PG_DTYPE_BF16, 1) > 0 and scratch(1 << 30, 1024, 128, L.PG_DTYPE_BF16, 1) < 0
+
+
+@gpu
+@pytest.mark.parametrize("t", [F32, F16])
+def test_more_rows_than_workgroups_of_a_launch(dev, hiplib, t):
+    """the joining of the rows' statistics goes round its grid: 262144 rows at a time"""
+    from pagraph_amd import ops
+    g = gen(77, dev)
+    n, K, C = 600001, 16, 61
+    lin = head(dev, K, C, t, g)
+    h = torch.randn(n, K, generator=g, device=dev).to(t)
+    lab = torch.randint(0, C, (n,), generator=g, device=dev)
+    with torch.no_grad():
+        each = ops.linear_cross_entropy(h, lin, lab, reduction="none")
+        parts = [ops.linear_cross_entropy(h[i:i + 200000], lin, lab[i:i + 200000], reduction="none") for i in range(0, n, 200000)]
+    assert (each - torch.cat(parts)).abs().max() <= 64 * 2.0 ** -24 * each.abs().max()
