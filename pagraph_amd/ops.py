@@ -2,6 +2,7 @@
 import ctypes
 import os
 import struct
+import threading
 import weakref
 
 import torch
@@ -923,7 +924,7 @@ def _once(name):
 # graphs of these operators that were recorded outside a capture and still live: their leaves' gradient accumulators belong to the
 # stream they were recorded on. A backward pass captured on another stream would make autograd wait across the capture's border,
 # which ends the process; the forward inside the capture is refused instead.
-_EAGER_GRAPHS = weakref.WeakSet()
+_EAGER_GRAPHS, _EAGER_LOCK = weakref.WeakSet(), threading.Lock()
 
 
 def _capture_state(device):
@@ -932,10 +933,12 @@ def _capture_state(device):
 
 def _watch_graph(name, ctx, device, *inputs):
     capturing, ctx.stream = _capture_state(device)
-    if not capturing:
-        _EAGER_GRAPHS.add(ctx)
-        return
-    for other in list(_EAGER_GRAPHS):
+    with _EAGER_LOCK:                                # (another thread may record a graph at any moment)
+        if not capturing:
+            _EAGER_GRAPHS.add(ctx)
+            return
+        others = list(_EAGER_GRAPHS)
+    for other in others:
         if other.stream != ctx.stream:
             for fn, _ in other.next_functions:
                 leaf = getattr(fn, "variable", None)

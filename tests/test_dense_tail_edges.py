@@ -237,3 +237,55 @@ def test_more_rows_than_workgroups_of_a_launch(dev, hiplib, t):
         each = ops.linear_cross_entropy(h, lin, lab, reduction="none")
         parts = [ops.linear_cross_entropy(h[i:i + 200000], lin, lab[i:i + 200000], reduction="none") for i in range(0, n, 200000)]
     assert (each - torch.cat(parts)).abs().max() <= 64 * 2.0 ** -24 * each.abs().max()
+
+
+# ---- graphs that live beside a capture -------------------------------------------------------------------------------------------
+@pytest.fixture
+def watched(monkeypatch):
+    """an operator that ops._watch_graph watches, without a GPU: whether its stream captures, and which it is, are made up"""
+    from pagraph_amd import ops
+    state = {"capturing": False, "stream": 1}
+    monkeypatch.setattr(ops, "_capture_state", lambda device: (state["capturing"], state["stream"]))
+    monkeypatch.setattr(ops, "_EAGER_GRAPHS", type(ops._EAGER_GRAPHS)())
+
+    class F(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            ops._watch_graph("f", ctx, x.device, x, w)
+            return x * w
+
+        @staticmethod
+        def backward(ctx, g):
+            return g, g
+    return F, state
+
+
+def test_graphs_are_recorded_by_other_threads_during_a_capture(watched, monkeypatch):
+    """another thread's eager graph comes in while a capture goes through those that live"""
+    import threading
+    from pagraph_amd import ops
+    F, state = watched
+    kept, others = [], []
+
+    def record():
+        kept.append(F.apply(torch.ones(3, requires_grad=True), torch.ones(3)))
+
+    class Interrupted(type(ops._EAGER_GRAPHS)):
+        def __iter__(self):
+            graphs = super().__iter__()
+            for graph in graphs:
+                yield graph
+                others.append(threading.Thread(target=record))
+                others[-1].start()
+                others[-1].join(0.3)                 # (comes in now, or waits until the capture is through them)
+    monkeypatch.setattr(ops, "_EAGER_GRAPHS", Interrupted())
+    here = threading.get_ident()
+    monkeypatch.setattr(ops, "_capture_state", lambda device: (state["capturing"] and threading.get_ident() == here, state["stream"]))
+    for _ in range(3):
+        record()
+    state.update(capturing=True, stream=2)
+    u = torch.ones(3, requires_grad=True)
+    F.apply(u, u)
+    for other in others:
+        other.join()
+    assert len(kept) == 6
