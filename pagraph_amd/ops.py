@@ -921,14 +921,29 @@ def _once(name):
         raise L.PgError(f"{name}: a gradient's own graph (create_graph=True) is not supported")
 
 
-# graphs of these operators that were recorded outside a capture and still live: their leaves' gradient accumulators belong to the
-# stream they were recorded on. A backward pass captured on another stream would make autograd wait across the capture's border,
-# which ends the process; the forward inside the capture is refused instead.
+# graphs of these operators that were recorded outside a capture and still live: their leaves' gradient accumulators, also of leaves
+# far behind them, belong to the stream they were recorded on. A backward pass captured on another stream would make autograd wait
+# across the capture's border, which ends the process; the forward inside the capture is refused instead.
 _EAGER_GRAPHS, _EAGER_LOCK = weakref.WeakSet(), threading.Lock()
 
 
 def _capture_state(device):
     return torch._C._cuda_isCurrentStreamCapturing(), torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _leaves(nodes):
+    """the leaves whose gradients a backward pass through `nodes` reaches, by id (None: an input without a gradient)"""
+    seen, leaves = set(), {}
+    while nodes:
+        fn = nodes.pop()
+        if fn is None or fn in seen:
+            continue
+        seen.add(fn)
+        leaf = getattr(fn, "variable", None)
+        if leaf is not None:
+            leaves[id(leaf)] = leaf
+        nodes.extend(behind for behind, _ in fn.next_functions)
+    return leaves
 
 
 def _watch_graph(name, ctx, device, *inputs):
@@ -937,14 +952,14 @@ def _watch_graph(name, ctx, device, *inputs):
         if not capturing:
             _EAGER_GRAPHS.add(ctx)
             return
-        others = list(_EAGER_GRAPHS)
-    for other in others:
-        if other.stream != ctx.stream:
-            for fn, _ in other.next_functions:
-                leaf = getattr(fn, "variable", None)
-                if leaf is not None and any(leaf is t for t in inputs):
-                    raise L.PgError(f"{name}: this capture's gradients would meet those of a graph that was recorded on another stream "
-                                    "and is still alive (a loss kept from an eager step?): drop it before the capture")
+        others = [other for other in _EAGER_GRAPHS if other.stream != ctx.stream]
+    if not others:
+        return
+    mine = _leaves([t.grad_fn for t in inputs if t is not None])
+    mine.update((id(t), t) for t in inputs if t is not None and t.is_leaf and t.requires_grad)
+    if not mine.keys().isdisjoint(_leaves([fn for other in others for fn, _ in other.next_functions])):
+        raise L.PgError(f"{name}: this capture's gradients would meet those of a graph that was recorded on another stream "
+                        "and is still alive (a loss kept from an eager step?): drop it before the capture")
 
 
 def _drop_fields(spec, step_used=0):

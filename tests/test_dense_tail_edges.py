@@ -260,6 +260,25 @@ def watched(monkeypatch):
     return F, state
 
 
+def test_a_capture_meets_no_living_graph_of_leaves_behind_its_inputs(watched):
+    from pagraph_amd import _lib
+    F, state = watched
+    x, w, u, v = (torch.ones(3, requires_grad=True) for _ in range(4))
+    fixed = torch.ones(3)
+    kept = F.apply(torch.relu(x * w), fixed) + 1.0
+    state.update(capturing=True, stream=2)
+    F.apply(torch.tanh(u) * v, v)                            # other leaves
+    F.apply(fixed, u)
+    for f in (lambda: F.apply(torch.tanh(u * w), v), lambda: F.apply(u, (x + v) * 2.0), lambda: F.apply(w, fixed)):
+        with pytest.raises(_lib.PgError, match="still alive"):
+            f()
+    state.update(stream=1)
+    F.apply(torch.tanh(u * w), v)                            # the stream the graph was recorded on
+    state.update(stream=2)
+    del kept
+    F.apply(torch.tanh(u * w), v)
+
+
 def test_graphs_are_recorded_by_other_threads_during_a_capture(watched, monkeypatch):
     """another thread's eager graph comes in while a capture goes through those that live"""
     import threading
