@@ -148,7 +148,7 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
     }
     float sv[16];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 4 && MODE != NX_DW; ++q) {
       const float4 v = *reinterpret_cast<const float4*>(side + yb * 32 + 8 * q + h4);
       sv[4 * q] = v.x; sv[4 * q + 1] = v.y; sv[4 * q + 2] = v.z; sv[4 * q + 3] = v.w;
     }
@@ -184,12 +184,14 @@ __device__ __forceinline__ void nx_step(const short* __restrict__ cur, const flo
           }
         } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4 v = *reinterpret_cast<const float4*>(side + 128 + yb * 32 + 8 * q + h4);
-            const float inv[4] = {v.x, v.y, v.z, v.w};
+          for (int q = 0; q < 4; ++q) {            // (four rows' values at a time: the registers are full)
+            const float4 t4 = *reinterpret_cast<const float4*>(side + yb * 32 + 8 * q + h4);
+            const float4 i4 = *reinterpret_cast<const float4*>(side + 128 + yb * 32 + 8 * q + h4);
+            const float top[4] = {t4.x, t4.y, t4.z, t4.w}, inv[4] = {i4.x, i4.y, i4.z, i4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              z[b][4 * q + e] = lx_exp(fmaf(z[b][4 * q + e], L2E, st.xa[b]) - sv[4 * q + e]) * inv[e];
+              z[b][4 * q + e] = lx_exp(fmaf(z[b][4 * q + e], L2E, st.xa[b]) - top[e]) * inv[e];
+            __builtin_amdgcn_sched_barrier(0);
           }
           // the wave's classes are 32 in a row: does any of the block's rows have one of them as its label?
           const int* lab = reinterpret_cast<const int*>(side + 64) + yb * 32;
@@ -237,8 +239,9 @@ __device__ __forceinline__ void next_tile() {
   __syncthreads();
 }
 
+// (fp32 of 64 columns: within the registers of a third workgroup on the CU)
 template <typename T, int KP, int XB, int MODE>
-__global__ __launch_bounds__(256, 2) void k_lx_narrow(NxArgs a) {
+__global__ __launch_bounds__(256, Mul<T>::NP == 3 && KP == 64 ? 3 : 2) void k_lx_narrow(NxArgs a) {
   typedef Narrow<T, KP, XB> N;
   __shared__ __align__(16) short buf[2 * N::TILE];
   __shared__ __align__(16) float side[2 * 256];
