@@ -109,8 +109,9 @@ __device__ __forceinline__ void drop_piece(float (&v)[4 * V], const UnitMask (&m
   }
 }
 
+// (y may be x: a thread has read its unit before it writes it)
 template <typename T, int V, bool RAGGED>
-__global__ __launch_bounds__(256) void k_dropout(const T* __restrict__ x, int64_t xs, T* __restrict__ y, int64_t ys, int64_t n, int d,
+__global__ __launch_bounds__(256) void k_dropout(const T* x, int64_t xs, T* y, int64_t ys, int64_t n, int d,
                                                  int units, int rows_per_block, float inv_units, DropArgs dr, uint64_t* step_used) {
   const uint32_t step = drop_step_of(dr);
   if (step_used && blockIdx.x == 0 && threadIdx.x == 0) *step_used = step;

@@ -4,7 +4,7 @@ test_dense_tail.py: one rounding of the result, plus the fp32 roundings on the w
 import pytest
 import torch
 
-from test_dense_tail import BF16, F16, F32, gen, gpu, head
+from test_dense_tail import BF16, F16, F32, Tail, check_xent, gen, gpu, head, mask_of, spec_of, tail_reference
 
 TYPES = pytest.mark.parametrize("t", [F32, BF16, F16])
 
@@ -308,3 +308,21 @@ def test_graphs_are_recorded_by_other_threads_during_a_capture(watched, monkeypa
     for other in others:
         other.join()
     assert len(kept) == 6
+
+
+# ---- dropout where it reads ---------------------------------------------------------------------------------------------------
+@gpu
+@TYPES
+@pytest.mark.parametrize("n,d", [(1, 3), (50, 64), (333, 602), (7, 2048), (2, 9001)])
+def test_dropout_in_place(dev, hiplib, n, d, t):
+    """pg_dropout_apply may write where it reads"""
+    import ctypes
+    from pagraph_amd import _lib as L
+    from pagraph_amd import ops
+    spec = spec_of(dev, 0.4)
+    x = torch.randn(n, d, generator=gen(78, dev), device=dev).to(t)
+    want = ops.dropout(x, spec)
+    drop = L.PgDropout(spec.threshold, spec.tag, spec.seed, spec.step.data_ptr(), 0)
+    L.check(hiplib.pg_dropout_apply(x.data_ptr(), d, x.data_ptr(), d, n, d, ops._DTYPES[t], ctypes.addressof(drop), None, L.stream_ptr()),
+            "pg_dropout_apply")
+    assert torch.equal(x, want)
