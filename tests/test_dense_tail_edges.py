@@ -326,3 +326,97 @@ def test_dropout_in_place(dev, hiplib, n, d, t):
     L.check(hiplib.pg_dropout_apply(x.data_ptr(), d, x.data_ptr(), d, n, d, ops._DTYPES[t], ctypes.addressof(drop), None, L.stream_ptr()),
             "pg_dropout_apply")
     assert torch.equal(x, want)
+
+
+# ---- the parts of fp32 products ----------------------------------------------------------------------------------------------------
+# values whose bf16 parts are (1, 0, 0), (1, 2^-8, 0) and (1, 2^-9, 2^-17)
+PARTS = (1.0, 1.0 + 2.0 ** -8, 1.0 + 2.0 ** -9 + 2.0 ** -17)
+
+
+def three_parts(x):
+    parts = []
+    for _ in range(3):
+        parts.append(torch.tensor(x, dtype=torch.float64).to(BF16).double().item())
+        x -= parts[-1]
+    return parts, x
+
+
+def test_the_parts_are_what_they_are_taken_for():
+    assert [three_parts(x) for x in PARTS] == [([1.0, 0.0, 0.0], 0.0), ([1.0, 2.0 ** -8, 0.0], 0.0), ([1.0, 2.0 ** -9, 2.0 ** -17], 0.0)]
+
+
+@gpu
+@pytest.mark.parametrize("n,K,C", [(2, 1, 2), (2, 100, 2), (300, 128, 3000), (2, 300, 2), (2100, 300, 7000), (5000, 1030, 9000), (300, 1030, 70000)])
+def test_fp32_products_keep_every_part_that_is_not_below_2_to_the_minus_23(dev, hiplib, n, K, C):
+    """logits of +-1024 in one row and two classes (the others masked, the other rows not counted, but one with a gradient of its own),
+    so that loss, dh and dW are single products of values whose parts are known. A product that lacked one of its six would be off
+    by 2^-16 (middle times middle) or 2^-17 (lowest times first, either way round)"""
+    from pagraph_amd import ops
+    lin = torch.nn.Linear(K, C, device=dev)
+    h = torch.zeros(n, K, device=dev, requires_grad=True)
+    lab = torch.full((n,), -100, dtype=torch.int64, device=dev)
+    up = torch.zeros(n, device=dev)
+    row, other, one, two, col = n - 1, 0, 0, C - 1, K - 1
+    lab[other], lab[row] = one, two
+    with torch.no_grad():
+        lin.weight.zero_()
+        lin.bias.fill_(float("-inf"))
+        lin.bias[one], lin.bias[two] = 0.0, 0.0
+    for x in PARTS:
+        for y in PARTS:
+            for f in PARTS:
+                with torch.no_grad():
+                    h[row, col] = 32.0 * x
+                    lin.weight[one, col], lin.weight[two, col] = 32.0 * y, -32.0 * y
+                up[other], up[row] = 1.0, 0.5 * f
+                each = ops.linear_cross_entropy(h, lin, lab, reduction="none")
+                dh, dw, db = torch.autograd.grad(each, [h, lin.weight, lin.bias], up)
+                # the three products left out are below 2^-22.9; six partial sums, into base 2 and out of it: 2^-24 each. (the gradients:
+                # the factors' quotient and product, G's own roundings)
+                off = 2.0 ** -22.9 + 12 * 2.0 ** -24
+                for got, want in ((each[row], 2048.0 * x * y), (dh[row, col], 32.0 * y * f), (dw[one, col], 16.0 * x * f), (dw[two, col], -16.0 * x * f)):
+                    assert abs(got.item() - want) <= off * abs(want), (x, y, f, got.item(), want)
+                # (the other row: two equal logits)
+                assert abs(db[one].item() - (0.5 * f - 0.5)) <= off and abs(db[two].item() - (0.5 - 0.5 * f)) <= off
+                assert abs(each[other].item() - 0.6931471805599453) <= off
+
+
+# ---- forms that a rule on sizes chooses ---------------------------------------------------------------------------------------------
+@gpu
+@TYPES
+@pytest.mark.parametrize("n,K,C", [(2100, 300, 7000), (4099, 1030, 8200)])
+@pytest.mark.parametrize("bias,reduction", [(True, "none"), (False, "none"), (False, "mean"), (False, "sum")])
+def test_large_tiles_with_row_gradients_and_without_a_bias(dev, hiplib, bias, reduction, n, K, C, t):
+    check_xent(dev, n, K, C, t, ignored=0.1, reduction=reduction, bias=bias)
+
+
+@gpu
+def test_gradients_of_the_tail_against_differences_along_them(dev, hiplib, oracle):
+    """the losses' own differences along each gradient, where they are largest. In 64 bits, how far a difference is from the derivative;
+    the kernels' losses are off by some 300 roundings one behind the other (two layers of depth <= 64, the row sums of 230 and 90), on
+    either side. Both together are well below the gradient: zeros, or the wrong sign, would not pass"""
+    g = gen(79, dev)
+    n, d, C = 90, 60, 230
+    m = Tail(d, C, dev)
+    x = torch.randn(n, d, generator=g, device=dev, requires_grad=True)
+    lab = torch.randint(0, C, (n,), generator=g, device=dev)
+    lab[::11] = -100
+    s1, s2 = spec_of(dev, 0.2, tag=1), spec_of(dev, 0.4, tag=2)
+    k1, k2 = [(lambda km: km[0].to(dev).double() * km[1])(mask_of(oracle, n, d, s, 5)) for s in (s1, s2)]
+    leaves = [x] + list(m.parameters())
+    grads = torch.autograd.grad(m(x, lab, s1, s2), leaves)
+    loss, exact = tail_reference(m, x, lab, k1, k2)
+    with torch.no_grad():
+        for p, gp, ge in zip(leaves, grads, exact):
+            size = ge.norm().item()
+            v, old, e, both = (ge / size).float(), p.detach().clone(), 5e-2, []
+            for sign in (e, -e):
+                p.copy_(old + sign * v)
+                with torch.enable_grad():
+                    both.append((m(x, lab, s1, s2).item(), tail_reference(m, x, lab, k1, k2)[0].item()))
+            p.copy_(old)
+            here, there = [(a - b) / (2 * e) for a, b in zip(*both)]
+            along = (gp.double() * v.double()).sum().item()
+            bound = abs(there - size) + 300 * 2.0 ** -24 * loss.item() / e
+            assert bound < 0.25 * size, (p.shape, bound, size)
+            assert abs(here - along) <= bound, (p.shape, here, along, bound)
