@@ -637,7 +637,8 @@ int pg_layer_norm_bwd(const pg_norm_desc_t* desc, pg_stream_t stream);
  *           counted); meta [1] = 1 / #counted rows (0).
  * backward: given the forward's top, sum, meta and grad = d objective / d loss (device fp32: one value for PG_XENT_MEAN / _SUM,
  *           [n] with grad_stride for PG_XENT_NONE): dh [n, K], dW [C, K], db [C], dense, each may be NULL. n >= 1.
- * scratch: pg_linear_xent_scratch(n, K, C, dtype, backward) bytes (negative: the sizes are refused). Deterministic.           */
+ * scratch: pg_linear_xent_scratch(n, K, C, dtype, backward) bytes (negative: the sizes are refused), 16-byte aligned. It holds
+ * statistics of 8 bytes for each row and 128 or 256 classes. Deterministic.                                                  */
 #define PG_XENT_MEAN 0
 #define PG_XENT_SUM 1
 #define PG_XENT_NONE 2

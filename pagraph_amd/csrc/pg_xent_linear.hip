@@ -917,6 +917,7 @@ int lx_args(const pg_linear_xent_desc_t* d, LxArgs* a) {
   if (rc != PG_OK) return rc;
   if ((d->h_stride < d->K && d->h_stride != 0) || d->w_stride < d->K) return PG_ERR_INVALID;
   if (!d->W || !d->meta || (d->n > 0 && (!d->h || !d->labels || !d->top || !d->sum || !d->scratch))) return PG_ERR_INVALID;
+  if ((uintptr_t)d->scratch % 16) return PG_ERR_INVALID;            // packed rows and G move 16 bytes a lane
   *a = LxArgs{};
   a->bias = d->bias; a->labels = d->labels;
   a->n = d->n; a->K = d->K; a->Kp = up(d->K, kPad); a->C = d->C; a->ignore = d->ignore_index;

@@ -223,6 +223,18 @@ def test_sizes_beyond_a_launch_are_refused_before_anything_is_allocated(hiplib):
     assert scratch(1 << 28, 1024, 128, L.PG_DTYPE_BF16, 1) > 0 and scratch(1 << 30, 1024, 128, L.PG_DTYPE_BF16, 1) < 0
 
 
+def test_a_workspace_that_is_not_aligned_is_refused(hiplib):
+    import ctypes
+    from pagraph_amd import _lib as L
+    x = L.PgLinearXentDesc()
+    for name in ("h", "W", "labels", "top", "sum", "row_loss", "loss", "meta", "grad", "dh", "dW", "db"):
+        setattr(x, name, 4096)                       # (never looked at)
+    x.n, x.K, x.C, x.h_stride, x.w_stride = 4, 8, 8, 8, 8
+    for scratch in (4100, 4104, 4097):
+        x.scratch = scratch
+        assert hiplib.pg_linear_xent_fwd(ctypes.addressof(x), None) == hiplib.pg_linear_xent_bwd(ctypes.addressof(x), None) == -1
+
+
 @gpu
 @pytest.mark.parametrize("t", [F32, F16])
 def test_more_rows_than_workgroups_of_a_launch(dev, hiplib, t):
