@@ -924,7 +924,7 @@ def _once(name):
 # graphs of these operators that were recorded outside a capture and still live: their leaves' gradient accumulators, also of leaves
 # far behind them, belong to the stream they were recorded on. A backward pass captured on another stream would make autograd wait
 # across the capture's border, which ends the process; the forward inside the capture is refused instead.
-_EAGER_GRAPHS, _EAGER_LOCK = weakref.WeakSet(), threading.Lock()
+_EAGER_GRAPHS, _EAGER_LOCK = weakref.WeakSet(), threading.RLock()      # (a collector may record one inside it)
 
 
 def _capture_state(device):
