@@ -4,8 +4,8 @@
 // function of (row, column, seed, tag, step), is never stored, and is the one the fused aggregations draw for the same row — the
 // backward pass draws it again. One Philox4x32-10 call makes eight 16-bit words: the columns 4p..4p+3 and 4p+256..4p+259 of one
 // row, so a thread owns those eight columns ("a pair of pieces") and no word is drawn twice. Ten rounds of two 32x32 products are
-// what the ALU pays; the bound is HBM (each element read once, written once): 16384 x 2048 bf16 26 us = 5.1 TB/s, 6000 x 602 fp32
-// 8.2 us = 3.5 TB/s (rows of no whole 16-byte pieces).
+// what the ALU pays; the bound is HBM (each element read once, written once): 16384 x 2048 bf16 26.6 us = 5.0 TB/s, 6000 x 602 fp32
+// 7.3 us = 4.0 TB/s (rows of no whole 16-byte pieces; six inputs in turn, 8.2 us under a profiler).
 //
 // Layer norm: s = dropout(x) + residual, y = (s - mean) * rstd * w + b, biased variance. A row lives in the registers of G lanes
 // (S pairs of pieces each), so mean and variance are two exact passes over registers and the row is read once. Backward:
@@ -13,7 +13,8 @@
 // in one pass over (gy, s, gs); dw = sum_r gy * xh and db = sum_r gy accumulate in registers over the rows a group walks, are
 // added up inside the workgroup and leave as one partial row per workgroup, which a second launch sums in a fixed order
 // (deterministic: no atomics). Bound: HBM: 16384 x 2048 bf16 with dropout and residual forward 58 us = 4.6 TB/s, backward 68 to 73 us
-// = 4.6 to 4.9 TB/s; 6000 x 602 fp32 with residual 13 and 17 us. Rows above 8192 columns spill in the backward pass.
+// = 4.6 to 4.9 TB/s; 6000 x 602 fp32 with residual 14 us = 4.1 TB/s, and 19.5 us = 3.0 TB/s with 4.8 more for the partial rows: the
+// fp32 backward pass reads no row ahead, and its 87 units stand on 128 places of two a lane. Rows above 8192 columns spill there.
 #include "pg_elem.h"
 
 namespace pg {
@@ -506,8 +507,9 @@ inline int norm_lanes(int64_t d, int v) {
 }
 
 // workgroups of the backward pass: each leaves one partial row of 2 d floats, so each walks 8 rows at least, which keeps that
-// traffic to a tenth of the rows' own. At most the three a CU holds at once (registers): a second, partly filled round of them
-// took as long as the first (1024 workgroups 117 us, 768 89 us at 16384 x 2048 bf16 with dropout and residual, before rows were kept as read)
+// traffic to a tenth of the rows' own. At most the three of 256 threads that a CU holds at once (registers): a second, partly filled round
+// of them took as long as the first (1024 workgroups 117 us, 768 89 us at 16384 x 2048 bf16 with dropout and residual, before rows were
+// kept as read). Of 512 and 1024 threads a CU holds one, and 768 workgroups are three rounds
 inline int64_t norm_bwd_blocks(int64_t n, int64_t d, int32_t dtype) {
   const int g = norm_lanes(d, norm_v(d, dtype)), rpb = g >= 256 ? 1 : 256 / g;
   const int64_t rows = rpb > 8 ? rpb : 8, b = ceil_div<int64_t>(n, rows);
@@ -554,8 +556,9 @@ int dispatch_norm(const NormArgs& a, int64_t bwd, hipStream_t st) {
 
 template <typename T>
 void launch_dropout(const void* x, int64_t xs, void* y, int64_t ys, int64_t n, int64_t d, const DropArgs& dr, uint64_t* used, hipStream_t st) {
-  // one unit a thread where a row has at most 128 of them, two up to 255 (fewer idle threads): with four, too few workgroups for the
-  // card on short batches (6000 x 602 fp32 8.6 against 7.2 us, 65536 x 17 fp16 6.7 against 4.6, 16384 x 2048 bf16 22.2 and 22.4)
+  // one unit a thread where a row has at most 128 of them, up to two below 256 (fewer idle threads): with two everywhere, too few
+  // workgroups for the card on short batches (six inputs in turn: 6000 x 602 fp32 7.8 against 7.3 us, 65536 x 17 fp16 4.7 against 4.1;
+  // 16384 x 2048 bf16, which fills it either way, 25.4 against 26.6)
   const int v = sizeof(T) == 2 && d % 8 == 0 ? 2 : 1, units = (row_pairs(d) + v - 1) / v;
   const int rows = units >= 256 ? 1 : units > 128 ? 512 / units : 256 / units;
   const int64_t blocks = ceil_div<int64_t>(n, rows);

@@ -14,8 +14,8 @@
 // G of 16-bit operands is held in 16 bits: |G| <= 1 and each element is off by half a step (bf16 2^-8, fp16 2^-11 relative),
 // independently per element, as are the outputs, which leave in the same type. fp16 G is held times 2^14 so that a probability
 // of 2^-28 is still a normal number.
-// Measured at bf16 8192 x 1024 -> 65536 (2 n K C = 1.1 TFLOP a product; the library's 16384^3 product reaches 1.59 PF): statistics
-// 1.02 ms, G 1.23 ms, dh 0.98 ms, dW 0.90 ms, that is 1.08, 0.90, 1.12, 1.22 PF, 4.1 ms with gradients.
+// Measured at bf16 8192 x 1024 -> 65536 (2 n K C = 1.1 TFLOP a product; the library's 16384^3 product reaches 1.47 PF on the same
+// card): statistics 1.09 ms, G 1.32 ms, dh 1.01 ms, dW 0.95 ms, that is 1.01, 0.83, 1.09, 1.15 PF, 4.3 ms with gradients.
 #include "pg_xent_narrow.h"
 
 namespace pg {
@@ -157,7 +157,8 @@ __global__ __launch_bounds__(256) void k_lx_pack(PackArgs a0, PackArgs a1, SideA
 
 // One BM-class x BN-row tile of logits; a lane holds one row's classes in registers: row = 32 j + lane % 32 of its wave's rows,
 // class = 32 i + 8 (e / 4) + 4 (lane / 32) + e % 4 of its wave's classes, so a row's maximum and sum are taken in registers.
-// The tile's exponentials and its LDS trip follow its product, some 8000 cycles behind 33 000 (K = 1024): what bounds it.
+// The tile's exponentials, and G's LDS trip, follow its product: at bf16 8192 x 1024 -> 65536 the statistics take 8 % longer than a
+// product of this size without them (k_lx_dh), G 31 %. The matrix units are busy in 56 and 44 % of the cycles: mm_run bounds both.
 // PIECE: writes G (through LDS: whole 16-byte pieces of rows) and the column sums of the tile, else the tile's row statistics.
 template <typename T, typename S, bool PIECE>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_logits(LxArgs a) {
@@ -414,7 +415,7 @@ __device__ __forceinline__ void each_output(const f32x16 (&acc)[S::FI][S::FJ], i
     }
 }
 
-// G [rows x classes] W: G's rows are read as they stand, W through the transposing reads. Bound by the matrix instructions.
+// G [rows x classes] W: G's rows are read as they stand, W through the transposing reads. Matrix units busy in 59 % of the cycles (mm_run).
 // dh: acc[split][r][k] (+)= sum over the split's classes of G[r][c] W[c][k]
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dh(LxArgs a) {
@@ -508,7 +509,7 @@ int lx_sums(const SumArgs& a, const SumArgs& b, const SumArgs& c, const LxArgs& 
   return PG_OK;
 }
 
-// G^T h, both through the transposing reads (neither is ever transposed in memory). Bound by the matrix instructions.
+// G^T h, both through the transposing reads (neither is ever transposed in memory). Matrix units busy in 59 % of the cycles (mm_run).
 // dW rows of a piece: sum over the split's rows of G[r][c] h[r][k]
 template <typename T, typename S>
 __global__ __launch_bounds__(S::THREADS, 2) void k_lx_dw(LxArgs a) {
@@ -582,8 +583,8 @@ inline LxPlan lx_plan(int64_t n, int64_t K, int64_t C, int32_t dtype, bool backw
   p.classes_p = up(C, 256) + 64;
   p.rows_p = p.h_rows + 64;
   p.side_bytes = up(p.classes_p * 4, 256) + 4 * up(p.rows_p * 4, 256);
-  // (us, narrow against wide. fp32 6000 -> 50000: 64 columns forward 223, 343, with gradients 1109, 2645; 128: 424, 501 and 1963,
-  // 3464. bf16 8192 -> 65536: 128 columns 188, 264 and 775, 1408; 192: 239, 325 and 1001, 1712; 256: forward 269, 390, but the
+  // (us, narrow against wide. fp32 6000 -> 50000: 64 columns forward 223, 343, with gradients 998, 2645; 128: 424, 501 and 1970,
+  // 3464. bf16 8192 -> 65536: 128 columns 188, 264 and 763, 1408; 192: 239, 325 and 1025, 1712; 256: forward 269, 390, but the
   // gradients alone 1652, 1478, since 256 columns of operands and sums do not fit the registers of a wave)
   p.narrow = p.Kp <= (np == 3 ? 128 : backward ? 192 : 256);
   if (p.narrow) {

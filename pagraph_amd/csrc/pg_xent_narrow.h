@@ -12,9 +12,10 @@
 // between lanes, no trip through LDS.
 // 10 n K C operations (2 + 4 + 4) and no G traffic, against 8 n K C and 6 bytes (fp32: 18) per element of [n, C] of the wide form:
 // as long as a wave's registers hold its operand rows and its sums, the traffic costs more than the repeated product.
-// Measured: fp32 6000 x 64 -> 50000 STATS 205, DH 382, DW 400 us (187, 201, 192 TF of fp32 products, 1.1 to 1.2 PF of bf16 ones;
-// the fp32 matrix instructions reach 154 TF); bf16 4096 x 256 -> 32000 STATS 77 us = 0.87 PF. Bound by the matrix instructions and,
-// beside them, the exponentials and the splitting of G, which other waves' products only partly cover.
+// Measured: fp32 6000 x 64 -> 50000 STATS 213, DH 411, DW 439 us (180, 187, 175 TF of fp32 products, 1.0 to 1.1 PF of bf16 ones;
+// the fp32 matrix instructions reach 154 TF), matrix units busy in 60, 63, 53 % of the cycles; bf16 4096 x 256 -> 32000 STATS 79 us =
+// 0.85 PF, 38 %. A wave's products, then its exponentials and the splitting of G, then products again: other waves' products only
+// partly cover what is between.
 // Exponents are kept in base 2: z log2(e) + b log2(e) is one fused multiply-add, and fp16's scale of G, 2^14, rides in the exponent.
 #pragma once
 #include "pg_mm.h"
