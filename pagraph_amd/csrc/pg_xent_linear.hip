@@ -339,7 +339,10 @@ __global__ __launch_bounds__(256) void k_lx_rows(LxArgs a) {
         loss = ((m - z) + log2f(s)) * kLn2;
         // the label's own class is masked by a finite bias that base 2 cannot hold (lx_side), another class is not: beside such a
         // bias h W is lost, the logit is the bias
-        if (z == kLowest && m > kLowest) loss = (m + log2f(s)) * kLn2 - (float)((const T*)a.bias)[a.labels[r]];
+        if (z == kLowest && m > kLowest && a.bias) {
+          const float b = (float)((const T*)a.bias)[a.labels[r]];
+          if (b * kLog2e < kLowest) loss = (m + log2f(s)) * kLn2 - b;
+        }
       }
       a.row_loss[r] = loss;
     }

@@ -91,6 +91,26 @@ def test_a_label_whose_class_is_masked_by_the_lowest_value(dev, hiplib, K, t):
     assert db[107] == -15 and (db[100:107] == 0).all() and (db[108:130] == 0).all()
 
 
+@gpu
+@pytest.mark.parametrize("bias", [True, False])
+def test_a_logit_at_the_lowest_value_in_base_2_that_is_no_mask(dev, hiplib, bias):
+    """h W and the bias together can be what a masked class's bias alone is held as, and there may be no bias at all"""
+    from pagraph_amd import ops
+    product, b = float.fromhex("-0x1.04p+126"), float.fromhex("-0x1.c1c85ep+126")
+    log2e = torch.tensor(1.4426950408889634).double()
+    # one fused multiply-add of the logit times log2(e), as the kernel has it, is the lowest fp32 value
+    assert (product * log2e + (b * log2e).float().double()).float().item() == torch.finfo(F32).min
+    lin = torch.nn.Linear(1, 2, bias=bias, device=dev)
+    with torch.no_grad():
+        lin.weight.copy_(torch.tensor([[1.0], [0.0]]))
+        if bias:
+            lin.bias.copy_(torch.tensor([b, 0.0]))
+    h = torch.full((5, 1), product, device=dev)
+    each = ops.linear_cross_entropy(h, lin, torch.zeros(5, dtype=torch.int64, device=dev), reduction="none")
+    want = -(product + (b if bias else 0.0))
+    assert ((each.double() - want).abs() <= 8 * 2.0 ** -24 * want).all()
+
+
 # ---- infinite weights ----------------------------------------------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("t", [BF16, F16])
