@@ -1118,7 +1118,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         each = reduction == L.PG_XENT_NONE
         grad = _needs_grad(ctx)
         grad = grad[0] or grad[1] or grad[2]
-        size, ctx.scratch = (L.load().pg_linear_xent_scratch(n, K, C, t, k) if k == 0 or grad else 0 for k in (0, 1))
+        size_of = L.load().pg_linear_xent_scratch
+        size, ctx.scratch = size_of(n, K, C, t, 0), size_of(n, K, C, t, 1) if grad else 0
         if size < 0 or ctx.scratch < 0:
             raise L.PgError(f"linear_cross_entropy: {n} rows x {C} classes x {K} columns are not supported")
         loss = torch.empty(h.shape[:-1] if each else (), dtype=torch.float32, device=dev)
